@@ -218,6 +218,113 @@ int b2_attention_blocks_split(int max_seq, int block);
 int b2_attention_blocks(float* out, uint16_t* out16, const float* q, int ldq, int M, int nq, int nkv, int hd,
                         const B2KVRef* kv, void* work, int block, int* err, b2_stream_t s);
 
+/* ─── paged KV cache (no counterpart in the reference) ───
+ * One layer's cache as pages of page_size positions that sequences of any
+ * length share a pool of.  Position (slot) j of sequence q lives in page
+ * page_table[q][j / page_size] at row j % page_size; K of kv head g is the
+ * head_dim FP16 values at
+ *     k_pages + page * page_stride + g * head_stride + row * row_stride
+ * (elements), and V likewise, so pages may be [head][position][dim] (head_stride
+ * = page_size * head_dim, row_stride = head_dim) or [position][head][dim], and
+ * K, V and layers may interleave in one pool.  A table entry outside
+ * [0, n_pages) is an unmapped page: its slots are never written, read or
+ * attended (pages behind a sliding window, say).
+ *
+ * A batch brings new rows for its sequences: rows [q_start[q], q_start[q+1])
+ * of the row arrays (M rows in all) are sequence q's newest positions, so row
+ * i of them has slot kv_len[q] - Q + i with Q = q_start[q+1] - q_start[q].  Q may
+ * be 0 (an idle sequence), 1 (a decode step) or a whole prompt.  Rows from
+ * q_start[n_seqs] on belong to nobody and are left as they are.  kv_len counts
+ * the new rows.  q_start must not decrease.
+ *
+ * k_pages and v_pages 16-byte aligned, strides multiples of 8 elements, the
+ * strides below 2^39 elements; page_size 16, 32, 64 or 128; n_seqs <=
+ * B2_PAGED_MAX_SEQS; head_dim 64 or 128. */
+#define B2_PAGED_MAX_SEQS 1024
+typedef struct {
+    uint16_t* k_pages;
+    uint16_t* v_pages;
+    long long page_stride;
+    long long head_stride;
+    long long row_stride;
+    int n_pages;
+    int page_size;
+    int n_seqs;
+    int max_pages;          /* entries of one row of page_table */
+    const int* page_table;  /* device [n_seqs][max_pages] */
+    const int* kv_len;      /* device [n_seqs] */
+    const int* q_start;     /* device [n_seqs + 1] */
+} B2PagedKV;
+
+/* b2_qk_rope_kv into a paged cache: per-head q/k RMSNorm (q_norm_w/k_norm_w
+ * may be NULL), RoPE at position pos[m] from tables cos/sin [max_pos][hd/2]
+ * (style 0 interleaved, 1 split-half), then q as FP16 rows q16 [M][ldq] (what
+ * b2_attention_paged takes) and K and V as FP16 at the row's slot.  pos (device
+ * int[M]) NULL takes the slot; it differs from the slot once positions were
+ * evicted.  A row whose position is outside [0, max_pos) is left out entirely;
+ * one whose slot is not mapped only writes q16.  qkv: device FP32 [M][ldqkv] =
+ * [q (nq*hd) | k (nkv*hd) | v (nkv*hd)], read only; 16-byte aligned, ldqkv a
+ * multiple of 4, ldq of 4. */
+int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int M, int nq, int nkv, int hd,
+                        const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_tab,
+                        const float* sin_tab, int max_pos, int rope_style, const int* pos, const B2PagedKV* kv,
+                        b2_stream_t s);
+
+/* Attention of every new row over its sequence's mapped slots up to its own
+ * (causal), GQA with nq / nkv <= 16 q heads per kv head, scores scaled by
+ * 1 / sqrtf(hd).  q16: device FP16 [M][ldq] (first nq*hd), out16: device FP16
+ * [M][nq*hd], lse (may be NULL): device FP32 [M][nq], the natural logarithm of
+ * the row's sum of exponentials.  A row that sees no slot gives zeros and
+ * -infinity.  max_q: no sequence brings more rows than this (M is always
+ * right; a decode step passes 1); a sequence's rows past the first max_q are
+ * left as they are.
+ * Sums and the softmax are FP32; the softmax weights are rounded to FP16 for
+ * the product with V.  V at slots that another row of the same call sees and
+ * this row does not must be finite (0 x inf); anything may lie in slots past
+ * kv_len.
+ * work: device scratch of b2_attention_paged_workspace(n_seqs, max_q, nq, nkv,
+ * hd) bytes, 16-byte aligned and zeroed once before its first use: calls leave
+ * its counters zero, and one buffer of the largest size serves calls of any
+ * shape one after the other, but not calls that may overlap.  A copy that does
+ * not arrive within the wait limit sets *err (device int) to 1 and leaves rows
+ * unfinished; zero work again after that.  q16 16-byte aligned, ldq a multiple
+ * of 8. */
+size_t b2_attention_paged_workspace(int n_seqs, int max_q, int nq, int nkv, int hd);
+int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq, int M, int max_q, int nq, int nkv,
+                       int hd, const B2PagedKV* kv, void* work, int* err, b2_stream_t s);
+
+/* Attention weight that the new rows gave each cached slot, added to what
+ * earlier calls gave it: for sequence q, kv head g and slot j < kv_len[q]
+ *     weights[q][g][j] = prev[q][g][j] + sum over the rows i that see j and the
+ *                        q heads h of g of exp(score(i, h, j) - lse[i][h])
+ * with q16, ldq, max_q and lse as given to and by b2_attention_paged; a row
+ * whose lse is -infinity gives nothing.  weights and prev: device FP32
+ * [n_seqs][nkv][ldw]; prev may be NULL (zeros) or weights itself.  Slots from
+ * kv_len[q] or ldw on are left as they are.  FP32 sums in a fixed order.  err as
+ * in b2_attention_paged. */
+int b2_attention_paged_weights(float* weights, const float* prev, long long ldw, const uint16_t* q16, int ldq,
+                               const float* lse, int M, int max_q, int nq, int nkv, int hd, const B2PagedKV* kv,
+                               int* err, b2_stream_t s);
+
+/* Eviction by accumulated attention weight: of each sequence's mapped slots
+ * below kv_len, each kv head keeps the first `sink` slots and the last `recent`
+ * slots, and of the rest those of the largest weight (device FP32
+ * [n_seqs][nkv][ldw], as b2_attention_paged_weights leaves them; the lowest
+ * slots among equal ones, NaN last), `budget` in all or every mapped slot when
+ * there are fewer.  Slots from ldw on weigh nothing.  What is kept moves, in slot
+ * order, to slots 0, 1, ... of the pages dst_table [n_seqs][dst_max_pages] of the
+ * same pool (unmapped entries are left out).  No page of dst_table may be among
+ * the sequences' own pages, which stay as they are: they may belong to other
+ * sequences too.
+ *   kept         device int   [n_seqs][nkv][budget]  slots kept
+ *   dst_weights  device FP32  [n_seqs][nkv][budget]  their weights (may be NULL)
+ *   new_len      device int   [n_seqs]               slots kept per kv head
+ * Entries from new_len[q] on are left as they are.  kv->q_start is not read.
+ * sink + recent <= budget. */
+int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const float* weights, long long ldw, int budget, int sink,
+                      int recent, const int* dst_table, int dst_max_pages, int* kept, float* dst_weights, int* new_len,
+                      b2_stream_t s);
+
 /* lm_head + argmax over V rows of `table` (int8 [V][K] with FP32 scales,
  * F16 [V][K], or F32 [V][K]).  Input row m is RMSNorm(x[m]; norm_w, eps)
  * (norm_w may be NULL), rounded to FP16 for the int8 table (the reference's

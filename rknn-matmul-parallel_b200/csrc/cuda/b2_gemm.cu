@@ -734,6 +734,22 @@ int b2_tensor_map_f16(void* map, const void* base, uint64_t inner, uint64_t oute
     return make_map(reinterpret_cast<CUtensorMap*>(map), base, true, inner, outer, row_bytes, box_inner, box_outer);
 }
 
+int b2_tensor_map_f16_5d(void* map, const void* base, const uint64_t (&dims)[5], const uint64_t (&strides)[4],
+                         const uint32_t (&box)[5]) {
+    EncodeTiledFn enc = encoder();
+    if (!enc) return b2_set_error(B2_ERR_CUDA, "cuTensorMapEncodeTiled unavailable");
+    cuuint64_t d[5], st[4];
+    cuuint32_t bx[5], es[5];
+    for (int i = 0; i < 5; i++) d[i] = dims[i], bx[i] = box[i], es[i] = 1;
+    for (int i = 0; i < 4; i++) st[i] = strides[i];
+    const CUresult r = enc(reinterpret_cast<CUtensorMap*>(map), CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 5,
+                           const_cast<void*>(base), d, st, bx, es, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                           CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                           CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return b2_set_error(B2_ERR_CUDA, "cuTensorMapEncodeTiled (5-D) failed (%d)", (int)r);
+    return 0;
+}
+
 extern "C" size_t b2_gemm_argmax_keys(int M, int N) { return (size_t)M * ((N + kBM - 1) / kBM) * 8; }
 
 extern "C" int b2_gemm(const B2GemmArgs* a, b2_stream_t stream) {

@@ -1,0 +1,172 @@
+// Shared pieces of the paged-cache kernels (b2_paged_kv.cu, b2_paged_attn.cu,
+// b2_paged_weights.cu): argument checks, the per-sequence view of a batch and
+// the barrier / copy wrappers.
+#pragma once
+#include <cuda.h>  // CUtensorMap
+#include <math.h>
+
+#include <atomic>
+
+#include "b2_common.cuh"
+
+// 5-D FP16 tensor map with the 128-byte swizzle; strides in bytes of dimensions
+// 1..4.  Defined in b2_gemm.cu.
+int b2_tensor_map_f16_5d(void* map, const void* base, const uint64_t (&dims)[5], const uint64_t (&strides)[4],
+                         const uint32_t (&box)[5]);
+
+// Host checks shared by the entry points; 0 or an error code with its message.
+int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool rows);
+// Tensor map of K or V pages: dimensions (64 dims, rows of a page, head_dim / 64,
+// kv heads, pages), boxes of box_rows rows and every dim: a box lands as
+// [head_dim / 64][box_rows][128 bytes], each 128-byte row swizzled.
+int b2_paged_map(CUtensorMap* map, const uint16_t* base, const B2PagedKV* kv, int nkv, int hd, int box_rows);
+
+namespace b2p {
+
+// A sequence of the batch, with the caller's device values bounded so that no
+// index computed from them leaves its array.
+struct Seq {
+    int row0;  // its first row
+    int Q;     // its rows
+    int len;   // cached positions, at most the table's capacity
+    int base;  // slot of row 0 (negative when kv_len < Q: those rows see nothing)
+};
+
+struct Batch {
+    const int* page_table;
+    const int* kv_len;
+    const int* q_start;
+    int n_seqs, max_pages, n_pages, page_shift, M;
+
+    __device__ __forceinline__ Seq seq(int s) const {
+        Seq x;
+        const int a = min(max(q_start[s], 0), M), b = min(max(q_start[s + 1], a), M), n = kv_len[s];
+        x.row0 = a;
+        x.Q = b - a;
+        x.base = n - x.Q;
+        const long long cap = (long long)max_pages << page_shift;
+        x.len = n < 0 ? 0 : (int)((long long)n < cap ? n : cap);
+        return x;
+    }
+    // Page of slot j, or -1 where none is mapped.
+    __device__ __forceinline__ int page(int s, int j) const {
+        const int p = page_table[(size_t)s * max_pages + (j >> page_shift)];
+        return p >= 0 && p < n_pages ? p : -1;
+    }
+};
+
+inline Batch make_batch(const B2PagedKV* kv, int M) {
+    Batch b{kv->page_table, kv->kv_len, kv->q_start, kv->n_seqs, kv->max_pages, kv->n_pages, 0, M};
+    while ((1 << b.page_shift) < kv->page_size) b.page_shift++;
+    return b;
+}
+
+__device__ __forceinline__ uint32_t smem_u32(const void* p) {
+    return static_cast<uint32_t>(__cvta_generic_to_shared(p));
+}
+__device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
+    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");
+}
+__device__ __forceinline__ void mbar_init_fence() {
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void mbar_expect_tx(uint64_t* bar, uint32_t bytes) {
+    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(smem_u32(bar)), "r"(bytes)
+                 : "memory");
+}
+__device__ __forceinline__ void mbar_arrive(uint64_t* bar) {
+    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
+    uint32_t ok;
+    asm volatile(
+        "{\n .reg .pred p;\n mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, 0, p;\n}\n"
+        : "=r"(ok)
+        : "r"(smem_u32(bar)), "r"(parity)
+        : "memory");
+    return ok != 0;
+}
+constexpr long long kWaitLimit = 1ll << 22;
+// Bounded wait: false, with the CTA's failure flag set, after kWaitLimit polls
+// or once another thread has given up.
+__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+    for (long long it = 0; !mbar_try_wait(bar, parity); it++) {
+        if (it > kWaitLimit || *failed) {
+            *failed = 1;
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int x, int row, int half, int head,
+                                            int page, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.5d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5, "
+        "%6}], [%7];" ::"r"(smem_u32(dst)),
+        "l"(map), "r"(x), "r"(row), "r"(half), "r"(head), "r"(page), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// 2^x (ex2.approx: 2 ulp; subnormal results flush to zero).
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_h2(float lo, float hi) {
+    __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, "
+        "{%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// Work of each sequence -> exclusive prefix pre[0..n] (shared memory, n + 1
+// ints), by all threads of the CTA.
+template <typename F>
+__device__ __forceinline__ void prefix_work(int* pre, int n, F work) {
+    for (int s = threadIdx.x; s < n; s += blockDim.x) pre[s + 1] = work(s);
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        const int lane = threadIdx.x;
+        int carry = 0;
+        for (int b = 0; b < n; b += 32) {
+            int v = b + lane < n ? pre[b + lane + 1] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int t = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v += t;
+            }
+            if (b + lane < n) pre[b + lane + 1] = carry + v;
+            carry += __shfl_sync(0xffffffffu, v, 31);
+        }
+        if (lane == 0) pre[0] = 0;
+    }
+    __syncthreads();
+}
+// Largest s in [0, n) with pre[s] <= x (x < pre[n]).
+__device__ __forceinline__ int prefix_find(const int* pre, int n, int x) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (pre[mid] <= x) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// Host: dynamic shared memory opt-in, once per kernel and device.
+template <typename K>
+inline cudaError_t allow_smem(K kern, size_t bytes, std::atomic<unsigned long long>& done, int dev) {
+    const unsigned long long bit = 1ull << (dev & 63);
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    const cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
+
+}  // namespace b2p

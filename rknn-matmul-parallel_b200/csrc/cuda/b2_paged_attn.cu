@@ -1,0 +1,521 @@
+// Attention of a batch's new rows over a paged KV cache (b2_attention_paged).
+//
+//   s_ij = q_i . k_j / sqrt(hd)   for the mapped slots j up to row i's own,
+//   o_i = sum_j exp(s_ij - m_i) v_j / l_i,   lse_i = m_i + ln l_i,
+// with the running maximum m and sum l of one pass over the slots (the online
+// softmax): a new maximum rescales what was summed before it.
+#include "b2_paged.cuh"
+
+namespace {
+
+using b2p::ex2;
+using b2p::smem_u32;
+
+constexpr float kLn2 = 0.69314718055994531f;
+// The weights are formed as 2^(s - m + kUp) with s and m in units of log2: the
+// FP16 copy that the product with V takes then keeps 11 bits down to 2^-28 of
+// the row's largest weight, where weights of a long row lie.  Sums carry the
+// same factor, which the division by l takes out.
+constexpr float kUp = 14.f;
+
+__device__ __forceinline__ void ldsm_x4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm_x4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ uint32_t movm_t(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+
+struct AttnParams {
+    b2p::Batch bt;
+    const __half* q16;
+    int ldq;
+    __half* out16;
+    float* lse;
+    int max_q, nq, nkv, G, T;  // T: tokens of one tile
+    float* part;               // partial tiles
+    int* counters;             // [grid], zero between calls
+    int* err;
+};
+
+// ─── few rows per sequence: decode steps, drafted tokens ───
+//
+// Bound by reading K and V once from HBM.  A tile is T tokens x the G q heads
+// of one kv head, at most R = 8 NT rows.  The work of the call is one line of
+// blocks of 64 slots: sequences, then tiles and kv heads, then the tile's
+// blocks.  Every CTA takes an equal stretch of that line, so sequences of any
+// mix of lengths load the SMs evenly; a tile that a stretch boundary cuts is
+// summed in pieces, which its last arriver merges in the line's order.
+//
+// A producer warp keeps a ring of stages (64 slots of K and V) filled by TMA,
+// through the page table, across tile boundaries.  Four warps compute, each on
+// 16 slots of a stage:
+//   S^T = K Q^T    mma m16n8k16: slots are the M rows, the tile's rows the N
+//                  columns;
+//   O^T += V^T P^T the head dims are M, the slots K; P^T moves from the
+//                  accumulator to the B-operand layout with movmatrix.
+constexpr int kBlk = 64;
+constexpr int kThreads = 160;  // four computing warps, one producer
+constexpr int kMinBlocks = 4;  // shortest stretch of a CTA
+
+template <int HD, int NT>
+struct Short {
+    static constexpr int R = 8 * NT;
+    static constexpr int kStage = kBlk * HD * 4;  // K and V, bytes
+    static constexpr int kStages = HD == 128 ? 3 : 6;
+    static constexpr int kLd = HD + 4;            // row of the merge buffer: the four lane columns hit distinct banks
+    static constexpr int kTile = R * (HD + 2);    // floats of one partial tile: o[R][HD], then (m, l)[R]
+};
+
+template <int HD, int NT>
+struct ShortSmem {
+    alignas(1024) unsigned char ring[Short<HD, NT>::kStages * Short<HD, NT>::kStage];
+    float o[Short<HD, NT>::R * Short<HD, NT>::kLd];
+    float m[4][Short<HD, NT>::R], l[4][Short<HD, NT>::R];
+    uint64_t full[Short<HD, NT>::kStages], empty[Short<HD, NT>::kStages];
+    int mapped[Short<HD, NT>::kStages];  // bit w: the 16 slots of warp w are mapped
+    int failed, last;
+    int pre[B2_PAGED_MAX_SEQS + 1];
+};
+
+// Factor of a piece with maximum m in a sum whose maximum is M.  A piece that
+// saw no slot has m = -inf and sums of 0; one that saw only NaN has NaN sums,
+// which the factor 1 keeps.
+__device__ __forceinline__ float piece_weight(float m, float M) { return m == -INFINITY ? 1.f : ex2(m - M); }
+
+__device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
+
+// A stretch's part of one tile: blocks [b0, b1) of the tile's nb.
+struct Seg {
+    int s, g, i0, rows_t;  // sequence, kv head, first token, tokens
+    int b0, b1, live;      // live: end of the blocks that some row of the tile sees
+    int nb, x0;            // the tile's blocks, and where it starts on the line
+    b2p::Seq sq;
+};
+
+__device__ __forceinline__ Seg find_seg(const AttnParams& p, const int* pre, int x, int x1) {
+    Seg r;
+    r.s = b2p::prefix_find(pre, p.bt.n_seqs, x);
+    r.sq = p.bt.seq(r.s);
+    r.nb = max(1, cdiv(r.sq.len, kBlk));
+    const int off = x - pre[r.s], item = off / r.nb;
+    r.b0 = off - item * r.nb;
+    r.b1 = min(r.nb, r.b0 + (x1 - x));
+    r.x0 = x - r.b0;
+    r.g = item % p.nkv;
+    r.i0 = item / p.nkv * p.T;
+    r.rows_t = min(p.T, min(r.sq.Q, p.max_q) - r.i0);
+    const int end = min(r.sq.len, max(0, r.sq.base + r.i0 + r.rows_t));
+    r.live = min(r.b1, cdiv(end, kBlk));
+    return r;
+}
+
+template <int HD, int NT>
+__global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_constant__ CUtensorMap tk,
+                                                              const __grid_constant__ CUtensorMap tv, const AttnParams p) {
+    using C = Short<HD, NT>;
+    constexpr int R = C::R;
+    extern __shared__ unsigned char smem_raw[];
+    ShortSmem<HD, NT>& sm = *reinterpret_cast<ShortSmem<HD, NT>*>(
+        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < C::kStages; i++) {
+            b2p::mbar_init(&sm.full[i], 1);
+            b2p::mbar_init(&sm.empty[i], 4);
+        }
+        sm.failed = 0;
+        b2p::mbar_init_fence();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
+    }
+    b2::pdl_trigger();
+    b2::pdl_wait();
+    b2p::prefix_work(sm.pre, p.bt.n_seqs, [&](int s) {
+        const b2p::Seq q = p.bt.seq(s);
+        return cdiv(min(q.Q, p.max_q), p.T) * p.nkv * max(1, cdiv(q.len, kBlk));
+    });
+    const int W = sm.pre[p.bt.n_seqs];
+    const int per = max(kMinBlocks, cdiv(W, gridDim.x));
+    const int x0 = min((long long)W, (long long)blockIdx.x * per), x1 = min(W, x0 + per);
+    if (x0 >= x1) return;
+    const int page_rows = 1 << p.bt.page_shift, box_rows = min(page_rows, kBlk);
+
+    if (warp == 4) {  // producer: lane i copies the i-th box of a stage
+        const int boxes = kBlk / box_rows, box_bytes = box_rows * HD * 2;
+        int k = 0;
+        bool ok = true;
+        for (int x = x0; x < x1 && ok;) {
+            const Seg g = find_seg(p, sm.pre, x, x1);
+            for (int b = g.b0; b < g.live; b++, k++) {
+                const int st = k % C::kStages, j = b * kBlk + lane * box_rows;
+                const int page = lane < boxes && j < g.sq.len ? p.bt.page(g.s, j) : -1;
+                if (k >= C::kStages && !b2p::mbar_wait(&sm.empty[st], (k / C::kStages - 1) & 1, &sm.failed)) ok = false;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+                const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
+                if (lane == 0) {
+                    int bits = 0;
+                    for (int w = 0; w < 4; w++) bits |= (have >> (w * 16 / box_rows) & 1) << w;
+                    sm.mapped[st] = bits;
+                    b2p::mbar_expect_tx(&sm.full[st], __popc(have) * 2 * box_bytes);
+                }
+                __syncwarp();
+                if (page >= 0) {
+                    unsigned char* dst = sm.ring + st * C::kStage + lane * box_bytes;
+                    const int row = j & (page_rows - 1);
+                    b2p::tma_load_5d(dst, &tk, 0, row, 0, g.g, page, &sm.full[st]);
+                    b2p::tma_load_5d(dst + C::kStage / 2, &tv, 0, row, 0, g.g, page, &sm.full[st]);
+                }
+            }
+            x += g.b1 - g.b0;
+        }
+        // a failed wait: let the copies in flight land (again bounded) before the CTA ends
+        if (!ok && lane == 0)
+            for (int i = max(0, k - C::kStages); i < k; i++)
+                for (long long it = 0; it <= b2p::kWaitLimit; it++)
+                    if (b2p::mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
+        return;
+    }
+
+    const float scale = 1.4426950408889634f / sqrtf((float)HD);  // to log2 units
+    const int pw = warp * 16;
+    const int bshift = box_rows == 16 ? 4 : box_rows == 32 ? 5 : 6;
+    int k = 0;
+    bool ok = true;
+    for (int x = x0; x < x1 && ok;) {
+        const Seg sg = find_seg(p, sm.pre, x, x1);
+        x += sg.b1 - sg.b0;
+        const int rows = sg.rows_t * p.G;  // rows of the tile: token i0 + r / G, q head g G + r % G
+        uint32_t qb[HD / 16][NT][2];
+        int lim[NT][2];  // last slot that this lane's two columns see
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            const int r = 8 * t + (lane >> 2);
+            const __half* qp = p.q16 + (size_t)(sg.sq.row0 + sg.i0 + r / p.G) * p.ldq +
+                               (size_t)(sg.g * p.G + r % p.G) * HD + 2 * (lane & 3);
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++) {
+                qb[i][t][0] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * i) : 0u;
+                qb[i][t][1] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * i + 8) : 0u;
+            }
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int c = 8 * t + 2 * (lane & 3) + j;
+                lim[t][j] = c < rows ? min(sg.sq.len - 1, sg.sq.base + sg.i0 + c / p.G) : -1;
+            }
+        }
+        float o[HD / 16][NT][4], mx[NT][2], ls[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++) o[i][t][0] = o[i][t][1] = o[i][t][2] = o[i][t][3] = 0.f;
+            mx[t][0] = mx[t][1] = -INFINITY;
+            ls[t][0] = ls[t][1] = 0.f;
+        }
+        for (int b = sg.b0; b < sg.live; b++, k++) {
+            const int st = k % C::kStages;
+            ok = b2p::mbar_wait(&sm.full[st], (k / C::kStages) & 1, &sm.failed);
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            unsigned char* stage = sm.ring + st * C::kStage;
+            const int j0 = b * kBlk + pw, np = sg.sq.len - j0;  // np: cached slots from this warp's first
+            if ((sm.mapped[st] >> warp & 1) && np > 0) {
+                // this warp's 16 rows within their box: [dims 0-63, 64-127][box_rows][128 bytes]
+                const uint32_t bo = (pw >> bshift) * box_rows * HD * 2 + (pw & (box_rows - 1)) * 128;
+                const uint32_t half = box_rows * 128;
+                const uint32_t ka = smem_u32(stage) + bo, va = ka + C::kStage / 2;
+                if (np < 16) {
+                    // V rows past kv_len may hold anything: zero them (their P is zero, and 0 x inf is not)
+                    for (int r = np + (lane >> 4); r < 16; r += 2) {
+                        const int c = lane & 15;
+                        if (c < HD / 8)
+                            *reinterpret_cast<uint4*>(stage + C::kStage / 2 + bo + (c >> 3) * half + r * 128 +
+                                                      (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    }
+                    // ordered before the next copy into this stage
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+                float sc[NT][4];
+#pragma unroll
+                for (int t = 0; t < NT; t++) sc[t][0] = sc[t][1] = sc[t][2] = sc[t][3] = 0.f;
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++) {
+                    // K rows (+8 for odd lane groups), dims 16 i (+8 for the upper two groups)
+                    const int r = (lane & 7) + ((lane >> 3) & 1) * 8, d = 16 * i + (lane >> 4) * 8;
+                    uint32_t a[4];
+                    ldsm_x4(ka + (d >> 6) * half + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4), a);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) b2p::mma16816(sc[t], a, qb[i][t][0], qb[i][t][1]);
+                }
+                const int ja = j0 + (lane >> 2), jb = ja + 8;
+                uint32_t pb[NT][2];
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+                    float pr[4], corr[2];
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const float sa = ja <= lim[t][j] ? sc[t][j] * scale : -INFINITY;
+                        const float sb = jb <= lim[t][j] ? sc[t][j + 2] * scale : -INFINITY;
+                        float cm = fmaxf(sa, sb);
+                        cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 4));
+                        cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 8));
+                        cm = fmaxf(cm, __shfl_xor_sync(0xffffffffu, cm, 16));
+                        const float mn = fmaxf(mx[t][j], cm);
+                        const float ref = mn == -INFINITY ? 0.f : mn - kUp;
+                        corr[j] = mn == -INFINITY ? 1.f : ex2(mx[t][j] - mn);
+                        pr[j] = ex2(sa - ref);
+                        pr[j + 2] = ex2(sb - ref);
+                        float rs = pr[j] + pr[j + 2];
+                        rs += __shfl_xor_sync(0xffffffffu, rs, 4);
+                        rs += __shfl_xor_sync(0xffffffffu, rs, 8);
+                        rs += __shfl_xor_sync(0xffffffffu, rs, 16);
+                        ls[t][j] = ls[t][j] * corr[j] + rs;
+                        mx[t][j] = mn;
+                    }
+#pragma unroll
+                    for (int i = 0; i < HD / 16; i++) {
+                        o[i][t][0] *= corr[0];
+                        o[i][t][1] *= corr[1];
+                        o[i][t][2] *= corr[0];
+                        o[i][t][3] *= corr[1];
+                    }
+                    pb[t][0] = movm_t(b2p::pack_h2(pr[0], pr[1]));
+                    pb[t][1] = movm_t(b2p::pack_h2(pr[2], pr[3]));
+                }
+#pragma unroll
+                for (int i = 0; i < HD / 16; i++) {
+                    // V^T: dims 16 i (+8 for odd lane groups), slots (+8 for the upper two groups)
+                    const int r = (lane & 7) + (lane >> 4) * 8, d = 16 * i + ((lane >> 3) & 1) * 8;
+                    uint32_t a[4];
+                    ldsm_x4_t(va + (d >> 6) * half + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4), a);
+#pragma unroll
+                    for (int t = 0; t < NT; t++) b2p::mma16816(o[i][t], a, pb[t][0], pb[t][1]);
+                }
+            }
+            __syncwarp();
+            if (lane == 0) b2p::mbar_arrive(&sm.empty[st]);
+        }
+        // merge the four warps' states, warp by warp
+        if (lane < 4) {
+#pragma unroll
+            for (int t = 0; t < NT; t++) {
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    sm.m[warp][8 * t + 2 * lane + j] = mx[t][j];
+                    sm.l[warp][8 * t + 2 * lane + j] = ls[t][j];
+                }
+            }
+        }
+        // one decision for the four warps (a failed wait ends the stretch)
+        int bad;
+        asm volatile(
+            "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.s32 %0, 1, 0, "
+            "q;\n}\n"
+            : "=r"(bad)
+            : "r"(ok ? 0 : 1)
+            : "memory");
+        if (bad) {
+            ok = false;
+            break;
+        }
+        float f[NT][2];
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int c = 8 * t + 2 * (lane & 3) + j;
+                const float M = fmaxf(fmaxf(sm.m[0][c], sm.m[1][c]), fmaxf(sm.m[2][c], sm.m[3][c]));
+                f[t][j] = piece_weight(mx[t][j], M);
+            }
+        }
+        for (int w = 0; w < 4; w++) {
+            if (w == warp) {
+#pragma unroll
+                for (int t = 0; t < NT; t++) {
+#pragma unroll
+                    for (int i = 0; i < HD / 16; i++) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float* d = &sm.o[(8 * t + 2 * (lane & 3) + (e & 1)) * C::kLd + 16 * i + (lane >> 2) + (e >> 1) * 8];
+                            const float v = o[i][t][e] * f[t][e & 1];
+                            *d = w ? *d + v : v;
+                        }
+                    }
+                }
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+        }
+        const bool whole = sg.b0 == 0 && sg.b1 == sg.nb;
+        const int tid = threadIdx.x;
+        const int own = sg.x0 / per;  // the CTA whose stretch holds the tile's first block
+        float* part = p.part + (size_t)(2 * blockIdx.x + (sg.b0 == 0 ? 1 : 0)) * C::kTile;
+        for (int i = tid; i < rows * (HD / 8); i += 128) {
+            const int r = i / (HD / 8), c = i % (HD / 8) * 8;
+            const float M = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
+            float l = 0.f;
+#pragma unroll
+            for (int w = 0; w < 4; w++) l = fmaf(sm.l[w][r], piece_weight(sm.m[w][r], M), l);
+            const float4 u = *reinterpret_cast<const float4*>(&sm.o[r * C::kLd + c]);
+            const float4 v = *reinterpret_cast<const float4*>(&sm.o[r * C::kLd + c + 4]);
+            if (whole) {
+                const float inv = l == 0.f ? 0.f : 1.f / l;
+                const size_t row = (size_t)(sg.sq.row0 + sg.i0 + r / p.G);
+                const int h = sg.g * p.G + r % p.G;
+                uint4 w;
+                w.x = b2p::pack_h2(u.x * inv, u.y * inv);
+                w.y = b2p::pack_h2(u.z * inv, u.w * inv);
+                w.z = b2p::pack_h2(v.x * inv, v.y * inv);
+                w.w = b2p::pack_h2(v.z * inv, v.w * inv);
+                *reinterpret_cast<uint4*>(p.out16 + (row * p.nq + h) * HD + c) = w;
+                if (c == 0 && p.lse) p.lse[row * p.nq + h] = l == 0.f ? -INFINITY : (M - kUp) * kLn2 + logf(l);
+            } else {
+                *reinterpret_cast<float4*>(part + r * HD + c) = u;
+                *reinterpret_cast<float4*>(part + r * HD + c + 4) = v;
+                if (c == 0) *reinterpret_cast<float2*>(part + R * HD + 2 * r) = make_float2(M, l);
+            }
+        }
+        if (!whole) {
+            const int last_cta = (sg.x0 + sg.nb - 1) / per;
+            __threadfence();
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (tid == 0) {
+                const int before = atomicAdd(&p.counters[own], 1);
+                __threadfence();
+                sm.last = before == last_cta - own;
+                if (sm.last) p.counters[own] = 0;
+            }
+            asm volatile("bar.sync 1, 128;" ::: "memory");
+            if (sm.last) {
+                // every piece has arrived: merge them in the line's order (the owner's piece, then the
+                // CTAs after it), one warp per row
+                for (int r = warp; r < rows; r += 4) {
+                    float M = -INFINITY;
+                    for (int c = own + lane; c <= last_cta; c += 32)
+                        M = fmaxf(M, __ldcg(p.part + (size_t)(2 * c + (c == own)) * C::kTile + R * HD + 2 * r));
+                    M = b2::warp_max(M);
+                    float l = 0.f, acc[HD / 32];
+#pragma unroll
+                    for (int i = 0; i < HD / 32; i++) acc[i] = 0.f;
+#pragma unroll 4
+                    for (int c = own; c <= last_cta; c++) {
+                        const float* q = p.part + (size_t)(2 * c + (c == own)) * C::kTile;
+                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + R * HD + 2 * r));
+                        const float wgt = piece_weight(ml.x, M);
+                        l = fmaf(ml.y, wgt, l);
+#pragma unroll
+                        for (int i = 0; i < HD / 32; i++) acc[i] = fmaf(__ldcg(q + r * HD + 32 * i + lane), wgt, acc[i]);
+                    }
+                    const float inv = l == 0.f ? 0.f : 1.f / l;
+                    const size_t row = (size_t)(sg.sq.row0 + sg.i0 + r / p.G);
+                    const int h = sg.g * p.G + r % p.G;
+#pragma unroll
+                    for (int i = 0; i < HD / 32; i++)
+                        p.out16[(row * p.nq + h) * HD + 32 * i + lane] = __float2half_rn(acc[i] * inv);
+                    if (lane == 0 && p.lse) p.lse[row * p.nq + h] = l == 0.f ? -INFINITY : (M - kUp) * kLn2 + logf(l);
+                }
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");  // the merge area is free for the next tile
+    }
+    if (!ok && lane == 0) atomicExch(p.err, 1);
+}
+
+constexpr int kMaxGroup = 16;
+constexpr size_t kCounterBytes = 4096;
+
+// CTAs of a launch: every SM's resident ones.
+template <int HD, int NT>
+int short_grid(int dev, int sms) {
+    static std::atomic<int> per[64];
+    std::atomic<int>& c = per[dev & 63];
+    int n = c.load(std::memory_order_relaxed);
+    if (n == 0) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_short_kernel<HD, NT>, kThreads,
+                                                          sizeof(ShortSmem<HD, NT>) + 1024) != cudaSuccess || n < 1)
+            n = 1;
+        c.store(n, std::memory_order_relaxed);
+    }
+    return (n < 2 ? n : 2) * sms;
+}
+
+template <int HD, int NT>
+int launch_short(AttnParams p, const CUtensorMap& tk, const CUtensorMap& tv, int dev, int sms, long long blocks,
+                 cudaStream_t s) {
+    static std::atomic<unsigned long long> done{0};
+    constexpr size_t smem = sizeof(ShortSmem<HD, NT>) + 1024;
+    cudaError_t e = b2p::allow_smem(attn_short_kernel<HD, NT>, smem, done, dev);
+    if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged smem: %s", cudaGetErrorString(e));
+    long long grid = short_grid<HD, NT>(dev, sms);
+    if (grid > (blocks + kMinBlocks - 1) / kMinBlocks) grid = (blocks + kMinBlocks - 1) / kMinBlocks;
+    e = b2::launch_pdl(attn_short_kernel<HD, NT>, dim3((unsigned)grid), dim3(kThreads), smem, s, tk, tv, p);
+    if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+int device_sms(int* dev) {
+    int sms = 148;
+    *dev = 0;
+    cudaGetDevice(dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, *dev);
+    return sms;
+}
+
+}  // namespace
+
+extern "C" size_t b2_attention_paged_workspace(int n_seqs, int max_q, int nq, int nkv, int hd) {
+    int dev;
+    const int sms = device_sms(&dev);
+    // two partial tiles of up to 32 rows for each of at most two CTAs per SM
+    return kCounterBytes + (size_t)sms * 2 * 2 * 32 * (hd + 2) * sizeof(float);
+}
+
+extern "C" int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq, int M, int max_q, int nq,
+                                  int nkv, int hd, const B2PagedKV* kv, void* work, int* err, b2_stream_t s) {
+    int rc = b2_paged_check("b2_attention_paged", kv, nkv, hd, true);
+    if (rc) return rc;
+    if (!out16 || !q16 || !work || !err || M < 0 || max_q < 0 || nq <= 0 || nq % nkv || nq / nkv > kMaxGroup)
+        return b2_set_error(B2_ERR_INVALID_ARG, "b2_attention_paged: bad arguments (nq a multiple of nkv, at most %d)",
+                            kMaxGroup);
+    if (ldq < nq * hd || ldq % 8 || (reinterpret_cast<uintptr_t>(q16) & 15) || (reinterpret_cast<uintptr_t>(out16) & 15) ||
+        (reinterpret_cast<uintptr_t>(work) & 15))
+        return b2_set_error(B2_ERR_INVALID_ARG,
+                            "b2_attention_paged: q16, out16 and work must be 16-byte aligned, ldq a multiple of 8 that "
+                            "holds every head");
+    if (M == 0 || kv->n_seqs == 0 || max_q == 0) return 0;
+    if (max_q > M) max_q = M;
+    int dev;
+    const int sms = device_sms(&dev);
+    CUtensorMap tk, tv;
+    const int box = kv->page_size < kBlk ? kv->page_size : kBlk;
+    rc = b2_paged_map(&tk, kv->k_pages, kv, nkv, hd, box);
+    if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, nkv, hd, box);
+    if (rc) return rc;
+    const int G = nq / nkv, rows = max_q * G, NT = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    AttnParams p{b2p::make_batch(kv, M), reinterpret_cast<const __half*>(q16), ldq, reinterpret_cast<__half*>(out16), lse,
+                 max_q, nq, nkv, G, 8 * NT / G,
+                 reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(work) + kCounterBytes),
+                 reinterpret_cast<int*>(work), err};
+    // the line's length when every sequence fills its table: what the kernel's 32-bit places must hold
+    const long long cap = ((long long)kv->max_pages * kv->page_size + kBlk - 1) / kBlk;
+    const long long tiles = (M + p.T - 1) / p.T + kv->n_seqs;
+    const long long blocks = tiles * nkv * cap;
+    if (blocks >= (1ll << 31) - 65536)
+        return b2_set_error(B2_ERR_INVALID_ARG, "b2_attention_paged: %lld blocks of work in one call", blocks);
+    cudaStream_t st = (cudaStream_t)s;
+#define B2_SHORT(HD)                                                                     \
+    (NT == 1   ? launch_short<HD, 1>(p, tk, tv, dev, sms, blocks, st)                    \
+     : NT == 2 ? launch_short<HD, 2>(p, tk, tv, dev, sms, blocks, st)                    \
+               : launch_short<HD, 4>(p, tk, tv, dev, sms, blocks, st))
+    return hd == 128 ? B2_SHORT(128) : B2_SHORT(64);
+#undef B2_SHORT
+}

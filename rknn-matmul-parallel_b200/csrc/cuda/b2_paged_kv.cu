@@ -1,0 +1,335 @@
+// Writing a paged KV cache: new rows (b2_qk_rope_kv_paged) and eviction by
+// accumulated attention weight (b2_kv_evict_paged).
+#include "b2_paged.cuh"
+
+int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool rows) {
+    if (!kv || !kv->k_pages || !kv->v_pages || !kv->page_table || !kv->kv_len || (rows && !kv->q_start))
+        return b2_set_error(B2_ERR_INVALID_ARG, "%s: null pointer in the cache description", who);
+    if (hd != 64 && hd != 128) return b2_set_error(B2_ERR_INVALID_ARG, "%s: head_dim %d not in {64, 128}", who, hd);
+    if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64 && kv->page_size != 128)
+        return b2_set_error(B2_ERR_INVALID_ARG, "%s: page_size %d not in {16, 32, 64, 128}", who, kv->page_size);
+    if (kv->n_pages <= 0 || kv->max_pages <= 0 || kv->n_seqs < 0 || kv->n_seqs > B2_PAGED_MAX_SEQS || nkv <= 0 ||
+        (long long)kv->max_pages * kv->page_size > 0x7fffff00ll)
+        return b2_set_error(B2_ERR_INVALID_ARG, "%s: bad counts (pages %d, table row %d, sequences %d of at most %d)",
+                            who, kv->n_pages, kv->max_pages, kv->n_seqs, B2_PAGED_MAX_SEQS);
+    const long long lim = 1ll << 39;
+    if ((reinterpret_cast<uintptr_t>(kv->k_pages) & 15) || (reinterpret_cast<uintptr_t>(kv->v_pages) & 15) ||
+        kv->page_stride % 8 || kv->head_stride % 8 || kv->row_stride % 8 || kv->page_stride <= 0 ||
+        kv->head_stride <= 0 || kv->row_stride < hd || kv->page_stride >= lim || kv->head_stride >= lim ||
+        kv->row_stride >= lim)
+        return b2_set_error(B2_ERR_INVALID_ARG,
+                            "%s: pages must be 16-byte aligned with positive strides that are multiples of 8", who);
+    return 0;
+}
+
+int b2_paged_map(CUtensorMap* map, const uint16_t* base, const B2PagedKV* kv, int nkv, int hd, int box_rows) {
+    const uint64_t dims[5] = {64, (uint64_t)kv->page_size, (uint64_t)hd / 64, (uint64_t)nkv, (uint64_t)kv->n_pages};
+    const uint64_t strides[4] = {(uint64_t)kv->row_stride * 2, 128, (uint64_t)kv->head_stride * 2,
+                                 (uint64_t)kv->page_stride * 2};
+    const uint32_t box[5] = {64, (uint32_t)box_rows, (uint32_t)hd / 64, 1, 1};
+    return b2_tensor_map_f16_5d(map, base, dims, strides, box);
+}
+
+namespace {
+
+struct PageStrides {
+    uint16_t *k, *v;
+    long long page, head, row;
+};
+
+// ─── b2_qk_rope_kv_paged ───
+//
+// x = one head of one row; for q and k (with norm weights)
+//     n = (x / sqrt(mean(x^2) + eps)) * w
+// then the rotation of pairs (2i, 2i + 1) or (i, i + hd / 2) by the angle of
+// the row's position, and the rounding to FP16: q for the tensor cores of the
+// attention, K and V as the cache keeps them.  FP32 throughout, the sum of
+// squares across the warp.  Bound by HBM: 4 bytes read and 2 written per
+// element.  A warp takes kHeads heads of one row at a time, so their loads are
+// in flight together and the row's angles are read once.
+constexpr int kAppendThreads = 256;
+constexpr int kHeads = 4;
+
+template <int HD>
+__global__ void __launch_bounds__(kAppendThreads) append_kernel(
+    __half* __restrict__ q16, int ldq, const float* __restrict__ qkv, int ldqkv, int nq, int nkv,
+    const float* __restrict__ q_norm_w, const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_tab,
+    const float* __restrict__ sin_tab, int max_pos, int rope_style, const int* __restrict__ pos_of, b2p::Batch bt,
+    PageStrides pg) {
+    constexpr int E = HD / 32;  // elements per lane
+    b2::pdl_trigger();
+    b2::pdl_wait();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int heads = nq + 2 * nkv, per_row = (heads + kHeads - 1) / kHeads;
+    const long long job = (long long)blockIdx.x * (kAppendThreads / 32) + warp;
+    const int m = (int)(job / per_row), h0 = (int)(job % per_row) * kHeads;
+    if (m >= bt.M || m >= bt.q_start[bt.n_seqs] || m < bt.q_start[0]) return;
+    // largest s with q_start[s] <= m: every lane tests one splitter per round
+    int lo = 0, hi = bt.n_seqs;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 31) / 32, at = lo + lane * step;
+        const unsigned le = __ballot_sync(0xffffffffu, at < hi && bt.q_start[at] <= m);
+        lo += (31 - __clz(le)) * step;
+        hi = min(hi, lo + step);
+    }
+    const b2p::Seq sq = bt.seq(lo);
+    const int slot = sq.base + (m - sq.row0);
+    const int pos = pos_of ? pos_of[m] : slot;
+    if (pos < 0 || pos >= max_pos || m - sq.row0 >= sq.Q) return;
+    const int page = slot >= 0 && slot < sq.len ? bt.page(lo, slot) : -1;
+    const long long at = page >= 0 ? page * pg.page + (slot & ((1 << bt.page_shift) - 1)) * pg.row : 0;
+
+    float x[kHeads][E];
+    const float* src = qkv + (size_t)m * ldqkv + lane * E;
+#pragma unroll
+    for (int i = 0; i < kHeads; i++) {
+        if (h0 + i >= heads) break;
+        const float* p = src + (size_t)(h0 + i) * HD;
+        if constexpr (E == 4) {
+            const float4 v = *reinterpret_cast<const float4*>(p);
+            x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
+        } else {
+            const float2 v = *reinterpret_cast<const float2*>(p);
+            x[i][0] = v.x, x[i][1] = v.y;
+        }
+    }
+    // angle index of element j: pairs (2i, 2i+1), or i and i + HD/2
+    float c[E], sn[E];
+#pragma unroll
+    for (int j = 0; j < E; j++) {
+        const int e = lane * E + j, i = rope_style == 0 ? e >> 1 : e & (HD / 2 - 1);
+        c[j] = cos_tab[(size_t)pos * (HD / 2) + i];
+        sn[j] = sin_tab[(size_t)pos * (HD / 2) + i];
+    }
+#pragma unroll
+    for (int i = 0; i < kHeads; i++) {
+        const int h = h0 + i;
+        if (h >= heads) break;
+        const bool is_q = h < nq, is_v = h >= nq + nkv;
+        if (!is_v) {
+            const float* w = is_q ? q_norm_w : k_norm_w;
+            if (w) {
+                float ss = 0.f;
+#pragma unroll
+                for (int j = 0; j < E; j++) ss = fmaf(x[i][j], x[i][j], ss);
+                const float r = 1.0f / sqrtf(b2::warp_sum(ss) / (float)HD + eps);
+#pragma unroll
+                for (int j = 0; j < E; j++) x[i][j] = (x[i][j] * r) * w[lane * E + j];
+            }
+            if (rope_style == 0) {
+#pragma unroll
+                for (int j = 0; j < E; j += 2) {
+                    const float a = x[i][j], b = x[i][j + 1];
+                    x[i][j] = a * c[j] - b * sn[j];
+                    x[i][j + 1] = b * c[j] + a * sn[j];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < E; j++) {
+                    const float o = __shfl_xor_sync(0xffffffffu, x[i][j], 16);
+                    x[i][j] = lane < 16 ? x[i][j] * c[j] - o * sn[j] : x[i][j] * c[j] + o * sn[j];
+                }
+            }
+        }
+        __half* dst;
+        if (is_q) {
+            dst = q16 + (size_t)m * ldq + (size_t)h * HD;
+        } else {
+            if (page < 0) continue;
+            const int g = is_v ? h - nq - nkv : h - nq;
+            dst = reinterpret_cast<__half*>(is_v ? pg.v : pg.k) + at + g * pg.head;
+        }
+        if constexpr (E == 4) {
+            uint2 u;
+            u.x = b2p::pack_h2(x[i][0], x[i][1]);
+            u.y = b2p::pack_h2(x[i][2], x[i][3]);
+            *reinterpret_cast<uint2*>(dst + lane * E) = u;
+        } else {
+            *reinterpret_cast<uint32_t*>(dst + lane * E) = b2p::pack_h2(x[i][0], x[i][1]);
+        }
+    }
+}
+
+// ─── b2_kv_evict_paged ───
+//
+// Selection per (sequence, kv head): the slots become keys that order as the
+// contract does (0: not mapped, the largest: always kept, else the weight's
+// order), and the k-th largest key is found 8 bits at a time from histograms.
+// Slots above it are kept, and as many of those equal to it as are missing,
+// lowest first; block-wide scans give their places in slot order.
+constexpr int kSelThreads = 1024;
+
+__device__ __forceinline__ uint32_t evict_key(const b2p::Batch& bt, const float* w, long long ldw, int s, int j, int len,
+                                              int sink, int recent) {
+    if (bt.page(s, j) < 0) return 0u;
+    if (j < sink || j >= len - recent) return 0xFFFFFFFFu;
+    // + 0 turns -0 into 0, so that the two are equal here too
+    const uint32_t k = b2::float_order((j < ldw ? w[j] : 0.f) + 0.f);
+    return min(max(k, 1u), 0xFFFFFFFEu);
+}
+
+// Inclusive scan over the CTA of one int per thread; total in *sum.
+__device__ __forceinline__ int block_scan(int v, int* ws, int* sum) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, v, o);
+        if (lane >= o) v += t;
+    }
+    if (lane == 31) ws[warp] = v;
+    __syncthreads();
+    int before = 0, all = 0;
+    for (int i = 0; i < kSelThreads / 32; i++) {
+        if (i < warp) before += ws[i];
+        all += ws[i];
+    }
+    __syncthreads();
+    *sum = all;
+    return v + before;
+}
+
+__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(b2p::Batch bt, const float* __restrict__ weights,
+                                                                   long long ldw, int nkv, int budget, int sink,
+                                                                   int recent, int* __restrict__ kept,
+                                                                   float* __restrict__ dst_weights,
+                                                                   int* __restrict__ new_len) {
+    __shared__ int hist[256];
+    __shared__ int ws[kSelThreads / 32];
+    __shared__ int sh[2];
+    b2::pdl_trigger();
+    b2::pdl_wait();
+    const int s = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
+    const int n = bt.kv_len[s];
+    const long long cap = (long long)bt.max_pages << bt.page_shift;
+    const int len = n < 0 ? 0 : (int)((long long)n < cap ? n : cap);
+    const float* w = weights + ((size_t)s * nkv + g) * ldw;
+    // mapped slots
+    int cnt = 0, mapped;
+    for (int j = tid; j < len; j += kSelThreads) cnt += bt.page(s, j) >= 0;
+    block_scan(cnt, ws, &mapped);
+    const int k = min(mapped, budget);
+    if (g == 0 && tid == 0) new_len[s] = k;
+    if (k == 0) return;
+    uint32_t prefix = 0;
+    int need = k;  // slots still to take among those that match the prefix
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int j = tid; j < len; j += kSelThreads) {
+            const uint32_t key = evict_key(bt, w, ldw, s, j, len, sink, recent);
+            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            int b = 255, sum = 0;
+            while (b > 0 && sum + hist[b] < need) sum += hist[b--];
+            sh[0] = b;
+            sh[1] = need - sum;
+        }
+        __syncthreads();
+        prefix |= (uint32_t)sh[0] << shift;
+        need = sh[1];
+        __syncthreads();
+    }
+    // prefix is the k-th largest key; `need` of the slots that equal it are kept
+    int ties = 0, out = 0;
+    const size_t o0 = ((size_t)s * nkv + g) * budget;
+    for (int b = 0; b < len; b += kSelThreads) {
+        const int j = b + tid;
+        const uint32_t key = j < len ? evict_key(bt, w, ldw, s, j, len, sink, recent) : 0u;
+        const bool eq = j < len && key == prefix;
+        int all;
+        const int rank = ties + block_scan(eq ? 1 : 0, ws, &all);
+        ties += all;
+        const bool take = (j < len && key > prefix) || (eq && rank <= need);
+        const int at = out + block_scan(take ? 1 : 0, ws, &all) - 1;
+        out += all;
+        if (take) {
+            kept[o0 + at] = j;
+            if (dst_weights) dst_weights[o0 + at] = j < ldw ? w[j] : 0.f;
+        }
+    }
+}
+
+// Moves the kept rows: 16 bytes per thread, K and V of a row by neighbouring
+// threads.
+constexpr int kMoveThreads = 256;
+
+template <int HD>
+__global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(b2p::Batch bt, PageStrides pg, int budget,
+                                                                  const int* __restrict__ dst_table, int dst_max_pages,
+                                                                  const int* __restrict__ kept,
+                                                                  const int* __restrict__ new_len) {
+    constexpr int C = HD / 8;  // 16-byte chunks of a row
+    constexpr int kRows = kMoveThreads / (2 * C);
+    b2::pdl_trigger();
+    b2::pdl_wait();
+    const int s = blockIdx.z, g = blockIdx.y, nkv = gridDim.y, n = new_len[s];
+    const int c = threadIdx.x % C, which = threadIdx.x / C % 2;
+    uint16_t* pool = which ? pg.v : pg.k;
+    const int mask = (1 << bt.page_shift) - 1;
+    for (int j = blockIdx.x * kRows + threadIdx.x / (2 * C); j < n; j += gridDim.x * kRows) {
+        const int dp = j >> bt.page_shift;
+        if (dp >= dst_max_pages) break;
+        const int to = dst_table[(size_t)s * dst_max_pages + dp];
+        const int from = kept[((size_t)s * nkv + g) * budget + j];
+        if (to < 0 || to >= bt.n_pages) continue;
+        const int p = bt.page(s, from);
+        if (p < 0) continue;
+        const uint4 v = *reinterpret_cast<const uint4*>(pool + p * pg.page + g * pg.head + (from & mask) * pg.row + c * 8);
+        *reinterpret_cast<uint4*>(pool + to * pg.page + g * pg.head + (j & mask) * pg.row + c * 8) = v;
+    }
+}
+
+}  // namespace
+
+extern "C" int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int M, int nq, int nkv, int hd,
+                                   const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_tab,
+                                   const float* sin_tab, int max_pos, int rope_style, const int* pos,
+                                   const B2PagedKV* kv, b2_stream_t s) {
+    int rc = b2_paged_check("b2_qk_rope_kv_paged", kv, nkv, hd, true);
+    if (rc) return rc;
+    if (!q16 || !qkv || !cos_tab || !sin_tab || M < 0 || nq <= 0 || max_pos <= 0 || (rope_style != 0 && rope_style != 1))
+        return b2_set_error(B2_ERR_INVALID_ARG, "b2_qk_rope_kv_paged: bad arguments");
+    if (ldqkv < (nq + 2 * nkv) * hd || ldq < nq * hd || ldqkv % 4 || ldq % 4 ||
+        (reinterpret_cast<uintptr_t>(qkv) & 15) || (reinterpret_cast<uintptr_t>(q16) & 7))
+        return b2_set_error(B2_ERR_INVALID_ARG,
+                            "b2_qk_rope_kv_paged: rows must be aligned (qkv 16 bytes, ldqkv %% 4; q16 8 bytes, ldq %% 4) "
+                            "and hold every head");
+    if (M == 0 || kv->n_seqs == 0) return 0;
+    const long long jobs = (long long)M * ((nq + 2 * nkv + kHeads - 1) / kHeads);
+    const long long grid = (jobs + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
+    if (grid > 0x7fffffffll) return b2_set_error(B2_ERR_INVALID_ARG, "b2_qk_rope_kv_paged: too many rows");
+    const PageStrides pg{kv->k_pages, kv->v_pages, kv->page_stride, kv->head_stride, kv->row_stride};
+    const cudaError_t e =
+        b2::launch_pdl(hd == 128 ? append_kernel<128> : append_kernel<64>, dim3((unsigned)grid), dim3(kAppendThreads), 0,
+                       (cudaStream_t)s, reinterpret_cast<__half*>(q16), ldq, qkv, ldqkv, nq, nkv, q_norm_w, k_norm_w,
+                       eps, cos_tab, sin_tab, max_pos, rope_style, pos, b2p::make_batch(kv, M), pg);
+    if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_qk_rope_kv_paged: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const float* weights, long long ldw, int budget,
+                                 int sink, int recent, const int* dst_table, int dst_max_pages, int* kept,
+                                 float* dst_weights, int* new_len, b2_stream_t s) {
+    int rc = b2_paged_check("b2_kv_evict_paged", kv, nkv, hd, false);
+    if (rc) return rc;
+    if (!weights || !dst_table || !kept || !new_len || ldw < 0 || budget < 0 || sink < 0 || recent < 0 ||
+        dst_max_pages <= 0 || (long long)sink + recent > budget || nkv > 65535)
+        return b2_set_error(B2_ERR_INVALID_ARG, "b2_kv_evict_paged: bad arguments (sink + recent <= budget)");
+    if (kv->n_seqs == 0) return 0;
+    const b2p::Batch bt = b2p::make_batch(kv, 0);
+    const PageStrides pg{kv->k_pages, kv->v_pages, kv->page_stride, kv->head_stride, kv->row_stride};
+    cudaStream_t st = (cudaStream_t)s;
+    cudaError_t e = b2::launch_pdl(evict_select_kernel, dim3(nkv, kv->n_seqs), dim3(kSelThreads), 0, st, bt, weights, ldw,
+                                   nkv, budget, sink, recent, kept, dst_weights, new_len);
+    if (e == cudaSuccess && budget > 0) {
+        const int rows = kMoveThreads / (2 * (hd / 8));
+        const int want = (budget + rows - 1) / rows;
+        const dim3 grid(want < 4096 ? want : 4096, nkv, kv->n_seqs);
+        e = b2::launch_pdl(hd == 128 ? evict_move_kernel<128> : evict_move_kernel<64>, grid, dim3(kMoveThreads), 0, st, bt,
+                           pg, budget, dst_table, dst_max_pages, (const int*)kept, (const int*)new_len);
+    }
+    if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_kv_evict_paged: %s", cudaGetErrorString(e));
+    return 0;
+}

@@ -78,6 +78,14 @@ class B2KVRef(ctypes.Structure):
                 ("rows_seq", c_vp), ("pos", c_vp), ("n_seqs", c_int)]
 
 
+class B2PagedKV(ctypes.Structure):
+    """One layer's paged KV cache and the batch's rows (B2PagedKV of include/b2_kernels.h)."""
+    _fields_ = [("k_pages", c_vp), ("v_pages", c_vp), ("page_stride", ctypes.c_longlong),
+                ("head_stride", ctypes.c_longlong), ("row_stride", ctypes.c_longlong), ("n_pages", c_int),
+                ("page_size", c_int), ("n_seqs", c_int), ("max_pages", c_int), ("page_table", c_vp),
+                ("kv_len", c_vp), ("q_start", c_vp)]
+
+
 # name -> (restype, argtypes); every symbol of include/matmul_decoder.h and
 # include/b2_kernels.h that has a non-inline definition.
 SIGNATURES = {
@@ -171,6 +179,15 @@ SIGNATURES = {
     "b2_attention_blocks_split": (c_int, [c_int, c_int]),
     "b2_attention_blocks": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_int, c_vp,
                                     c_vp]),
+    "b2_qk_rope_kv_paged": (c_int, [c_vp, c_int, c_vp, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_float,
+                                    c_vp, c_vp, c_int, c_int, c_vp, c_vp, c_vp]),
+    "b2_attention_paged_workspace": (c_size, [c_int, c_int, c_int, c_int, c_int]),
+    "b2_attention_paged": (c_int, [c_vp, c_vp, c_vp, c_int, c_int, c_int, c_int, c_int, c_int, c_vp, c_vp, c_vp,
+                                   c_vp]),
+    "b2_attention_paged_weights": (c_int, [c_vp, c_vp, ctypes.c_longlong, c_vp, c_int, c_vp, c_int, c_int, c_int,
+                                           c_int, c_int, c_vp, c_vp, c_vp]),
+    "b2_kv_evict_paged": (c_int, [c_vp, c_int, c_int, c_vp, ctypes.c_longlong, c_int, c_int, c_int, c_vp, c_int,
+                                  c_vp, c_vp, c_vp, c_vp]),
     "b2_lm_head_workspace": (c_size, [c_int, c_int]),
     "b2_loop_advance": (c_int, [c_vp, c_vp, c_int, c_vp]),
     "b2_lm_head_noalloc_max_keys": (c_size, []),

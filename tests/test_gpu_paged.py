@@ -1,0 +1,648 @@
+"""The paged KV cache operators (b2_qk_rope_kv_paged, b2_attention_paged,
+b2_attention_paged_weights, b2_kv_evict_paged) against a plain 64-bit form.
+
+Everything a sequence does not own holds NaN: slots past kv_len, unmapped
+pages, spare pages, padding columns of the row arrays.  What a call must leave
+alone holds a marker and is compared bit by bit.
+
+Tolerances.  u = 2^-11 is half a step of FP16.  The score of a row and a slot is
+a sum of hd exact products added in FP32, in any order and with truncation:
+off by at most e = (hd + 2) 2^-23 sum|q k| / sqrt(hd), and its exponential by a
+factor 1 +- (e + 2^-20).  The softmax weights are rounded to FP16 (u each), the
+output too, so an output may be off by u |o| + (u + 2 (e + 2^-20)) sum p |v|, plus
+half of FP16's smallest subnormal step.  The second-order terms are covered by the factor 1.01."""
+from __future__ import annotations
+
+import ctypes
+import math
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+pytestmark = pytest.mark.gpu
+
+import b200_decoder as bd  # noqa: E402
+
+if not torch.cuda.is_available():  # pragma: no cover - CPU containers
+    pytest.skip("needs a CUDA device", allow_module_level=True)
+
+DEV = torch.device("cuda:0")
+U = 2.0 ** -11
+F64 = torch.float64
+
+
+def stream():
+    return torch.cuda.current_stream().cuda_stream
+
+
+class Paged:
+    """A batch over a paged cache.  seqs: (new rows, kv_len, unmapped page indexes)."""
+
+    def __init__(self, seqs, nq=16, nkv=8, hd=128, page=64, layout="head", seed=0, tail=0, scale=1.0, bad=-1,
+                 extra_pages=3, extra_cols=0):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        r = np.random.default_rng(seed)
+        self.seqs, self.nq, self.nkv, self.hd, self.page, self.G = seqs, nq, nkv, hd, page, nq // nkv
+        B = len(seqs)
+        self.width = max([1] + [-(-n // page) for _, n, _ in seqs]) + extra_cols
+        count = sum(-(-n // page) for _, n, _ in seqs)
+        self.n_pages = count + extra_pages
+        order = r.permutation(self.n_pages)
+        table = np.full((B, self.width), bad, np.int64)
+        at = 0
+        for s, (_, n, holes) in enumerate(seqs):
+            for p in range(-(-n // page)):
+                if p not in holes:
+                    table[s, p] = order[at]
+                at += 1
+        self.spare = [int(x) for x in order[at:]]
+        self.table = torch.from_numpy(table.astype(np.int32)).to(DEV)
+        self.kv_len = torch.tensor([n for _, n, _ in seqs], dtype=torch.int32, device=DEV)
+        starts = np.concatenate([[0], np.cumsum([q for q, _, _ in seqs])])
+        self.rows = int(starts[-1])
+        self.M = self.rows + tail
+        self.starts = starts
+        self.q_start = torch.from_numpy(starts.astype(np.int32)).to(DEV)
+        self.k, self.v = self._pools(layout)
+        self.q16 = (torch.randn(max(1, self.M), nq * hd + 8, generator=g, device=DEV) * scale).half()
+        self.q16[:, nq * hd:] = math.nan  # padding columns
+        for s, (_, n, holes) in enumerate(seqs):
+            for p in range(-(-n // page)):
+                if p in holes:
+                    continue
+                m = min(page, n - p * page)
+                for t in (self.k, self.v):
+                    t[table[s, p], :, :m] = (torch.randn(nkv, m, hd, generator=g, device=DEV) * scale).half()
+        size = bd.capi().b2_attention_paged_workspace(B, max(1, self.M), nq, nkv, hd)
+        self.work = torch.zeros(size, dtype=torch.uint8, device=DEV)
+        self.err = torch.zeros(1, dtype=torch.int32, device=DEV)
+        self.max_q = max([1] + [q for q, _, _ in seqs])
+
+    def _pools(self, layout):
+        n, h, p, d = self.n_pages, self.nkv, self.page, self.hd
+        nan = lambda *shape: torch.full(shape, math.nan, dtype=torch.float16, device=DEV)  # noqa: E731
+        if layout == "head":
+            return nan(n, h, p, d), nan(n, h, p, d)
+        if layout == "token":
+            return nan(n, p, h, d).transpose(1, 2), nan(n, p, h, d).transpose(1, 2)
+        both = nan(n, 3, h, p, d + 8)  # K and V of one layer among others, padded rows
+        return both[:, 0, :, :, :d], both[:, 2, :, :, :d]
+
+    def kv(self, q_start=None):
+        k, qs = self.k, self.q_start if q_start is None else q_start
+        assert k.stride() == self.v.stride() and k.stride(3) == 1
+        return bd.B2PagedKV(k.data_ptr(), self.v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), self.n_pages,
+                            self.page, len(self.seqs), self.table.shape[1], self.table.data_ptr(),
+                            self.kv_len.data_ptr(), qs.data_ptr())
+
+    def attend(self, max_q=None, want_lse=True, st=None):
+        out = torch.full((max(1, self.M), self.nq * self.hd), 7.0, dtype=torch.float16, device=DEV)
+        lse = torch.full((max(1, self.M), self.nq), 7.0, device=DEV)
+        bd.check(bd.capi().b2_attention_paged(
+            out.data_ptr(), lse.data_ptr() if want_lse else None, self.q16.data_ptr(), self.q16.stride(0), self.M,
+            self.max_q if max_q is None else max_q, self.nq, self.nkv, self.hd, ctypes.byref(self.kv()),
+            self.work.data_ptr(), self.err.data_ptr(), stream() if st is None else st), "b2_attention_paged")
+        return out, lse
+
+    def weigh(self, lse, prev, out, max_q=None):
+        bd.check(bd.capi().b2_attention_paged_weights(
+            out.data_ptr(), None if prev is None else prev.data_ptr(), out.stride(1), self.q16.data_ptr(),
+            self.q16.stride(0), lse.data_ptr(), self.M, self.max_q if max_q is None else max_q, self.nq, self.nkv,
+            self.hd, ctypes.byref(self.kv()), self.err.data_ptr(), stream()), "b2_attention_paged_weights")
+        return out
+
+    def slots(self, s):
+        """Mapped slots below kv_len of sequence s (host list) and their K, V [slot][head][hd] in 64 bits."""
+        n = self.seqs[s][1]
+        row = self.table[s].tolist()
+        js = [j for j in range(min(n, len(row) * self.page)) if 0 <= row[j // self.page] < self.n_pages]
+        pg = torch.tensor([row[j // self.page] for j in js], dtype=torch.long, device=DEV)
+        off = torch.tensor([j % self.page for j in js], dtype=torch.long, device=DEV)
+        j = torch.tensor(js, dtype=torch.long, device=DEV)
+        return j, self.k[pg, :, off].to(F64), self.v[pg, :, off].to(F64)
+
+    def reference(self):
+        """out, lse, the tolerance of out, and that of lse, for the rows of the sequences."""
+        nq, hd, G = self.nq, self.hd, self.G
+        out = torch.zeros(self.rows, nq, hd, dtype=F64, device=DEV)
+        lse = torch.full((self.rows, nq), -math.inf, dtype=F64, device=DEV)
+        tol, tl = torch.zeros_like(out), torch.zeros_like(lse)
+        for s, (q, n, _) in enumerate(self.seqs):
+            j, K, V = self.slots(s)
+            if q == 0 or len(j) == 0:
+                continue
+            r = slice(int(self.starts[s]), int(self.starts[s]) + q)
+            Q = self.q16[r, :nq * hd].to(F64).view(q, nq, hd)
+            K, V = (t.repeat_interleave(G, 1) for t in (K, V))
+            x = torch.einsum("rhd,jhd->hrj", Q, K) / math.sqrt(hd)
+            mag = torch.einsum("rhd,jhd->hrj", Q.abs(), K.abs()) / math.sqrt(hd)
+            sees = j[None] <= (n - q + torch.arange(q, device=DEV))[:, None]
+            x = x.masked_fill(~sees, -math.inf)
+            m = x.amax(-1, keepdim=True)
+            p = (x - torch.where(m == -math.inf, 0.0, m)).exp()
+            l = p.sum(-1, keepdim=True)
+            p = p / torch.where(l > 0, l, 1.0)
+            e = (hd + 2) * 2.0 ** -23 * mag.masked_fill(~sees, 0).amax(-1) + 2.0 ** -20
+            o = torch.einsum("hrj,jhd->rhd", p, V)
+            a = torch.einsum("hrj,jhd->rhd", p, V.abs())
+            out[r] = o
+            tol[r] = U * o.abs() + (U + 2 * e.T[..., None]) * a
+            lse[r] = (m + l.log())[..., 0].T
+            tl[r] = e.T + 2.0 ** -21 * (1 + lse[r].abs().nan_to_num(posinf=0))
+        return out.reshape(self.rows, -1), lse, 1.01 * tol.reshape(self.rows, -1) + 2.0 ** -25, tl
+
+
+def check_attention(b, out, lse, max_q=None):
+    """out and lse of a call on b, with rows past max_q of a sequence and the tail untouched."""
+    assert b.err.item() == 0
+    assert not b.work[:4096].any(), "counters stay zero"
+    ro, rl, tol, tl = b.reference()
+    done = torch.zeros(out.shape[0], dtype=torch.bool, device=DEV)
+    for s, (q, _, _) in enumerate(b.seqs):
+        a = int(b.starts[s])
+        done[a:a + min(q, q if max_q is None else max_q)] = True
+    assert bool((out[~done] == 7).all()) and bool((lse[~done] == 7).all())
+    n = b.rows
+    d = (out[:n].to(F64) - ro).abs()
+    ok = (d <= tol) | ~done[:n, None]
+    assert bool(ok.all()), (int((~ok).sum()), float((d / tol)[done[:n]].max()), torch.nonzero(~ok)[:4].tolist())
+    dl = lse[:n].to(F64)
+    empty = rl == -math.inf
+    assert bool(((dl == -math.inf) == empty)[done[:n]].all())
+    okl = ((dl - rl).abs() <= tl) | empty | ~done[:n, None]
+    assert bool(okl.all()), float(((dl - rl).abs() / tl)[~empty & done[:n, None]].max())
+
+
+HEADS = [(16, 8, 128), (16, 4, 64), (3, 1, 128), (14, 2, 128), (32, 4, 64), (5, 1, 64), (8, 8, 128), (16, 1, 128)]
+
+
+@pytest.mark.parametrize("page", [16, 32, 64, 128])
+@pytest.mark.parametrize("nq,nkv,hd", HEADS)
+def test_attention_lengths(nq, nkv, hd, page):
+    """Cached lengths from nothing to several blocks, one to a few new rows, idle sequences."""
+    seqs = [(1, n, ()) for n in (1, 2, 15, 16, 17, 63, 64, 65, 127, 128, 129, 257, 1000)]
+    seqs += [(0, 40, ()), (0, 0, ()), (2, 2, ()), (3, 66, ()), (2, 300, ())]
+    b = Paged(seqs, nq, nkv, hd, page, layout=["head", "token", "mixed"][page % 3], seed=page + nq, tail=3)
+    check_attention(b, *b.attend())
+
+
+@pytest.mark.parametrize("q", [2, 4, 5, 8, 9, 16, 17, 33, 64, 65, 100, 128, 130, 257, 400])
+@pytest.mark.parametrize("nq,nkv,hd,page", [(16, 8, 128, 64), (16, 4, 64, 16), (3, 1, 128, 32), (16, 1, 64, 128),
+                                            (7, 1, 128, 16)])
+def test_attention_chunks(nq, nkv, hd, page, q):
+    """Chunks of new rows behind caches of several lengths, next to single tokens."""
+    seqs = [(q, q, ()), (1, 70, ()), (q, q + 1, ()), (q - 1, q + 63, ()), (0, 9, ()), (q, q + 517, ()), (1, 1, ())]
+    b = Paged(seqs, nq, nkv, hd, page, layout="token" if q % 2 else "head", seed=q, tail=1)
+    check_attention(b, *b.attend())
+
+
+@pytest.mark.parametrize("page", [16, 64, 128])
+@pytest.mark.parametrize("q", [1, 3, 70, 200])
+@pytest.mark.parametrize("bad", [-1, 1 << 30, -(1 << 31), None])
+def test_attention_unmapped_pages(page, q, bad):
+    """Unmapped pages in front, in the middle, at the end and everywhere; rows that see nothing at all."""
+    n = 5 * page + 3 + q
+    k = -(-n // page)
+    seqs = [(q, n, (0,)), (q, n, (0, 1, 2)), (q, n, (2,)), (q, n, (1, 3)), (q, n, (k - 1,)), (q, n, tuple(range(k))),
+            (q, n, (0, k - 1)), (q, n, ()), (q, q, tuple(range(-(-q // page))))]
+    if bad is None:  # the first id past the pool
+        bad = sum(-(-m // page) for _, m, _ in seqs) + 3
+    b = Paged(seqs, 8, 4, 128, page, seed=page + q, bad=bad)
+    check_attention(b, *b.attend())
+
+
+@pytest.mark.parametrize("q", [2, 40, 150])
+def test_attention_fewer_cached_than_new(q):
+    """kv_len below the number of new rows: the first rows have no slot and see nothing."""
+    b = Paged([(q, q - 1, ()), (q, 1, ()), (q, 0, ()), (1, 0, ()), (q, q // 2, ())], 4, 2, 64, 16, seed=q)
+    check_attention(b, *b.attend())
+
+
+@pytest.mark.parametrize("q", [1, 6, 90])
+def test_attention_kv_len_beyond_table(q):
+    """kv_len past what the table can hold: the slots behind it are not there."""
+    b = Paged([(q, 128, ()), (q, 100, ())], 4, 2, 128, 64, seed=q)
+    b.table = b.table[:, :1].contiguous()
+    b.width = 1
+    check_attention(b, *b.attend())
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page,q,n", [(2, 1, 128, 128, 1, 30_011), (14, 2, 128, 16, 1, 20_000),
+                                                (16, 8, 64, 64, 4, 9_000), (4, 4, 128, 32, 1, 12_345),
+                                                (2, 1, 128, 64, 100, 20_100), (8, 1, 64, 32, 70, 33_333)])
+def test_attention_long(nq, nkv, hd, page, q, n):
+    """Contexts that many CTAs share; the pieces are merged in a fixed order, so calls repeat bit by bit."""
+    b = Paged([(q, n, ())], nq, nkv, hd, page, seed=n)
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    for _ in range(3):
+        o2, l2 = b.attend()
+        assert torch.equal(out, o2) and torch.equal(lse, l2)
+
+
+@pytest.mark.parametrize("seqs_n", [1, 31, 32, 33, 64, 500, 1024])
+def test_attention_many_sequences(seqs_n):
+    r = np.random.default_rng(seqs_n)
+    seqs = [(int(r.integers(0, 3)), int(r.integers(3, 90)), ()) for _ in range(seqs_n)]
+    b = Paged(seqs, 4, 2, 64, 16, seed=seqs_n, tail=2)
+    check_attention(b, *b.attend())
+
+
+@pytest.mark.parametrize("seqs,max_q", [([(9, 30, ()), (1, 5, ())], 4), ([(300, 300, ()), (2, 70, ())], 130),
+                                        ([(70, 200, ())], 1)])
+def test_attention_max_q_cuts(seqs, max_q):
+    """Rows past the first max_q of a sequence are left as they were."""
+    b = Paged(seqs, 4, 2, 128, 32, seed=max_q)
+    out, lse = b.attend(max_q=max_q)
+    check_attention(b, out, lse, max_q=max_q)
+
+
+def test_attention_without_lse():
+    b = Paged([(1, 700, ()), (90, 300, ())], seed=3)
+    out, _ = b.attend()
+    again, untouched = b.attend(want_lse=False)
+    assert torch.equal(out, again) and bool((untouched == 7).all())
+
+
+@pytest.mark.parametrize("q", [1, 5, 130])
+def test_attention_extreme_scores(q):
+    """Scores of +-2000 (one slot takes everything), equal scores, and the type's lowest values in K."""
+    b = Paged([(q, 200 + q, ()), (q, 300 + q, ()), (q, 150 + q, ())], 4, 2, 128, 64, seed=q, scale=12.0)
+    pages = b.table.tolist()
+    for p in pages[1][:5]:
+        b.k[p][~b.k[p].isnan()] = 0.25  # every slot weighs the same
+    b.k[pages[2][0], :, 3] = -65504.0
+    b.k[pages[2][1], :, 5] = 65504.0
+    # scores near 1e6 x 2^-17 relative error say nothing about a softmax, so q is small there
+    r = slice(int(b.starts[2]), int(b.starts[2]) + q)
+    b.q16[r, :512] *= 2.0 ** -12
+    check_attention(b, *b.attend())
+
+
+@pytest.mark.parametrize("q", [1, 4, 140])
+def test_attention_non_finite_values(q):
+    """Infinities in slots nobody sees change nothing; a NaN in a seen slot reaches the rows that see it."""
+    b = Paged([(q, 160 + q, (1,)), (q, 90 + q, ())], 4, 2, 128, 64, seed=q)
+    for p in b.spare:
+        b.k[p], b.v[p] = math.inf, -math.inf
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    page = int(b.table[1, 0])
+    b.k[page, 1, 7] = math.nan  # kv head 1 of sequence 1
+    out2, lse2 = b.attend()
+    r = slice(int(b.starts[1]), int(b.starts[1]) + q)
+    assert bool(out2[r, 256:].isnan().all()) and bool(lse2[r, 2:].isnan().all())
+    out2[r, 256:], lse2[r, 2:] = out[r, 256:], lse[r, 2:]
+    assert torch.equal(out, out2) and torch.equal(lse, lse2)
+
+
+@pytest.mark.parametrize("q", [1, 90])
+def test_attention_graph_streams_and_shared_workspace(q):
+    """Captured and replayed with other lengths, on another stream, with one workspace for calls of other shapes."""
+    small = Paged([(1, 33, ())], 8, 1, 64, 16, seed=9)
+    b = Paged([(q, 500 + q, ()), (q, 1200 + q, ()), (1, 64, ())], seed=q)
+    small.work = b.work
+    side = torch.cuda.Stream()
+    b.attend()  # the first call sets the kernels up outside the capture
+    torch.cuda.synchronize()
+    out = torch.full((b.M, b.nq * b.hd), 7.0, dtype=torch.float16, device=DEV)
+    lse = torch.full((b.M, b.nq), 7.0, device=DEV)
+    kv = b.kv()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        bd.check(bd.capi().b2_attention_paged(
+            out.data_ptr(), lse.data_ptr(), b.q16.data_ptr(), b.q16.stride(0), b.M, b.max_q, b.nq, b.nkv, b.hd,
+            ctypes.byref(kv), b.work.data_ptr(), b.err.data_ptr(), torch.cuda.current_stream().cuda_stream))
+    graph.replay()
+    torch.cuda.synchronize()
+    check_attention(b, out, lse)
+    check_attention(small, *small.attend())
+    # shorter contexts for the same graph: the first two sequences lose their newest slots
+    b.seqs = [(q, 100 + q, ()), (q, 700 + q, ()), (1, 64, ())]
+    b.kv_len.copy_(torch.tensor([n for _, n, _ in b.seqs], dtype=torch.int32))
+    graph.replay()
+    torch.cuda.synchronize()
+    check_attention(b, out, lse)
+
+
+# ── append ──
+
+
+def rope_reference(b, qkv, qn, kn, cos, sin, pos, style):
+    """q and k rows [M][head][hd] in 64 bits, and their rounding tolerances' magnitudes."""
+    nq, nkv, hd = b.nq, b.nkv, b.hd
+    x = qkv[:, :(nq + 2 * nkv) * hd].to(F64).view(len(qkv), nq + 2 * nkv, hd)
+    y = x[:, :nq + nkv].clone()
+    for lo, hi, w in ((0, nq, qn), (nq, nq + nkv, kn)):
+        if w is not None:
+            y[:, lo:hi] = y[:, lo:hi] / (y[:, lo:hi].square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.to(F64)
+    c, s = cos[pos.clamp(0, len(cos) - 1).long()].to(F64)[:, None], sin[pos.clamp(0, len(cos) - 1).long()].to(F64)[:, None]
+    z, mag = torch.empty_like(y), torch.empty_like(y)
+    a, d = (y[..., 0::2], y[..., 1::2]) if style == 0 else (y[..., :hd // 2], y[..., hd // 2:])
+    for t, u, v, m in ((z, a * c - d * s, d * c + a * s, 0), (mag, (a * c).abs() + (d * s).abs(), (d * c).abs() + (a * s).abs(), 1)):
+        if style == 0:
+            t[..., 0::2], t[..., 1::2] = u, v
+        else:
+            t[..., :hd // 2], t[..., hd // 2:] = u, v
+    return z, x[:, nq + nkv:], mag
+
+
+@pytest.mark.parametrize("style", [0, 1])
+@pytest.mark.parametrize("norm", [True, False])
+@pytest.mark.parametrize("nq,nkv,hd,page,layout", [(16, 8, 128, 64, "head"), (3, 1, 128, 16, "token"),
+                                                   (14, 2, 64, 32, "mixed"), (5, 5, 64, 128, "head"),
+                                                   (1, 1, 128, 64, "token")])
+def test_append(nq, nkv, hd, page, layout, norm, style):
+    """Rows of sequences of every kind: idle, one, a chunk over pages, slots that are unmapped, negative or past the
+    table, positions outside the angle tables, padding rows."""
+    seqs = [(1, 1, ()), (0, 30, ()), (40, 170, ()), (1, 129, ()), (9, 9, ()), (5, 3, ()), (3, 200, (-(-200 // page) - 1,)),
+            (1, 64, ()), (0, 0, ()), (2, 65, ())]
+    b = Paged(seqs, nq, nkv, hd, page, layout, seed=nq + style, tail=2)
+    g = torch.Generator(device=DEV).manual_seed(nq)
+    width = (nq + 2 * nkv) * hd
+    qkv = torch.randn(b.M, width + 4, generator=g, device=DEV) * 2
+    qkv[:, width:] = math.nan
+    qn, kn = ((1 + 0.2 * torch.randn(hd, generator=g, device=DEV)) if norm else None for _ in range(2))
+    angle = torch.rand(400, hd // 2, generator=g, device=DEV, dtype=F64) * 6.3
+    cos, sin = angle.cos().float(), angle.sin().float()
+    slot = torch.cat([torch.arange(n - q, n) for q, n, _ in seqs] + [torch.zeros(2)]).int().to(DEV)
+    pos = (slot + 37).clamp(min=0)
+    pos[2], pos[50] = 400, -1  # outside the tables: these rows are left out
+    q16 = torch.full((b.M, nq * hd + 4), 7.0, dtype=torch.float16, device=DEV)
+    before = [t.clone() for t in (b.k, b.v)]
+    for p in (pos, None):
+        b.k.copy_(before[0]), b.v.copy_(before[1]), q16.fill_(7.0)
+        bd.check(bd.capi().b2_qk_rope_kv_paged(
+            q16.data_ptr(), q16.stride(0), qkv.data_ptr(), qkv.stride(0), b.M, nq, nkv, hd,
+            qn.data_ptr() if norm else None, kn.data_ptr() if norm else None, 1e-6, cos.data_ptr(), sin.data_ptr(), 400,
+            style, None if p is None else p.data_ptr(), ctypes.byref(b.kv()), stream()), "b2_qk_rope_kv_paged")
+        at = slot if p is None else p
+        z, v, mag = rope_reference(b, qkv, qn, kn, cos, sin, at, style)
+        # FP32: the norm's three roundings and the sum of squares, two products and a sum: 16 half steps of the terms
+        tol = U * z.abs() + 16 * 2.0 ** -24 * mag + 2.0 ** -25
+        k_exp, v_exp = (t.to(F64) for t in before)
+        k_tol = torch.zeros_like(k_exp)
+        row = 0
+        for s, (q, n, holes) in enumerate(seqs):
+            for i in range(q):
+                m, j = row, n - q + i
+                row += 1
+                if not 0 <= int(at[m]) < 400:
+                    assert bool((q16[m] == 7).all())
+                    continue
+                d = (q16[m, :nq * hd].to(F64).view(nq, hd) - z[m, :nq]).abs()
+                assert bool((d <= tol[m, :nq]).all()), (m, float((d / tol[m, :nq]).max()))
+                if j < 0 or j // page in holes:
+                    continue
+                pg = int(b.table[s, j // page])
+                k_exp[pg, :, j % page], k_tol[pg, :, j % page] = z[m, nq:], tol[m, nq:]
+                v_exp[pg, :, j % page] = v[m].half().to(F64)
+        assert bool((q16[b.rows:] == 7).all()) and bool((q16[:, nq * hd:] == 7).all())
+        same = (b.k.to(F64) - k_exp).abs() <= k_tol
+        assert bool((same | (b.k.isnan() & k_exp.isnan())).all())
+        got = b.v.to(F64)
+        assert bool(((got == v_exp) | (got.isnan() & v_exp.isnan())).all())
+
+
+# ── attention weights ──
+
+
+def check_weights(b, lse, prev, out, ldw, mark):
+    for s, (q, n, _) in enumerate(b.seqs):
+        j, K, _ = b.slots(s)
+        r = slice(int(b.starts[s]), int(b.starts[s]) + q)
+        total = torch.zeros(b.nkv, max(1, n), dtype=F64, device=DEV)
+        tol = torch.zeros_like(total)
+        if q and len(j):
+            Q = b.q16[r, :b.nq * b.hd].to(F64).view(q, b.nkv, b.G, b.hd)
+            x = torch.einsum("rghd,jgd->ghrj", Q, K) / math.sqrt(b.hd)
+            mag = torch.einsum("rghd,jgd->ghrj", Q.abs(), K.abs()) / math.sqrt(b.hd)
+            le = lse[r].to(F64).view(q, b.nkv, b.G).permute(1, 2, 0)[..., None]
+            sees = (j[None] <= (n - q + torch.arange(q, device=DEV))[:, None]) & (le > -math.inf)
+            p = torch.where(sees, (x - le.nan_to_num(neginf=0)).exp(), 0.0)
+            e = (b.hd + 2) * 2.0 ** -23 * mag + 2.0 ** -22 * (x.abs() + le.nan_to_num(neginf=0).abs()) + 2.0 ** -20
+            total[:, j] = p.sum((1, 2))
+            tol[:, j] = (p * e).sum((1, 2)) + (q * b.G + 8) * 2.0 ** -24 * total[:, j]
+        m = min(n, ldw)
+        was = torch.zeros_like(total[:, :m]) if prev is None else prev[s, :, :m].to(F64)
+        d = (out[s, :, :m].to(F64) - (was + total[:, :m])).abs()
+        t = 1.01 * tol[:, :m] + 2.0 ** -23 * (was + total[:, :m]).abs()
+        assert bool((d <= t).all()), (s, float((d / t.clamp(min=1e-30)).max()))
+        assert bool((out[s, :, m:] == mark).all())
+    assert b.err.item() == 0
+
+
+@pytest.mark.parametrize("with_prev", [True, False])
+@pytest.mark.parametrize("nq,nkv,hd,page", [(16, 8, 128, 64), (14, 2, 64, 16), (3, 1, 128, 32), (16, 1, 64, 128)])
+@pytest.mark.parametrize("q", [1, 2, 7, 33, 130, 300])
+def test_weights(nq, nkv, hd, page, q, with_prev):
+    seqs = [(q, q, ()), (q, q + 1, ()), (1, 70, ()), (0, 40, ()), (q, q + 300, (1,)), (q, q - 1, ()), (1, 1, ()), (0, 0, ()),
+            (q, q + 129, (0, 1))]
+    b = Paged(seqs, nq, nkv, hd, page, layout="token" if q % 2 else "head", seed=q, tail=2)
+    _, lse = b.attend()
+    ldw = q + 310
+    prev = torch.rand(len(seqs), nkv, ldw, device=DEV) if with_prev else None
+    out = torch.full((len(seqs), nkv, ldw), 7.0, device=DEV)
+    b.weigh(lse, prev, out)
+    check_weights(b, lse, prev, out, ldw, 7.0)
+    again = torch.full_like(out, 7.0)
+    b.weigh(lse, prev, again)
+    assert torch.equal(out, again)
+    if with_prev:  # in place
+        here = torch.where(out == 7.0, 7.0, prev)
+        b.weigh(lse, here, here)
+        assert torch.equal(here, out)
+
+
+@pytest.mark.parametrize("q", [1, 200])
+def test_weights_of_one_row_sum_to_the_group(q):
+    """Every row gives each of its q heads a total of one."""
+    b = Paged([(q, 900 + q, ())], seed=q)
+    _, lse = b.attend()
+    out = b.weigh(lse, None, torch.zeros(1, b.nkv, 900 + q, device=DEV))
+    # 1100 slots of e ~ 2^-13 relative error at most
+    assert bool(((out.to(F64).sum(-1) / (q * b.G) - 1).abs() < 2.0 ** -12).all())
+
+
+def test_weights_narrow_rows_and_max_q():
+    """Weight rows shorter than the cache, and rows past max_q that give nothing."""
+    b = Paged([(5, 200, ()), (80, 100, ())], 4, 2, 64, 32, seed=4)
+    _, lse = b.attend()
+    out = torch.full((2, 2, 90), 7.0, device=DEV)
+    b.weigh(lse, None, out)
+    check_weights(b, lse, None, out, 90, 7.0)
+    few = lse.clone()
+    few[3:5], few[5 + 3:] = -math.inf, -math.inf
+    out2 = torch.full((2, 2, 90), 7.0, device=DEV)
+    b.weigh(lse, None, out2, max_q=3)
+    check_weights(b, few, None, out2, 90, 7.0)
+
+
+# ── eviction ──
+
+
+def evict(b, w, budget, sink, recent, dst, dst_weights=True):
+    B = len(b.seqs)
+    kept = torch.full((B, b.nkv, max(1, budget)), -7, dtype=torch.int32, device=DEV)
+    dw = torch.full((B, b.nkv, max(1, budget)), -7.0, device=DEV)
+    n = torch.full((B,), -7, dtype=torch.int32, device=DEV)
+    bd.check(bd.capi().b2_kv_evict_paged(
+        ctypes.byref(b.kv()), b.nkv, b.hd, w.data_ptr(), w.stride(1), budget, sink, recent, dst.data_ptr(), dst.shape[1],
+        kept.data_ptr(), dw.data_ptr() if dst_weights else None, n.data_ptr(), stream()), "b2_kv_evict_paged")
+    return kept, dw, n
+
+
+def evict_reference(b, w, budget, sink, recent):
+    """[(kept slots per kv head)] per sequence."""
+    got = []
+    for s, (_, n, _) in enumerate(b.seqs):
+        js = b.slots(s)[0].tolist()
+        heads = []
+        for g in range(b.nkv):
+            row = w[s, g].tolist()
+            val = lambda j: (row[j] if j < len(row) else 0.0) + 0.0  # noqa: E731
+            must = {j for j in js if j < sink or j >= n - recent}
+            rest = sorted((j for j in js if j not in must), key=lambda j: (math.isnan(val(j)), 0 if math.isnan(val(j)) else -val(j), j))
+            heads.append(sorted(list(must) + rest[:max(0, min(budget, len(js)) - len(must))]))
+        got.append(heads)
+    return got
+
+
+@pytest.mark.parametrize("budget,sink,recent", [(64, 4, 16), (100, 0, 0), (1, 0, 0), (1, 1, 0), (1, 0, 1), (37, 37, 0),
+                                                (200, 0, 200), (5000, 4, 100), (0, 0, 0)])
+@pytest.mark.parametrize("hd,page,layout", [(128, 64, "head"), (64, 16, "token"), (128, 32, "mixed")])
+def test_evict(budget, sink, recent, hd, page, layout):
+    seqs = [(0, 500, ()), (0, 1, ()), (0, 0, ()), (0, 64, ()), (0, 301, (0, 2)), (0, 150, tuple(range(-(-150 // page)))),
+            (0, 1500, (1,)), (0, 99, ())]
+    per = max(1, -(-budget // page))
+    b = Paged(seqs, 4, 2, hd, page, layout, seed=budget, extra_pages=per * len(seqs) + 2)
+    dst = torch.tensor(b.spare[:per * len(seqs)], dtype=torch.int32, device=DEV).view(len(seqs), per)
+    if per > 1:
+        dst[3, 1] = -1  # an unmapped destination
+    g = torch.Generator(device=DEV).manual_seed(budget)
+    w = torch.rand(len(seqs), 2, 1400, generator=g, device=DEV)  # narrower than the longest sequence
+    w[0, 0, :400] = 0.5        # equal weights: the lowest slots
+    w[0, 1, 100:300] = 0.0
+    w[0, 1, 150:160] = -0.0    # equal to 0
+    w[3, 0, 10:20] = math.nan  # last
+    w[3, 1, 5], w[3, 1, 7] = math.inf, -1.0
+    before = [t.clone() for t in (b.k, b.v)]
+    kept, dw, n = evict(b, w, budget, sink, recent, dst)
+    ref = evict_reference(b, w, budget, sink, recent)
+    k_exp, v_exp = (t.clone() for t in before)
+    for s, heads in enumerate(ref):
+        assert int(n[s]) == len(heads[0])
+        for h, js in enumerate(heads):
+            assert kept[s, h, :len(js)].tolist() == js, (s, h)
+            assert bool((kept[s, h, len(js):] == -7).all()) and bool((dw[s, h, len(js):] == -7).all())
+            if not js:
+                continue
+            j = torch.tensor(js, device=DEV)
+            exp = torch.where(j < 1400, w[s, h, j.clamp(max=1399)], 0.0)
+            assert bool(((dw[s, h, :len(js)] == exp) | exp.isnan()).all())
+            to = torch.arange(len(js), device=DEV)
+            on = dst[s, to // page] >= 0
+            src, at = b.table[s, j // page].long()[on], dst[s, to // page].long()[on]
+            for t, e in ((before[0], k_exp), (before[1], v_exp)):
+                e[at, h, (to % page)[on]] = t[src, h, (j % page)[on]]
+    for t, e in ((b.k, k_exp), (b.v, v_exp)):
+        assert bool(((t == e) | (t.isnan() & e.isnan())).all())
+    k2, _, n2 = evict(b, w, budget, sink, recent, dst, dst_weights=False)
+    assert torch.equal(k2, kept) and torch.equal(n2, n)
+
+
+@pytest.mark.parametrize("n,budget", [(40_000, 10_000), (40_000, 39_999), (70_001, 1), (20_000, 20_000)])
+def test_evict_long(n, budget):
+    page = 128
+    per = -(-budget // page)
+    b = Paged([(0, n, ()), (0, n // 3, ())], 2, 1, 64, page, seed=n, extra_pages=2 * per + 1)
+    dst = torch.tensor(b.spare[:2 * per], dtype=torch.int32, device=DEV).view(2, per)
+    w = (torch.rand(2, 1, n, device=DEV) * 50).floor() / 50  # many equal weights
+    kept, dw, got = evict(b, w, budget, min(2, budget), min(100, budget // 4), dst)
+    for s, heads in enumerate(evict_reference(b, w, budget, min(2, budget), min(100, budget // 4))):
+        assert kept[s, 0, :int(got[s])].tolist() == heads[0]
+        j = torch.tensor(heads[0], device=DEV)
+        to = torch.arange(len(j), device=DEV)
+        assert torch.equal(dw[s, 0, :len(j)], w[s, 0, j])
+        assert torch.equal(b.v[dst[s, to // page].long(), 0, to % page], b.v[b.table[s, j // page].long(), 0, j % page])
+
+
+# ── all of them, as a serving loop uses them ──
+
+
+def test_serving_loop():
+    """Two sequences: prompts in chunks, decode steps, then eviction to a budget, then more steps at positions that
+    the cache no longer counts.  Every step's attention is checked against the cache as it stands, the cache against
+    the rows it was given."""
+    nq, nkv, hd, page, budget = 8, 4, 128, 16, 48
+    L, G = bd.capi(), nq // nkv
+    n_pages = 64
+    k, v = (torch.full((n_pages, nkv, page, hd), math.nan, dtype=torch.float16, device=DEV) for _ in range(2))
+    free = list(np.random.default_rng(1).permutation(n_pages))
+    own = [[], []]
+    length, pos = [0, 0], [0, 0]
+    angle = torch.arange(512, device=DEV, dtype=F64)[:, None] * 1e4 ** (-torch.arange(hd // 2, device=DEV, dtype=F64) / 64)
+    cos, sin = angle.cos().float(), angle.sin().float()
+    g = torch.Generator(device=DEV).manual_seed(5)
+    weights = torch.zeros(2, nkv, 256, device=DEV)
+    work = torch.zeros(L.b2_attention_paged_workspace(2, 64, nq, nkv, hd), dtype=torch.uint8, device=DEV)
+    err = torch.zeros(1, dtype=torch.int32, device=DEV)
+    kept_rows = [[torch.zeros(0, hd, dtype=F64, device=DEV)] * nkv for _ in range(2)]  # K the cache should hold
+
+    def ints(a):
+        return torch.tensor(a, dtype=torch.int32, device=DEV)
+
+    for step, news in enumerate([(30, 1), (40, 25), (1, 1), (1, 0), "evict", (1, 1), (5, 1), (1, 60), "evict", (1, 1)]):
+        if news == "evict":
+            table = ints([o + [-1] * (16 - len(o)) for o in own])
+            per = -(-budget // page)
+            fresh = [[free.pop() for _ in range(per)] for _ in range(2)]
+            kv = bd.B2PagedKV(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), n_pages, page, 2, 16,
+                              table.data_ptr(), (kl := ints(length)).data_ptr(), None)
+            kept = torch.zeros(2, nkv, budget, dtype=torch.int32, device=DEV)
+            new_len, to = ints([0, 0]), ints(fresh)
+            moved = torch.zeros(2, nkv, budget, device=DEV)
+            bd.check(L.b2_kv_evict_paged(ctypes.byref(kv), nkv, hd, weights.data_ptr(), 256, budget, 4, 16, to.data_ptr(),
+                                         per, kept.data_ptr(), moved.data_ptr(), new_len.data_ptr(), stream()))
+            length = new_len.tolist()
+            assert length == [min(budget, n) for n in kl.tolist()]
+            weights.zero_()
+            for s in range(2):
+                free.extend(own[s])
+                own[s] = fresh[s][:-(-length[s] // page)]
+                free.extend(fresh[s][len(own[s]):])
+                weights[s, :, :length[s]] = moved[s, :, :length[s]]
+                for h in range(nkv):
+                    kept_rows[s][h] = kept_rows[s][h][kept[s, h, :length[s]].long()]
+            continue
+        for s in range(2):
+            length[s] += news[s]
+            while len(own[s]) * page < length[s]:
+                own[s].append(free.pop())
+        M = sum(news)
+        qkv = torch.randn(M, (nq + 2 * nkv) * hd, generator=g, device=DEV)
+        at = ints(list(range(pos[0], pos[0] + news[0])) + list(range(pos[1], pos[1] + news[1])))
+        table, kl, qs = ints([o + [-1] * (16 - len(o)) for o in own]), ints(length), ints([0, news[0], M])
+        kv = bd.B2PagedKV(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), n_pages, page, 2, 16,
+                          table.data_ptr(), kl.data_ptr(), qs.data_ptr())
+        b = Paged([(news[s], length[s], ()) for s in range(2)], nq, nkv, hd, page, extra_pages=0)
+        b.k, b.v, b.n_pages, b.table, b.work, b.err = k, v, n_pages, table, work, err
+        b.q16 = torch.zeros(M, nq * hd, dtype=torch.float16, device=DEV)
+        bd.check(L.b2_qk_rope_kv_paged(b.q16.data_ptr(), nq * hd, qkv.data_ptr(), qkv.stride(0), M, nq, nkv, hd, None, None,
+                                       1e-6, cos.data_ptr(), sin.data_ptr(), 512, 1, at.data_ptr(), ctypes.byref(kv),
+                                       stream()))
+        z, _, _ = rope_reference(b, qkv, None, None, cos, sin, at, 1)
+        out, lse = b.attend()
+        check_attention(b, out, lse)
+        before = weights.clone()
+        b.weigh(lse, weights, weights)
+        check_weights(b, lse, before, weights, 256, 0.0)
+        for s in range(2):
+            r = slice(int(b.starts[s]), int(b.starts[s]) + news[s])
+            _, K, _ = b.slots(s)
+            for h in range(nkv):
+                kept_rows[s][h] = torch.cat([kept_rows[s][h], z[r, nq + h]])
+                assert bool(((K[:, h] - kept_rows[s][h]).abs() <= U * kept_rows[s][h].abs() + 2.0 ** -18).all())
+            pos[s] += news[s]
+    assert err.item() == 0
