@@ -17,9 +17,10 @@ int b2_tensor_map_f16_5d(void* map, const void* base, const uint64_t (&dims)[5],
 // Host checks shared by the entry points; 0 or an error code with its message.
 int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool rows);
 // Tensor map of K or V pages: dimensions (64 dims, rows of a page, head_dim / 64,
-// kv heads, pages), boxes of box_rows rows and every dim: a box lands as
-// [head_dim / 64][box_rows][128 bytes], each 128-byte row swizzled.
-int b2_paged_map(CUtensorMap* map, const uint16_t* base, const B2PagedKV* kv, int nkv, int hd, int box_rows);
+// kv heads, pages), boxes of box_rows rows and box_halves times 64 dims: a box
+// lands as [box_halves][box_rows][128 bytes], each 128-byte row swizzled.
+int b2_paged_map(CUtensorMap* map, const uint16_t* base, const B2PagedKV* kv, int nkv, int hd, int box_rows,
+                 int box_halves);
 
 namespace b2p {
 
@@ -159,6 +160,47 @@ __device__ __forceinline__ int prefix_find(const int* pre, int n, int x) {
     return lo;
 }
 
+// What both attention kernels of a call take.
+struct AttnParams {
+    Batch bt;
+    const __half* q16;
+    int ldq;
+    __half* out16;
+    float* lse;
+    int max_q, nq, nkv, G;
+    int short_rows;  // sequences with at most this many (token, head) rows per kv head are the short kernel's
+    int* counters;   // zero between calls
+    float* part;     // the short kernel's partial tiles
+    struct Cut* cuts;       // [long CTAs] tiles that the long kernel left in pieces
+    float* long_part;       // their pieces
+    int long_ctas;          // CTAs of the long kernel (0: none launched)
+    int* err;
+};
+
+// A tile pair that the long kernel's CTA c (its owner) began and later CTAs
+// finished: pieces c, c + 1, ... wait for the merge.
+struct Cut {
+    int pieces;  // 0: none
+    int row0;    // first token row
+    int tokens;
+    int g;
+};
+// Floats of one piece: for each of two tiles o[hd / 4][128 rows][4], then
+// (maximum, sum)[2][128].  CTA c's slot 2 c holds a piece that continues a
+// pair, slot 2 c + 1 one that begins it.
+constexpr int kLongRows = 128;
+__host__ __device__ constexpr int long_piece_floats(int hd) { return 2 * kLongRows * (hd + 2); }
+
+constexpr float kLn2 = 0.69314718055994531f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// Factor of a piece with maximum m (log2 units) in a sum whose maximum is M.  A
+// piece that saw no slot has m = -inf and sums of 0; one that saw only NaN has
+// NaN sums, which the factor 1 keeps.
+__device__ __forceinline__ float piece_weight(float m, float M) { return m == -INFINITY ? 1.f : ex2(m - M); }
+
+__host__ __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
+
 // Host: dynamic shared memory opt-in, once per kernel and device.
 template <typename K>
 inline cudaError_t allow_smem(K kern, size_t bytes, std::atomic<unsigned long long>& done, int dev) {
@@ -170,3 +212,7 @@ inline cudaError_t allow_smem(K kern, size_t bytes, std::atomic<unsigned long lo
 }
 
 }  // namespace b2p
+
+// The long kernel (b2_paged_chunk.cu): launches it for the sequences with more
+// than p.short_rows rows and sets p.long_ctas.
+int b2_paged_attention_long(b2p::AttnParams& p, const B2PagedKV* kv, int hd, int dev, int sms, cudaStream_t s);

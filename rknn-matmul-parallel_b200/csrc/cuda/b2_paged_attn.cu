@@ -8,10 +8,8 @@
 
 namespace {
 
-using b2p::ex2;
-using b2p::smem_u32;
+using namespace b2p;
 
-constexpr float kLn2 = 0.69314718055994531f;
 // The weights are formed as 2^(s - m + kUp) with s and m in units of log2: the
 // FP16 copy that the product with V takes then keeps 11 bits down to 2^-28 of
 // the row's largest weight, where weights of a long row lie.  Sums carry the
@@ -33,18 +31,6 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
-
-struct AttnParams {
-    b2p::Batch bt;
-    const __half* q16;
-    int ldq;
-    __half* out16;
-    float* lse;
-    int max_q, nq, nkv, G, T;  // T: tokens of one tile
-    float* part;               // partial tiles
-    int* counters;             // [grid], zero between calls
-    int* err;
-};
 
 // ─── few rows per sequence: decode steps, drafted tokens ───
 //
@@ -86,24 +72,18 @@ struct ShortSmem {
     int pre[B2_PAGED_MAX_SEQS + 1];
 };
 
-// Factor of a piece with maximum m in a sum whose maximum is M.  A piece that
-// saw no slot has m = -inf and sums of 0; one that saw only NaN has NaN sums,
-// which the factor 1 keeps.
-__device__ __forceinline__ float piece_weight(float m, float M) { return m == -INFINITY ? 1.f : ex2(m - M); }
-
-__device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
-
 // A stretch's part of one tile: blocks [b0, b1) of the tile's nb.
 struct Seg {
     int s, g, i0, rows_t;  // sequence, kv head, first token, tokens
     int b0, b1, live;      // live: end of the blocks that some row of the tile sees
     int nb, x0;            // the tile's blocks, and where it starts on the line
-    b2p::Seq sq;
+    Seq sq;
 };
 
-__device__ __forceinline__ Seg find_seg(const AttnParams& p, const int* pre, int x, int x1) {
+// T: tokens of one tile.
+__device__ __forceinline__ Seg find_seg(const AttnParams& p, int T, const int* pre, int x, int x1) {
     Seg r;
-    r.s = b2p::prefix_find(pre, p.bt.n_seqs, x);
+    r.s = prefix_find(pre, p.bt.n_seqs, x);
     r.sq = p.bt.seq(r.s);
     r.nb = max(1, cdiv(r.sq.len, kBlk));
     const int off = x - pre[r.s], item = off / r.nb;
@@ -111,11 +91,87 @@ __device__ __forceinline__ Seg find_seg(const AttnParams& p, const int* pre, int
     r.b1 = min(r.nb, r.b0 + (x1 - x));
     r.x0 = x - r.b0;
     r.g = item % p.nkv;
-    r.i0 = item / p.nkv * p.T;
-    r.rows_t = min(p.T, min(r.sq.Q, p.max_q) - r.i0);
+    r.i0 = item / p.nkv * T;
+    r.rows_t = min(T, min(r.sq.Q, p.max_q) - r.i0);
     const int end = min(r.sq.len, max(0, r.sq.base + r.i0 + r.rows_t));
     r.live = min(r.b1, cdiv(end, kBlk));
     return r;
+}
+
+// ─── the long kernel's pieces ───
+//
+// Tile pairs that it left in pieces, by the four computing warps, one row per
+// thread.  A task is CC chunks of four dims of one tile; the tasks of all pairs
+// go round the CTAs.
+template <int HD, int CC>
+__device__ __forceinline__ void merge_task(const AttnParams& p, int owner, const Cut& cut, int t, int c0) {
+    const int r = threadIdx.x, T = kLongRows / p.G, tok = r / p.G;
+    if (tok >= min(T, cut.tokens - t * T)) return;
+    auto piece = [&](int i) { return p.long_part + (size_t)(2 * (owner + i) + (i == 0)) * long_piece_floats(HD); };
+    const int ml = 2 * kLongRows * HD + 2 * (t * kLongRows + r);
+    float M = -INFINITY;
+    for (int i = 0; i < cut.pieces; i++) M = fmaxf(M, __ldcg(piece(i) + ml));
+    float l = 0.f;
+    float4 acc[CC];
+#pragma unroll
+    for (int c = 0; c < CC; c++) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll(CC == 1 ? 8 : 2)
+    for (int i = 0; i < cut.pieces; i++) {
+        const float* q = piece(i);
+        const float2 v = __ldcg(reinterpret_cast<const float2*>(q + ml));
+        const float w = piece_weight(v.x, M);
+        l = fmaf(v.y, w, l);
+#pragma unroll
+        for (int c = 0; c < CC; c++) {
+            const float4 o = __ldcg(reinterpret_cast<const float4*>(q + ((size_t)(t * (HD / 4) + c0 + c) * kLongRows + r) * 4));
+            acc[c].x = fmaf(o.x, w, acc[c].x);
+            acc[c].y = fmaf(o.y, w, acc[c].y);
+            acc[c].z = fmaf(o.z, w, acc[c].z);
+            acc[c].w = fmaf(o.w, w, acc[c].w);
+        }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const size_t row = (size_t)(cut.row0 + t * T + tok);
+    const int h = cut.g * p.G + r % p.G;
+    __half* dst = p.out16 + (row * p.nq + h) * HD + 4 * c0;
+#pragma unroll
+    for (int c = 0; c < CC; c++) {
+        uint2 u;
+        u.x = pack_h2(acc[c].x * inv, acc[c].y * inv);
+        u.y = pack_h2(acc[c].z * inv, acc[c].w * inv);
+        *reinterpret_cast<uint2*>(dst + 4 * c) = u;
+    }
+    if (c0 == 0 && p.lse) p.lse[row * p.nq + h] = l == 0.f ? -INFINITY : M * kLn2 + logf(l);
+}
+
+template <int HD>
+__device__ __forceinline__ void merge_long(const AttnParams& p, int* scratch) {
+    constexpr int kBatch = 256;  // cuts read at a time
+    static_assert(kBatch * 4 <= B2_PAGED_MAX_SEQS, "scratch");
+    constexpr int kFew = 16;  // pieces up to which a task takes 8 chunks; more pieces, more tasks
+    Cut* cuts = reinterpret_cast<Cut*>(scratch);
+    int next = 0;  // tasks before
+    for (int base = 0; base < p.long_ctas; base += kBatch) {
+        const int n = min(kBatch, p.long_ctas - base);
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int i = threadIdx.x; i < n; i += 128) {
+            const int4 v = __ldcg(reinterpret_cast<const int4*>(p.cuts + base + i));
+            cuts[i] = Cut{v.x, v.y, v.z, v.w};
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int i = 0; i < n; i++) {
+            const Cut cut = cuts[i];
+            if (cut.pieces == 0) continue;
+            const bool few = cut.pieces <= kFew;
+            const int per_tile = few ? HD / 32 : HD / 4, tasks = per_tile * (cut.tokens * p.G > kLongRows / p.G * p.G ? 2 : 1);
+            const int grid = gridDim.x;
+            for (int k = ((int)blockIdx.x - next % grid + grid) % grid; k < tasks; k += grid) {
+                if (few) merge_task<HD, 8>(p, base + i, cut, k / per_tile, k % per_tile * 8);
+                else merge_task<HD, 1>(p, base + i, cut, k / per_tile, k % per_tile);
+            }
+            next += tasks;
+        }
+    }
 }
 
 template <int HD, int NT>
@@ -129,24 +185,27 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kStages; i++) {
-            b2p::mbar_init(&sm.full[i], 1);
-            b2p::mbar_init(&sm.empty[i], 4);
+            mbar_init(&sm.full[i], 1);
+            mbar_init(&sm.empty[i], 4);
         }
         sm.failed = 0;
-        b2p::mbar_init_fence();
+        mbar_init_fence();
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
     }
     b2::pdl_trigger();
-    b2::pdl_wait();
-    b2p::prefix_work(sm.pre, p.bt.n_seqs, [&](int s) {
-        const b2p::Seq q = p.bt.seq(s);
-        return cdiv(min(q.Q, p.max_q), p.T) * p.nkv * max(1, cdiv(q.len, kBlk));
+    // Behind the long kernel this grid starts once that one's CTAs have seen the
+    // kernels before them complete; it works beside them and waits for them below.
+    if (!p.long_ctas) b2::pdl_wait();
+    const int T = R / p.G;
+    prefix_work(sm.pre, p.bt.n_seqs, [&](int s) {
+        const Seq q = p.bt.seq(s);
+        const int n = min(q.Q, p.max_q);
+        return n * p.G > p.short_rows ? 0 : cdiv(n, T) * p.nkv * max(1, cdiv(q.len, kBlk));
     });
     const int W = sm.pre[p.bt.n_seqs];
     const int per = max(kMinBlocks, cdiv(W, gridDim.x));
-    const int x0 = min((long long)W, (long long)blockIdx.x * per), x1 = min(W, x0 + per);
-    if (x0 >= x1) return;
+    const int x0 = (int)min((long long)W, (long long)blockIdx.x * per), x1 = min(W, x0 + per);
     const int page_rows = 1 << p.bt.page_shift, box_rows = min(page_rows, kBlk);
 
     if (warp == 4) {  // producer: lane i copies the i-th box of a stage
@@ -154,11 +213,11 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
         int k = 0;
         bool ok = true;
         for (int x = x0; x < x1 && ok;) {
-            const Seg g = find_seg(p, sm.pre, x, x1);
+            const Seg g = find_seg(p, T, sm.pre, x, x1);
             for (int b = g.b0; b < g.live; b++, k++) {
                 const int st = k % C::kStages, j = b * kBlk + lane * box_rows;
                 const int page = lane < boxes && j < g.sq.len ? p.bt.page(g.s, j) : -1;
-                if (k >= C::kStages && !b2p::mbar_wait(&sm.empty[st], (k / C::kStages - 1) & 1, &sm.failed)) ok = false;
+                if (k >= C::kStages && !mbar_wait(&sm.empty[st], (k / C::kStages - 1) & 1, &sm.failed)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
@@ -166,14 +225,14 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                     int bits = 0;
                     for (int w = 0; w < 4; w++) bits |= (have >> (w * 16 / box_rows) & 1) << w;
                     sm.mapped[st] = bits;
-                    b2p::mbar_expect_tx(&sm.full[st], __popc(have) * 2 * box_bytes);
+                    mbar_expect_tx(&sm.full[st], __popc(have) * 2 * box_bytes);
                 }
                 __syncwarp();
                 if (page >= 0) {
                     unsigned char* dst = sm.ring + st * C::kStage + lane * box_bytes;
                     const int row = j & (page_rows - 1);
-                    b2p::tma_load_5d(dst, &tk, 0, row, 0, g.g, page, &sm.full[st]);
-                    b2p::tma_load_5d(dst + C::kStage / 2, &tv, 0, row, 0, g.g, page, &sm.full[st]);
+                    tma_load_5d(dst, &tk, 0, row, 0, g.g, page, &sm.full[st]);
+                    tma_load_5d(dst + C::kStage / 2, &tv, 0, row, 0, g.g, page, &sm.full[st]);
                 }
             }
             x += g.b1 - g.b0;
@@ -181,8 +240,8 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
         // a failed wait: let the copies in flight land (again bounded) before the CTA ends
         if (!ok && lane == 0)
             for (int i = max(0, k - C::kStages); i < k; i++)
-                for (long long it = 0; it <= b2p::kWaitLimit; it++)
-                    if (b2p::mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
+                for (long long it = 0; it <= kWaitLimit; it++)
+                    if (mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
         return;
     }
 
@@ -192,7 +251,7 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
     int k = 0;
     bool ok = true;
     for (int x = x0; x < x1 && ok;) {
-        const Seg sg = find_seg(p, sm.pre, x, x1);
+        const Seg sg = find_seg(p, T, sm.pre, x, x1);
         x += sg.b1 - sg.b0;
         const int rows = sg.rows_t * p.G;  // rows of the tile: token i0 + r / G, q head g G + r % G
         uint32_t qb[HD / 16][NT][2];
@@ -223,7 +282,7 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
         }
         for (int b = sg.b0; b < sg.live; b++, k++) {
             const int st = k % C::kStages;
-            ok = b2p::mbar_wait(&sm.full[st], (k / C::kStages) & 1, &sm.failed);
+            ok = mbar_wait(&sm.full[st], (k / C::kStages) & 1, &sm.failed);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             unsigned char* stage = sm.ring + st * C::kStage;
@@ -255,7 +314,7 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                     uint32_t a[4];
                     ldsm_x4(ka + (d >> 6) * half + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4), a);
 #pragma unroll
-                    for (int t = 0; t < NT; t++) b2p::mma16816(sc[t], a, qb[i][t][0], qb[i][t][1]);
+                    for (int t = 0; t < NT; t++) mma16816(sc[t], a, qb[i][t][0], qb[i][t][1]);
                 }
                 const int ja = j0 + (lane >> 2), jb = ja + 8;
                 uint32_t pb[NT][2];
@@ -289,8 +348,8 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                         o[i][t][2] *= corr[0];
                         o[i][t][3] *= corr[1];
                     }
-                    pb[t][0] = movm_t(b2p::pack_h2(pr[0], pr[1]));
-                    pb[t][1] = movm_t(b2p::pack_h2(pr[2], pr[3]));
+                    pb[t][0] = movm_t(pack_h2(pr[0], pr[1]));
+                    pb[t][1] = movm_t(pack_h2(pr[2], pr[3]));
                 }
 #pragma unroll
                 for (int i = 0; i < HD / 16; i++) {
@@ -299,11 +358,11 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                     uint32_t a[4];
                     ldsm_x4_t(va + (d >> 6) * half + r * 128 + ((((d & 63) >> 3) ^ (r & 7)) << 4), a);
 #pragma unroll
-                    for (int t = 0; t < NT; t++) b2p::mma16816(o[i][t], a, pb[t][0], pb[t][1]);
+                    for (int t = 0; t < NT; t++) mma16816(o[i][t], a, pb[t][0], pb[t][1]);
                 }
             }
             __syncwarp();
-            if (lane == 0) b2p::mbar_arrive(&sm.empty[st]);
+            if (lane == 0) mbar_arrive(&sm.empty[st]);
         }
         // merge the four warps' states, warp by warp
         if (lane < 4) {
@@ -372,10 +431,10 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                 const size_t row = (size_t)(sg.sq.row0 + sg.i0 + r / p.G);
                 const int h = sg.g * p.G + r % p.G;
                 uint4 w;
-                w.x = b2p::pack_h2(u.x * inv, u.y * inv);
-                w.y = b2p::pack_h2(u.z * inv, u.w * inv);
-                w.z = b2p::pack_h2(v.x * inv, v.y * inv);
-                w.w = b2p::pack_h2(v.z * inv, v.w * inv);
+                w.x = pack_h2(u.x * inv, u.y * inv);
+                w.y = pack_h2(u.z * inv, u.w * inv);
+                w.z = pack_h2(v.x * inv, v.y * inv);
+                w.w = pack_h2(v.z * inv, v.w * inv);
                 *reinterpret_cast<uint4*>(p.out16 + (row * p.nq + h) * HD + c) = w;
                 if (c == 0 && p.lse) p.lse[row * p.nq + h] = l == 0.f ? -INFINITY : (M - kUp) * kLn2 + logf(l);
             } else {
@@ -428,12 +487,17 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
         asm volatile("bar.sync 1, 128;" ::: "memory");  // the merge area is free for the next tile
     }
     if (!ok && lane == 0) atomicExch(p.err, 1);
+    if (p.long_ctas) {
+        b2::pdl_wait();
+        merge_long<HD>(p, sm.pre);
+    }
 }
 
 constexpr int kMaxGroup = 16;
-constexpr size_t kCounterBytes = 4096;
+constexpr int kShortRows = 16;  // (token, head) rows of a kv head that the short kernel takes, at most
+constexpr size_t kCounterBytes = 4096, kCutBytes = 4096;
 
-// CTAs of a launch: every SM's resident ones.
+// CTAs of a launch: one or two per SM.
 template <int HD, int NT>
 int short_grid(int dev, int sms) {
     static std::atomic<int> per[64];
@@ -443,20 +507,25 @@ int short_grid(int dev, int sms) {
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_short_kernel<HD, NT>, kThreads,
                                                           sizeof(ShortSmem<HD, NT>) + 1024) != cudaSuccess || n < 1)
             n = 1;
+        n = n < 2 ? n : 2;
         c.store(n, std::memory_order_relaxed);
     }
-    return (n < 2 ? n : 2) * sms;
+    return n * sms;
 }
 
 template <int HD, int NT>
-int launch_short(AttnParams p, const CUtensorMap& tk, const CUtensorMap& tv, int dev, int sms, long long blocks,
-                 cudaStream_t s) {
+int launch_short(const AttnParams& p, const B2PagedKV* kv, int dev, int sms, long long blocks, cudaStream_t s) {
     static std::atomic<unsigned long long> done{0};
     constexpr size_t smem = sizeof(ShortSmem<HD, NT>) + 1024;
-    cudaError_t e = b2p::allow_smem(attn_short_kernel<HD, NT>, smem, done, dev);
+    cudaError_t e = allow_smem(attn_short_kernel<HD, NT>, smem, done, dev);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged smem: %s", cudaGetErrorString(e));
+    CUtensorMap tk, tv;
+    const int box = kv->page_size < kBlk ? kv->page_size : kBlk;
+    int rc = b2_paged_map(&tk, kv->k_pages, kv, p.nkv, HD, box, HD / 64);
+    if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, p.nkv, HD, box, HD / 64);
+    if (rc) return rc;
     long long grid = short_grid<HD, NT>(dev, sms);
-    if (grid > (blocks + kMinBlocks - 1) / kMinBlocks) grid = (blocks + kMinBlocks - 1) / kMinBlocks;
+    if (!p.long_ctas && grid > (blocks + kMinBlocks - 1) / kMinBlocks) grid = (blocks + kMinBlocks - 1) / kMinBlocks;
     e = b2::launch_pdl(attn_short_kernel<HD, NT>, dim3((unsigned)grid), dim3(kThreads), smem, s, tk, tv, p);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged: %s", cudaGetErrorString(e));
     return 0;
@@ -470,13 +539,18 @@ int device_sms(int* dev) {
     return sms;
 }
 
+// Workspace: counters, cuts, the short kernel's pieces (two of up to 16 rows for
+// each of at most two CTAs per SM), the long kernel's (two per SM).
+size_t short_part_bytes(int sms, int hd) { return (size_t)sms * 2 * 2 * kShortRows * (hd + 2) * sizeof(float); }
+
 }  // namespace
 
 extern "C" size_t b2_attention_paged_workspace(int n_seqs, int max_q, int nq, int nkv, int hd) {
     int dev;
     const int sms = device_sms(&dev);
-    // two partial tiles of up to 32 rows for each of at most two CTAs per SM
-    return kCounterBytes + (size_t)sms * 2 * 2 * 32 * (hd + 2) * sizeof(float);
+    const bool any_long = n_seqs > 0 && nkv > 0 && (long long)max_q * nq > (long long)kShortRows * nkv;
+    return kCounterBytes + kCutBytes + short_part_bytes(sms, hd) +
+           (any_long ? (size_t)sms * 2 * long_piece_floats(hd) * sizeof(float) : 0);
 }
 
 extern "C" int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq, int M, int max_q, int nq,
@@ -495,27 +569,24 @@ extern "C" int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q
     if (max_q > M) max_q = M;
     int dev;
     const int sms = device_sms(&dev);
-    CUtensorMap tk, tv;
-    const int box = kv->page_size < kBlk ? kv->page_size : kBlk;
-    rc = b2_paged_map(&tk, kv->k_pages, kv, nkv, hd, box);
-    if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, nkv, hd, box);
-    if (rc) return rc;
-    const int G = nq / nkv, rows = max_q * G, NT = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
-    AttnParams p{b2p::make_batch(kv, M), reinterpret_cast<const __half*>(q16), ldq, reinterpret_cast<__half*>(out16), lse,
-                 max_q, nq, nkv, G, 8 * NT / G,
-                 reinterpret_cast<float*>(reinterpret_cast<unsigned char*>(work) + kCounterBytes),
-                 reinterpret_cast<int*>(work), err};
+    const int G = nq / nkv;
+    const long long rows = (long long)max_q * G;
+    unsigned char* w = reinterpret_cast<unsigned char*>(work);
+    AttnParams p{make_batch(kv, M), reinterpret_cast<const __half*>(q16), ldq, reinterpret_cast<__half*>(out16), lse, max_q,
+                 nq, nkv, G, kShortRows, reinterpret_cast<int*>(w),
+                 reinterpret_cast<float*>(w + kCounterBytes + kCutBytes), reinterpret_cast<Cut*>(w + kCounterBytes),
+                 reinterpret_cast<float*>(w + kCounterBytes + kCutBytes + short_part_bytes(sms, hd)), 0, err};
     // the line's length when every sequence fills its table: what the kernel's 32-bit places must hold
     const long long cap = ((long long)kv->max_pages * kv->page_size + kBlk - 1) / kBlk;
-    const long long tiles = (M + p.T - 1) / p.T + kv->n_seqs;
-    const long long blocks = tiles * nkv * cap;
+    const long long tiles = (long long)kv->n_seqs * kShortRows;
+    const long long blocks = (tiles < M + 0ll ? tiles : (long long)M) * nkv * cap;
     if (blocks >= (1ll << 31) - 65536)
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_attention_paged: %lld blocks of work in one call", blocks);
     cudaStream_t st = (cudaStream_t)s;
-#define B2_SHORT(HD)                                                                     \
-    (NT == 1   ? launch_short<HD, 1>(p, tk, tv, dev, sms, blocks, st)                    \
-     : NT == 2 ? launch_short<HD, 2>(p, tk, tv, dev, sms, blocks, st)                    \
-               : launch_short<HD, 4>(p, tk, tv, dev, sms, blocks, st))
-    return hd == 128 ? B2_SHORT(128) : B2_SHORT(64);
-#undef B2_SHORT
+    if (rows > kShortRows) {
+        rc = b2_paged_attention_long(p, kv, hd, dev, sms, st);
+        if (rc) return rc;
+    }
+    if (rows <= 8) return hd == 128 ? launch_short<128, 1>(p, kv, dev, sms, blocks, st) : launch_short<64, 1>(p, kv, dev, sms, blocks, st);
+    return hd == 128 ? launch_short<128, 2>(p, kv, dev, sms, blocks, st) : launch_short<64, 2>(p, kv, dev, sms, blocks, st);
 }

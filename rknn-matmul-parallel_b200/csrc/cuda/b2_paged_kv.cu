@@ -22,11 +22,12 @@ int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool r
     return 0;
 }
 
-int b2_paged_map(CUtensorMap* map, const uint16_t* base, const B2PagedKV* kv, int nkv, int hd, int box_rows) {
+int b2_paged_map(CUtensorMap* map, const uint16_t* base, const B2PagedKV* kv, int nkv, int hd, int box_rows,
+                 int box_halves) {
     const uint64_t dims[5] = {64, (uint64_t)kv->page_size, (uint64_t)hd / 64, (uint64_t)nkv, (uint64_t)kv->n_pages};
     const uint64_t strides[4] = {(uint64_t)kv->row_stride * 2, 128, (uint64_t)kv->head_stride * 2,
                                  (uint64_t)kv->page_stride * 2};
-    const uint32_t box[5] = {64, (uint32_t)box_rows, (uint32_t)hd / 64, 1, 1};
+    const uint32_t box[5] = {64, (uint32_t)box_rows, (uint32_t)box_halves, 1, 1};
     return b2_tensor_map_f16_5d(map, base, dims, strides, box);
 }
 
