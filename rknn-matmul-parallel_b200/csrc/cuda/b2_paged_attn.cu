@@ -238,6 +238,7 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
             x += g.b1 - g.b0;
         }
         // a failed wait: let the copies in flight land (again bounded) before the CTA ends
+        if (!ok && lane == 0) atomicExch(p.err, 1);
         if (!ok && lane == 0)
             for (int i = max(0, k - C::kStages); i < k; i++)
                 for (long long it = 0; it <= kWaitLimit; it++)

@@ -294,8 +294,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             // ── tensor cores ──
             if (lane == 0) {
                 constexpr uint32_t id_s = idesc_f16(128, 128, false), id_o = idesc_f16(128, HD, true);
-                int k = 0, seg = 0, all_segs = 0;
+                int k = 0, seg = 0;
                 int np[2] = {0, 0};  // P tiles consumed
+                int no[2] = {0, 0};  // segments whose O the tile has summed
                 auto mma_s = [&](int t, int st) {
                     const uint32_t a = smem_u32(sm.q[t]), b = smem_u32(sm.ring[st]);
 #pragma unroll
@@ -308,20 +309,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 for (int x = x0; x < x1 && ok;) {
                     const Seg g = find_seg<HD>(p, sm, items, x, x1);
                     x += g.b1 - g.b0;
-                    // The softmax frees O_t once per segment: waited for before the
-                    // segment's first product into it, and never skipped.
-                    const int before = all_segs++;
-                    bool held[2] = {before > 0, before > 0};
-                    auto take_o = [&](int t) {
-                        if (!held[t]) return true;
-                        held[t] = false;
-                        return mbar_wait(&sm.o_free[t], (before - 1) & 1, failed);
-                    };
                     const int e = g.end();
-                    if (e <= g.b0) {
-                        ok = take_o(0) && take_o(1);
-                        continue;
-                    }
+                    if (e <= g.b0) continue;
                     ok = mbar_wait(&sm.q_full, seg & 1, failed);
                     seg++;
                     if (!ok) break;
@@ -338,7 +327,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         ok = mbar_wait(&sm.full[sv], ((k + 1) / C::kStages) & 1, failed);
                         for (int t = 0; t < 2 && ok; t++) {
                             if (b < g.live[t]) {
-                                ok = take_o(t) && mbar_wait(&sm.p_ready[t], np[t] & 1, failed);
+                                // the segment before's O has been read
+                                if (b == g.b0 && no[t]++) ok = mbar_wait(&sm.o_free[t], no[t] & 1, failed);
+                                ok = ok && mbar_wait(&sm.p_ready[t], np[t] & 1, failed);
                                 np[t]++;
                                 if (!ok) break;
                                 tc_fence_after();
@@ -360,7 +351,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                         if (b + 1 < e) umma_commit(&sm.empty[sk]);
                         if (b + 2 == e) umma_commit(&sm.q_empty);
                     }
-                    ok = ok && take_o(0) && take_o(1);
                 }
                 if (!ok) {  // nothing of the tensor cores may be left running
                     umma_commit(&sm.drain);
@@ -509,7 +499,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     p.a.lse[row * p.a.nq + h] = l == 0.f ? -INFINITY : (m - kUp) * kLn2 + logf(l);
             }
             tc_fence_before();
-            mbar_arrive(&sm.o_free[t]);
+            if (any) mbar_arrive(&sm.o_free[t]);
             if (!whole && g.b0 == 0) {
                 owns = true;
                 if (threadIdx.x == 0)
@@ -518,8 +508,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         if (threadIdx.x == 0 && !owns) p.a.cuts[blockIdx.x] = Cut{0, 0, 0, 0};
-        if (!ok && lane == 0) atomicExch(p.a.err, 1);
     }
+    if (!ok && lane == 0) atomicExch(p.a.err, 1);
     tc_fence_before();
     __syncthreads();
     if (warp == 9) {
