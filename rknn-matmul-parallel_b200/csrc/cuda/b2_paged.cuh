@@ -108,6 +108,26 @@ __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, i
         : "memory");
 }
 
+// Untiled copy: addresses and size multiples of 16 bytes.
+__device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t bytes, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
+        "l"(src), "r"(bytes), "r"(smem_u32(bar))
+        : "memory");
+}
+
+// Loads past L1 of what other CTAs wrote.
+__device__ __forceinline__ float2 ld_cg2(const float* p) {
+    float2 v;
+    asm volatile("ld.global.cg.v2.f32 {%0,%1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ld_cg4(const float* p) {
+    float4 v;
+    asm volatile("ld.global.cg.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "l"(p) : "memory");
+    return v;
+}
+
 // 2^x (ex2.approx: 2 ulp; subnormal results flush to zero).
 __device__ __forceinline__ float ex2(float x) {
     float y;

@@ -39,48 +39,74 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
 // blocks of 64 slots: sequences, then tiles and kv heads, then the tile's
 // blocks.  Every CTA takes an equal stretch of that line, so sequences of any
 // mix of lengths load the SMs evenly; a tile that a stretch boundary cuts is
-// summed in pieces, which its last arriver merges in the line's order.
+// summed in pieces, which the last CTA to arrive merges in the line's order.
+// A boundary near a tile's end moves there (snap_of): a piece costs about as
+// much as six blocks.
 //
-// A producer warp keeps a ring of stages (64 slots of K and V) filled by TMA,
-// through the page table, across tile boundaries.  Four warps compute, each on
-// 16 slots of a stage:
+// A producer warp walks the stretch: for each tile it copies the Q rows, then
+// the K and V blocks through the page table into a ring of stages, across tile
+// boundaries.  Four warps compute, each on 16 slots of a stage:
 //   S^T = K Q^T    mma m16n8k16: slots are the M rows, the tile's rows the N
 //                  columns;
 //   O^T += V^T P^T the head dims are M, the slots K; P^T moves from the
 //                  accumulator to the B-operand layout with movmatrix.
 constexpr int kBlk = 64;
 constexpr int kThreads = 160;  // four computing warps, one producer
-constexpr int kMinBlocks = 4;  // shortest stretch of a CTA
+constexpr int kMinBlocks = 2;  // shortest stretch of a CTA
+constexpr int kFan = 16;       // pieces that one CTA merges; more are merged in two levels
+
+// A stretch's part of one tile: blocks [b0, b1) of the tile's nb.
+struct Seg {
+    int g, i0, rows_t;  // kv head, first token, tokens
+    int b0, b1, live;   // live: end of the blocks that some row of the tile sees
+    int nb, x0;         // the tile's blocks, and where it starts on the line
+    int s;
+    Seq sq;
+};
 
 template <int HD, int NT>
 struct Short {
     static constexpr int R = 8 * NT;
     static constexpr int kStage = kBlk * HD * 4;  // K and V, bytes
     static constexpr int kStages = HD == 128 ? 3 : 6;
-    static constexpr int kLd = HD + 4;            // row of the merge buffer: the four lane columns hit distinct banks
-    static constexpr int kTile = R * (HD + 2);    // floats of one partial tile: o[R][HD], then (m, l)[R]
+    static constexpr int kQ = NT == 1 || HD == 64 ? 2 : 1;  // Q tiles ahead: what two CTAs per SM leave room for
+    static constexpr int kLdQ = HD + 8;           // row of a Q tile (halves): eight rows hit distinct banks
+    // Row of the merge buffer: + 4 lets the four lane columns hit distinct banks,
+    // where two CTAs per SM leave room for it.
+    static constexpr int kLd = HD + (NT == 1 || HD == 64 ? 4 : 0);
+    // Floats of one partial tile: o[R][HD], (m, l)[R], (m, l)[R] of a first merge.
+    static constexpr int kTile = R * (HD + 4);
+    static constexpr int kFrag = HD / 16 * 32 * 4;  // floats of one warp's O for one column group
+    static constexpr int kMerge = 2 * kFrag > R * kLd ? 2 * kFrag : R * kLd;
 };
 
 template <int HD, int NT>
 struct ShortSmem {
     alignas(1024) unsigned char ring[Short<HD, NT>::kStages * Short<HD, NT>::kStage];
-    float o[Short<HD, NT>::R * Short<HD, NT>::kLd];
+    float o[Short<HD, NT>::kMerge];
+    alignas(16) __half q[Short<HD, NT>::kQ][Short<HD, NT>::R * Short<HD, NT>::kLdQ];
     float m[4][Short<HD, NT>::R], l[4][Short<HD, NT>::R];
     uint64_t full[Short<HD, NT>::kStages], empty[Short<HD, NT>::kStages];
+    uint64_t q_full[Short<HD, NT>::kQ], q_empty[Short<HD, NT>::kQ];
+    Seg seg[Short<HD, NT>::kQ];
     int mapped[Short<HD, NT>::kStages];  // bit w: the 16 slots of warp w are mapped
     int failed, last;
     int pre[B2_PAGED_MAX_SEQS + 1];
 };
 
-// A stretch's part of one tile: blocks [b0, b1) of the tile's nb.
-struct Seg {
-    int s, g, i0, rows_t;  // sequence, kv head, first token, tokens
-    int b0, b1, live;      // live: end of the blocks that some row of the tile sees
-    int nb, x0;            // the tile's blocks, and where it starts on the line
-    Seq sq;
-};
+// Blocks within which a boundary moves to a tile's end: short stretches rather
+// take a tile of up to 16 blocks whole than split it.
+__device__ __forceinline__ int snap_of(int per) { return per <= 8 ? 8 : max(3, per / 8); }
 
-// T: tokens of one tile.
+// Where the stretch of CTA c begins.  T: tokens of one tile.
+__device__ __forceinline__ int stretch_start(const AttnParams& p, const int* pre, int W, int per, int c) {
+    const long long at = (long long)c * per;
+    if (at >= W) return W;
+    const int x = (int)at, s = prefix_find(pre, p.bt.n_seqs, x);
+    const int nb = max(1, cdiv(p.bt.seq(s).len, kBlk)), b = (x - pre[s]) % nb, snap = snap_of(per);
+    return b <= snap && b <= nb - b ? x - b : nb - b <= snap ? x - b + nb : x;
+}
+
 __device__ __forceinline__ Seg find_seg(const AttnParams& p, int T, const int* pre, int x, int x1) {
     Seg r;
     r.s = prefix_find(pre, p.bt.n_seqs, x);
@@ -96,6 +122,71 @@ __device__ __forceinline__ Seg find_seg(const AttnParams& p, int T, const int* p
     const int end = min(r.sq.len, max(0, r.sq.base + r.i0 + r.rows_t));
     r.live = min(r.b1, cdiv(end, kBlk));
     return r;
+}
+
+// The rows of a tile from pieces of CTAs first, first + step, ... (n of them, own
+// the one that begins the tile): to the outputs, or to the slot of `first`.
+template <int HD, int NT>
+__device__ __forceinline__ void merge_pieces(const AttnParams& p, const Seg& sg, int own, int first, int step, int n,
+                                             bool final) {
+    using C = Short<HD, NT>;
+    constexpr int kWide = 16;
+    const int rows = sg.rows_t * p.G, ml0 = C::R * (HD + (step > 1 ? 2 : 0));
+    auto slot = [&](int i) {
+        const int c = first + i * step;
+        return p.part + (size_t)(2 * c + (c == own)) * C::kTile;
+    };
+    const int all = rows * (HD / 4);
+    for (int i0 = threadIdx.x; i0 < (all + 31) / 32 * 32; i0 += 128) {
+        const int i = min(i0, all - 1), r = i / (HD / 4), c = i % (HD / 4) * 4;
+        float M = -INFINITY, l = 0.f;
+        float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+        // kWide pieces in flight: the loads' latency is what a merge costs
+        for (int j0 = 0; j0 < n; j0 += kWide) {
+            float2 ml[kWide];
+            float4 o[kWide];
+#pragma unroll
+            for (int j = 0; j < kWide; j++) {
+                const float* q = slot(min(j0 + j, n - 1));
+                ml[j] = ld_cg2(q + ml0 + 2 * r);
+                o[j] = ld_cg4(q + r * HD + c);
+            }
+            // No load moves behind this: left alone the compiler puts each load in front of its use,
+            // and a merge of 16 pieces waits 16 times (8.5 instead of 2.9 us).
+            __syncwarp();
+            float top = M;
+#pragma unroll
+            for (int j = 0; j < kWide; j++) top = fmaxf(top, ml[j].x);
+            const float f = piece_weight(M, top);
+            M = top;
+            l *= f;
+            acc.x *= f, acc.y *= f, acc.z *= f, acc.w *= f;
+#pragma unroll
+            for (int j = 0; j < kWide; j++) {
+                if (j0 + j >= n) break;
+                const float w = piece_weight(ml[j].x, M);
+                l = fmaf(ml[j].y, w, l);
+                acc.x = fmaf(o[j].x, w, acc.x);
+                acc.y = fmaf(o[j].y, w, acc.y);
+                acc.z = fmaf(o[j].z, w, acc.z);
+                acc.w = fmaf(o[j].w, w, acc.w);
+            }
+        }
+        if (i0 >= all) continue;
+        if (final) {
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            const size_t row = (size_t)(sg.sq.row0 + sg.i0 + r / p.G);
+            const int h = sg.g * p.G + r % p.G;
+            uint2 u;
+            u.x = pack_h2(acc.x * inv, acc.y * inv);
+            u.y = pack_h2(acc.z * inv, acc.w * inv);
+            *reinterpret_cast<uint2*>(p.out16 + (row * p.nq + h) * HD + c) = u;
+            if (c == 0 && p.lse) p.lse[row * p.nq + h] = l == 0.f ? -INFINITY : (M - kUp) * kLn2 + logf(l);
+        } else {
+            *reinterpret_cast<float4*>(slot(0) + r * HD + c) = acc;
+            if (c == 0) *reinterpret_cast<float2*>(slot(0) + C::R * (HD + 2) + 2 * r) = make_float2(M, l);
+        }
+    }
 }
 
 // ─── the long kernel's pieces ───
@@ -175,18 +266,22 @@ __device__ __forceinline__ void merge_long(const AttnParams& p, int* scratch) {
 }
 
 template <int HD, int NT>
-__global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_constant__ CUtensorMap tk,
-                                                              const __grid_constant__ CUtensorMap tv, const AttnParams p) {
+__global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_constant__ CUtensorMap tk,
+                                                                 const __grid_constant__ CUtensorMap tv,
+                                                                 const AttnParams p) {
     using C = Short<HD, NT>;
     constexpr int R = C::R;
-    extern __shared__ unsigned char smem_raw[];
-    ShortSmem<HD, NT>& sm = *reinterpret_cast<ShortSmem<HD, NT>*>(
-        (reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    extern __shared__ __align__(1024) unsigned char smem_raw[];
+    ShortSmem<HD, NT>& sm = *reinterpret_cast<ShortSmem<HD, NT>*>(smem_raw);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kStages; i++) {
             mbar_init(&sm.full[i], 1);
             mbar_init(&sm.empty[i], 4);
+        }
+        for (int i = 0; i < C::kQ; i++) {
+            mbar_init(&sm.q_full[i], 1);
+            mbar_init(&sm.q_empty[i], 4);
         }
         sm.failed = 0;
         mbar_init_fence();
@@ -205,19 +300,46 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
     });
     const int W = sm.pre[p.bt.n_seqs];
     const int per = max(kMinBlocks, cdiv(W, gridDim.x));
-    const int x0 = (int)min((long long)W, (long long)blockIdx.x * per), x1 = min(W, x0 + per);
+    const int x0 = stretch_start(p, sm.pre, W, per, blockIdx.x), x1 = stretch_start(p, sm.pre, W, per, blockIdx.x + 1);
     const int page_rows = 1 << p.bt.page_shift, box_rows = min(page_rows, kBlk);
+    volatile int* failed = &sm.failed;
 
-    if (warp == 4) {  // producer: lane i copies the i-th box of a stage
+    if (warp == 4) {  // producer: lane i copies the i-th box of a stage and the i-th row of a Q tile
         const int boxes = kBlk / box_rows, box_bytes = box_rows * HD * 2;
-        int k = 0;
+        int k = 0, n = 0;
         bool ok = true;
-        for (int x = x0; x < x1 && ok;) {
+        for (int x = x0; x < x1 && ok; n++) {
             const Seg g = find_seg(p, T, sm.pre, x, x1);
+            x += g.b1 - g.b0;
+            const int qb = n % C::kQ, rows = g.rows_t * p.G;
+            // page ids of the next 32 boxes, one per lane
+            int ids_from = g.b0, id = -1;
+            auto load_ids = [&]() {
+                const int j = ids_from * kBlk + lane * box_rows;
+                id = j < g.sq.len && ids_from + lane / boxes < g.live ? p.bt.page(g.s, j) : -1;
+            };
+            load_ids();
+            if (n >= C::kQ && !mbar_wait(&sm.q_empty[qb], (n / C::kQ - 1) & 1, failed)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            if (lane == 0) {
+                sm.seg[qb] = g;
+                mbar_expect_tx(&sm.q_full[qb], rows * HD * 2);
+            }
+            __syncwarp();
+            if (lane < rows)
+                bulk_copy(sm.q[qb] + lane * C::kLdQ,
+                          p.q16 + (size_t)(g.sq.row0 + g.i0 + lane / p.G) * p.ldq + (size_t)(g.g * p.G + lane % p.G) * HD,
+                          HD * 2, &sm.q_full[qb]);
             for (int b = g.b0; b < g.live; b++, k++) {
                 const int st = k % C::kStages, j = b * kBlk + lane * box_rows;
-                const int page = lane < boxes && j < g.sq.len ? p.bt.page(g.s, j) : -1;
-                if (k >= C::kStages && !mbar_wait(&sm.empty[st], (k / C::kStages - 1) & 1, &sm.failed)) ok = false;
+                if ((b - ids_from + 1) * boxes > 32) {
+                    ids_from = b;
+                    load_ids();
+                }
+                const int mine = __shfl_sync(0xffffffffu, id, ((b - ids_from) * boxes + lane) & 31);
+                const int page = lane < boxes ? mine : -1;
+                if (k >= C::kStages && !mbar_wait(&sm.empty[st], (k / C::kStages - 1) & 1, failed)) ok = false;
                 ok = __all_sync(0xffffffffu, ok);
                 if (!ok) break;
                 const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
@@ -235,37 +357,43 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                     tma_load_5d(dst + C::kStage / 2, &tv, 0, row, 0, g.g, page, &sm.full[st]);
                 }
             }
-            x += g.b1 - g.b0;
         }
-        // a failed wait: let the copies in flight land (again bounded) before the CTA ends
-        if (!ok && lane == 0) atomicExch(p.err, 1);
-        if (!ok && lane == 0)
+        if (!ok && lane == 0) {
+            atomicExch(p.err, 1);
+            // let the copies in flight land (again bounded) before the CTA ends
             for (int i = max(0, k - C::kStages); i < k; i++)
                 for (long long it = 0; it <= kWaitLimit; it++)
                     if (mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
+            for (int i = max(0, n + 1 - C::kQ); i <= n; i++)
+                for (long long it = 0; it <= kWaitLimit; it++)
+                    if (mbar_try_wait(&sm.q_full[i % C::kQ], (i / C::kQ) & 1)) break;
+        }
         return;
     }
 
-    const float scale = 1.4426950408889634f / sqrtf((float)HD);  // to log2 units
+    const float scale = kLog2e / sqrtf((float)HD);  // to log2 units
     const int pw = warp * 16;
     const int bshift = box_rows == 16 ? 4 : box_rows == 32 ? 5 : 6;
-    int k = 0;
+    const int tid = threadIdx.x;
+    auto sync4 = [] { asm volatile("bar.sync 1, 128;" ::: "memory"); };
+    int k = 0, n = 0;
     bool ok = true;
-    for (int x = x0; x < x1 && ok;) {
-        const Seg sg = find_seg(p, T, sm.pre, x, x1);
+    for (int x = x0; x < x1; n++) {
+        const int qi = n % C::kQ;
+        ok = mbar_wait(&sm.q_full[qi], (n / C::kQ) & 1, failed);
+        ok = __all_sync(0xffffffffu, ok);
+        const Seg sg = sm.seg[qi];
         x += sg.b1 - sg.b0;
         const int rows = sg.rows_t * p.G;  // rows of the tile: token i0 + r / G, q head g G + r % G
         uint32_t qb[HD / 16][NT][2];
         int lim[NT][2];  // last slot that this lane's two columns see
 #pragma unroll
         for (int t = 0; t < NT; t++) {
-            const int r = 8 * t + (lane >> 2);
-            const __half* qp = p.q16 + (size_t)(sg.sq.row0 + sg.i0 + r / p.G) * p.ldq +
-                               (size_t)(sg.g * p.G + r % p.G) * HD + 2 * (lane & 3);
+            const __half* qp = sm.q[qi] + (8 * t + (lane >> 2)) * C::kLdQ + 2 * (lane & 3);
 #pragma unroll
             for (int i = 0; i < HD / 16; i++) {
-                qb[i][t][0] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * i) : 0u;
-                qb[i][t][1] = r < rows ? *reinterpret_cast<const uint32_t*>(qp + 16 * i + 8) : 0u;
+                qb[i][t][0] = *reinterpret_cast<const uint32_t*>(qp + 16 * i);
+                qb[i][t][1] = *reinterpret_cast<const uint32_t*>(qp + 16 * i + 8);
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
@@ -273,6 +401,8 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                 lim[t][j] = c < rows ? min(sg.sq.len - 1, sg.sq.base + sg.i0 + c / p.G) : -1;
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&sm.q_empty[qi]);
         float o[HD / 16][NT][4], mx[NT][2], ls[NT][2];
 #pragma unroll
         for (int t = 0; t < NT; t++) {
@@ -281,9 +411,9 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
             mx[t][0] = mx[t][1] = -INFINITY;
             ls[t][0] = ls[t][1] = 0.f;
         }
-        for (int b = sg.b0; b < sg.live; b++, k++) {
+        for (int b = sg.b0; b < sg.live && ok; b++, k++) {
             const int st = k % C::kStages;
-            ok = mbar_wait(&sm.full[st], (k / C::kStages) & 1, &sm.failed);
+            ok = mbar_wait(&sm.full[st], (k / C::kStages) & 1, failed);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             unsigned char* stage = sm.ring + st * C::kStage;
@@ -335,11 +465,7 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
                         corr[j] = mn == -INFINITY ? 1.f : ex2(mx[t][j] - mn);
                         pr[j] = ex2(sa - ref);
                         pr[j + 2] = ex2(sb - ref);
-                        float rs = pr[j] + pr[j + 2];
-                        rs += __shfl_xor_sync(0xffffffffu, rs, 4);
-                        rs += __shfl_xor_sync(0xffffffffu, rs, 8);
-                        rs += __shfl_xor_sync(0xffffffffu, rs, 16);
-                        ls[t][j] = ls[t][j] * corr[j] + rs;
+                        ls[t][j] = fmaf(ls[t][j], corr[j], pr[j] + pr[j + 2]);  // this lane's slots only
                         mx[t][j] = mn;
                     }
 #pragma unroll
@@ -365,66 +491,105 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
             __syncwarp();
             if (lane == 0) mbar_arrive(&sm.empty[st]);
         }
-        // merge the four warps' states, warp by warp
-        if (lane < 4) {
+        // Merge the four warps' states: 2 into 0 and 3 into 1, then 1 into 0.
 #pragma unroll
-            for (int t = 0; t < NT; t++) {
+        for (int t = 0; t < NT; t++) {
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                ls[t][j] += __shfl_xor_sync(0xffffffffu, ls[t][j], 4);
+                ls[t][j] += __shfl_xor_sync(0xffffffffu, ls[t][j], 8);
+                ls[t][j] += __shfl_xor_sync(0xffffffffu, ls[t][j], 16);
+            }
+        }
+        auto give = [&](int t, float* to) {
+            if (lane < 4) {
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     sm.m[warp][8 * t + 2 * lane + j] = mx[t][j];
                     sm.l[warp][8 * t + 2 * lane + j] = ls[t][j];
                 }
             }
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++)
+                *reinterpret_cast<float4*>(to + (i * 32 + lane) * 4) = make_float4(o[i][t][0], o[i][t][1], o[i][t][2], o[i][t][3]);
+        };
+        auto take = [&](int t, const float* from, int w) {
+            float fa[2], fb[2];
+#pragma unroll
+            for (int j = 0; j < 2; j++) {
+                const int c = 8 * t + 2 * (lane & 3) + j;
+                const float m2 = sm.m[w][c], l2 = sm.l[w][c], M = fmaxf(mx[t][j], m2);
+                fa[j] = piece_weight(mx[t][j], M);
+                fb[j] = piece_weight(m2, M);
+                ls[t][j] = ls[t][j] * fa[j] + l2 * fb[j];
+                mx[t][j] = M;
+            }
+#pragma unroll
+            for (int i = 0; i < HD / 16; i++) {
+                const float4 v = *reinterpret_cast<const float4*>(from + (i * 32 + lane) * 4);
+                o[i][t][0] = o[i][t][0] * fa[0] + v.x * fb[0];
+                o[i][t][1] = o[i][t][1] * fa[1] + v.y * fb[1];
+                o[i][t][2] = o[i][t][2] * fa[0] + v.z * fb[0];
+                o[i][t][3] = o[i][t][3] * fa[1] + v.w * fb[1];
+            }
+        };
+        int bad = 0;
+#pragma unroll
+        for (int t = 0; t < NT; t++) {
+            if (warp >= 2) give(t, sm.o + (warp - 2) * C::kFrag);
+            if (t == 0) {
+                // one decision for the four warps: a failed wait ends the stretch
+                asm volatile(
+                    "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.s32 "
+                    "%0, 1, 0, q;\n}\n"
+                    : "=r"(bad)
+                    : "r"(ok ? 0 : 1)
+                    : "memory");
+                if (bad) break;
+            } else {
+                sync4();
+            }
+            if (warp < 2) take(t, sm.o + warp * C::kFrag, warp + 2);
+            if (warp == 1) give(t, sm.o + C::kFrag);
+            sync4();
+            if (warp == 0) take(t, sm.o + C::kFrag, 1);
+            if (t + 1 < NT) sync4();
         }
-        // one decision for the four warps (a failed wait ends the stretch)
-        int bad;
-        asm volatile(
-            "{\n .reg .pred p, q;\n setp.ne.s32 p, %1, 0;\n barrier.cta.red.or.pred q, 1, 128, p;\n selp.s32 %0, 1, 0, "
-            "q;\n}\n"
-            : "=r"(bad)
-            : "r"(ok ? 0 : 1)
-            : "memory");
         if (bad) {
             ok = false;
             break;
         }
-        float f[NT][2];
+        // Warp 0 has the sum: through shared memory to rows.
+        if (warp == 0) {
+            __syncwarp();
 #pragma unroll
-        for (int t = 0; t < NT; t++) {
+            for (int t = 0; t < NT; t++) {
+                const int c = 8 * t + 2 * (lane & 3);
 #pragma unroll
-            for (int j = 0; j < 2; j++) {
-                const int c = 8 * t + 2 * (lane & 3) + j;
-                const float M = fmaxf(fmaxf(sm.m[0][c], sm.m[1][c]), fmaxf(sm.m[2][c], sm.m[3][c]));
-                f[t][j] = piece_weight(mx[t][j], M);
-            }
-        }
-        for (int w = 0; w < 4; w++) {
-            if (w == warp) {
+                for (int i = 0; i < HD / 16; i++) {
 #pragma unroll
-                for (int t = 0; t < NT; t++) {
+                    for (int e = 0; e < 4; e++)
+                        sm.o[(c + (e & 1)) * C::kLd + 16 * i + (lane >> 2) + (e >> 1) * 8] = o[i][t][e];
+                }
+                if (lane < 4) {
 #pragma unroll
-                    for (int i = 0; i < HD / 16; i++) {
-#pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            float* d = &sm.o[(8 * t + 2 * (lane & 3) + (e & 1)) * C::kLd + 16 * i + (lane >> 2) + (e >> 1) * 8];
-                            const float v = o[i][t][e] * f[t][e & 1];
-                            *d = w ? *d + v : v;
-                        }
+                    for (int j = 0; j < 2; j++) {
+                        sm.m[0][c + j] = mx[t][j];
+                        sm.l[0][c + j] = ls[t][j];
                     }
                 }
             }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
         }
-        const bool whole = sg.b0 == 0 && sg.b1 == sg.nb;
-        const int tid = threadIdx.x;
-        const int own = sg.x0 / per;  // the CTA whose stretch holds the tile's first block
+        sync4();
+        // A boundary strictly inside the tile, away from its ends, cuts it.
+        const int snap = snap_of(per);
+        const int c_lo = (sg.x0 + snap) / per + 1, c_hi = (sg.x0 + sg.nb - snap + per - 1) / per - 1;
+        const bool whole = c_lo > c_hi;
+        const int own = c_lo - 1, last = c_hi;  // CTAs of the pieces
         float* part = p.part + (size_t)(2 * blockIdx.x + (sg.b0 == 0 ? 1 : 0)) * C::kTile;
         for (int i = tid; i < rows * (HD / 8); i += 128) {
             const int r = i / (HD / 8), c = i % (HD / 8) * 8;
-            const float M = fmaxf(fmaxf(sm.m[0][r], sm.m[1][r]), fmaxf(sm.m[2][r], sm.m[3][r]));
-            float l = 0.f;
-#pragma unroll
-            for (int w = 0; w < 4; w++) l = fmaf(sm.l[w][r], piece_weight(sm.m[w][r], M), l);
+            const float M = sm.m[0][r], l = sm.l[0][r];
             const float4 u = *reinterpret_cast<const float4*>(&sm.o[r * C::kLd + c]);
             const float4 v = *reinterpret_cast<const float4*>(&sm.o[r * C::kLd + c + 4]);
             if (whole) {
@@ -445,47 +610,31 @@ __global__ void __launch_bounds__(kThreads) attn_short_kernel(const __grid_const
             }
         }
         if (!whole) {
-            const int last_cta = (sg.x0 + sg.nb - 1) / per;
-            __threadfence();
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (tid == 0) {
-                const int before = atomicAdd(&p.counters[own], 1);
+            // true for the CTA that finds the other n - 1 arrivals counted (and resets the count)
+            auto last_of = [&](int* count, int all) {
                 __threadfence();
-                sm.last = before == last_cta - own;
-                if (sm.last) p.counters[own] = 0;
-            }
-            asm volatile("bar.sync 1, 128;" ::: "memory");
-            if (sm.last) {
-                // every piece has arrived: merge them in the line's order (the owner's piece, then the
-                // CTAs after it), one warp per row
-                for (int r = warp; r < rows; r += 4) {
-                    float M = -INFINITY;
-                    for (int c = own + lane; c <= last_cta; c += 32)
-                        M = fmaxf(M, __ldcg(p.part + (size_t)(2 * c + (c == own)) * C::kTile + R * HD + 2 * r));
-                    M = b2::warp_max(M);
-                    float l = 0.f, acc[HD / 32];
-#pragma unroll
-                    for (int i = 0; i < HD / 32; i++) acc[i] = 0.f;
-#pragma unroll 4
-                    for (int c = own; c <= last_cta; c++) {
-                        const float* q = p.part + (size_t)(2 * c + (c == own)) * C::kTile;
-                        const float2 ml = __ldcg(reinterpret_cast<const float2*>(q + R * HD + 2 * r));
-                        const float wgt = piece_weight(ml.x, M);
-                        l = fmaf(ml.y, wgt, l);
-#pragma unroll
-                        for (int i = 0; i < HD / 32; i++) acc[i] = fmaf(__ldcg(q + r * HD + 32 * i + lane), wgt, acc[i]);
-                    }
-                    const float inv = l == 0.f ? 0.f : 1.f / l;
-                    const size_t row = (size_t)(sg.sq.row0 + sg.i0 + r / p.G);
-                    const int h = sg.g * p.G + r % p.G;
-#pragma unroll
-                    for (int i = 0; i < HD / 32; i++)
-                        p.out16[(row * p.nq + h) * HD + 32 * i + lane] = __float2half_rn(acc[i] * inv);
-                    if (lane == 0 && p.lse) p.lse[row * p.nq + h] = l == 0.f ? -INFINITY : (M - kUp) * kLn2 + logf(l);
+                sync4();
+                if (tid == 0) {
+                    sm.last = atomicAdd(count, 1) == all - 1;
+                    __threadfence();
+                    if (sm.last) *count = 0;
+                }
+                sync4();
+                return sm.last != 0;
+            };
+            const int pieces = last - own + 1, me = (int)blockIdx.x;
+            if (pieces <= kFan) {
+                if (last_of(p.counters + 2 * own + 1, pieces)) merge_pieces<HD, NT>(p, sg, own, own, 1, pieces, true);
+            } else {
+                const int first = own + (me - own) / kFan * kFan, some = min(kFan, last - first + 1);
+                if (last_of(p.counters + 2 * first + (first == own), some)) {
+                    merge_pieces<HD, NT>(p, sg, own, first, 1, some, false);
+                    if (last_of(p.counters + 2 * gridDim.x + own, cdiv(pieces, kFan)))
+                        merge_pieces<HD, NT>(p, sg, own, own, kFan, cdiv(pieces, kFan), true);
                 }
             }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");  // the merge area is free for the next tile
+        sync4();  // the merge area is free for the next tile
     }
     if (!ok && lane == 0) atomicExch(p.err, 1);
     if (p.long_ctas) {
@@ -506,7 +655,7 @@ int short_grid(int dev, int sms) {
     int n = c.load(std::memory_order_relaxed);
     if (n == 0) {
         if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&n, attn_short_kernel<HD, NT>, kThreads,
-                                                          sizeof(ShortSmem<HD, NT>) + 1024) != cudaSuccess || n < 1)
+                                                          sizeof(ShortSmem<HD, NT>)) != cudaSuccess || n < 1)
             n = 1;
         n = n < 2 ? n : 2;
         c.store(n, std::memory_order_relaxed);
@@ -517,7 +666,8 @@ int short_grid(int dev, int sms) {
 template <int HD, int NT>
 int launch_short(const AttnParams& p, const B2PagedKV* kv, int dev, int sms, long long blocks, cudaStream_t s) {
     static std::atomic<unsigned long long> done{0};
-    constexpr size_t smem = sizeof(ShortSmem<HD, NT>) + 1024;
+    constexpr size_t smem = sizeof(ShortSmem<HD, NT>);
+    static_assert(smem <= 115712, "two CTAs per SM");
     cudaError_t e = allow_smem(attn_short_kernel<HD, NT>, smem, done, dev);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged smem: %s", cudaGetErrorString(e));
     CUtensorMap tk, tv;
@@ -542,7 +692,7 @@ int device_sms(int* dev) {
 
 // Workspace: counters, cuts, the short kernel's pieces (two of up to 16 rows for
 // each of at most two CTAs per SM), the long kernel's (two per SM).
-size_t short_part_bytes(int sms, int hd) { return (size_t)sms * 2 * 2 * kShortRows * (hd + 2) * sizeof(float); }
+size_t short_part_bytes(int sms, int hd) { return (size_t)sms * 2 * 2 * kShortRows * (hd + 4) * sizeof(float); }
 
 }  // namespace
 
