@@ -41,12 +41,12 @@ struct Batch {
 
     __device__ __forceinline__ Seq seq(int s) const {
         Seq x;
-        const int a = min(max(q_start[s], 0), M), b = min(max(q_start[s + 1], a), M), n = kv_len[s];
+        const int a = min(max(q_start[s], 0), M), b = min(max(q_start[s + 1], a), M), n = max(kv_len[s], 0);
         x.row0 = a;
         x.Q = b - a;
         x.base = n - x.Q;
         const long long cap = (long long)max_pages << page_shift;
-        x.len = n < 0 ? 0 : (int)((long long)n < cap ? n : cap);
+        x.len = (int)((long long)n < cap ? n : cap);
         return x;
     }
     // Page of slot j, or -1 where none is mapped.

@@ -26,7 +26,7 @@
 // The work of the call is one line of blocks, cut into equal stretches for the
 // CTAs; pairs that a cut divides leave pieces (maximum, sum, unnormalised O) in
 // the workspace, which the kernel launched behind this one merges.
-#include "b2_paged.cuh"
+#include "b2_tc.cuh"
 
 namespace {
 
@@ -65,67 +65,6 @@ struct Smem {
     int pre_seq[B2_PAGED_MAX_SEQS + 1];
     int pre[kMaxItems + 1];
 };
-
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void umma_commit(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-                 : "memory");
-}
-// Operand in 128-byte rows with the 128-byte swizzle, eight-row groups 1024 bytes
-// apart.  K-major (Q, K): a row is 64 consecutive k.  Also the form of V, whose
-// rows are k and whose 64-wide column chunks lie `lead` bytes apart.
-__device__ __forceinline__ uint64_t sw128_desc(uint32_t saddr, uint32_t lead) {
-    return (uint64_t)((saddr & 0x3FFFFu) >> 4) | ((uint64_t)((lead >> 4) & 0x3FFF) << 16) |
-           ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-// kind::f16: FP16 operands, FP32 accumulator; bit 16: B's rows are k (MN-major).
-__host__ __device__ constexpr uint32_t idesc_f16(int m, int n, bool b_mn) {
-    return (1u << 4) | ((uint32_t)b_mn << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(m >> 4) << 24);
-}
-__device__ __forceinline__ void umma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
-__device__ __forceinline__ void umma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t acc) {
-    asm volatile(
-        "{\n .reg .pred p;\n setp.ne.b32 p, %4, 0;\n tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc)
-        : "memory");
-}
-#define B2_R32(v, o)                                                                                                  \
-    "=r"(v[o + 0]), "=r"(v[o + 1]), "=r"(v[o + 2]), "=r"(v[o + 3]), "=r"(v[o + 4]), "=r"(v[o + 5]), "=r"(v[o + 6]),   \
-        "=r"(v[o + 7]), "=r"(v[o + 8]), "=r"(v[o + 9]), "=r"(v[o + 10]), "=r"(v[o + 11]), "=r"(v[o + 12]),            \
-        "=r"(v[o + 13]), "=r"(v[o + 14]), "=r"(v[o + 15]), "=r"(v[o + 16]), "=r"(v[o + 17]), "=r"(v[o + 18]),         \
-        "=r"(v[o + 19]), "=r"(v[o + 20]), "=r"(v[o + 21]), "=r"(v[o + 22]), "=r"(v[o + 23]), "=r"(v[o + 24]),         \
-        "=r"(v[o + 25]), "=r"(v[o + 26]), "=r"(v[o + 27]), "=r"(v[o + 28]), "=r"(v[o + 29]), "=r"(v[o + 30]),         \
-        "=r"(v[o + 31])
-// 32 columns of this warp's lanes (no wait).
-template <int O, int N>
-__device__ __forceinline__ void tmem_ld32(uint32_t addr, uint32_t (&v)[N]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
-        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : B2_R32(v, O)
-        : "r"(addr)
-        : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-#define B2_I32(v)                                                                                                \
-    "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]), \
-        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]),          \
-        "r"(v[18]), "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]),          \
-        "r"(v[26]), "r"(v[27]), "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const uint32_t (&v)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-        "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-        B2_I32(v)
-        : "memory");
-}
 
 // A stretch's part of one tile pair: blocks [b0, b1) of its nb.
 struct Seg {
@@ -208,11 +147,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
     }
-    if (warp == 9) {
-        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sm.tmem)), "n"(512)
-                     : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-    }
+    if (warp == 9) tmem_alloc512(&sm.tmem);
     b2::pdl_wait();
     // The kernel behind this one works on other rows and waits for this grid before
     // it merges, but it does not wait for the kernels before this one: let it start
@@ -514,7 +449,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     __syncthreads();
     if (warp == 9) {
         tc_fence_after();
-        asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "n"(512) : "memory");
+        tmem_free512(tmem);
     }
 }
 
@@ -528,10 +463,7 @@ int launch_long(LongParams& p, const B2PagedKV* kv, int dev, int sms, cudaStream
     const int box = kv->page_size < kBlk ? kv->page_size : kBlk;
     int rc = b2_paged_map(&tk, kv->k_pages, kv, p.a.nkv, HD, box, 1);
     if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, p.a.nkv, HD, box, 1);
-    const uint64_t dims[5] = {64, (uint64_t)p.a.G, (uint64_t)p.a.bt.M, (uint64_t)HD / 64, (uint64_t)p.a.nkv};
-    const uint64_t strides[4] = {(uint64_t)HD * 2, (uint64_t)p.a.ldq * 2, 128, (uint64_t)p.a.G * HD * 2};
-    const uint32_t bx[5] = {64, (uint32_t)p.a.G, (uint32_t)p.T, 1, 1};
-    if (!rc) rc = b2_tensor_map_f16_5d(&tq, p.a.q16, dims, strides, bx);
+    if (!rc) rc = q_map(&tq, p.a.q16, p.a.ldq, p.a.bt.M, p.a.nkv, p.a.G, HD, p.T);
     if (rc) return rc;
     e = b2::launch_pdl(attn_long_kernel<HD>, dim3(sms), dim3(kThreads), smem, s, tq, tk, tv, p);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged: %s", cudaGetErrorString(e));

@@ -5,14 +5,14 @@
 // over the new rows i that see slot j, from q, K and the row sums that the
 // attention left.  Every slot belongs to one warp, which adds its rows in
 // their order: no atomics, and the result does not depend on timing.
-#include "b2_paged.cuh"
+#include "b2_tc.cuh"
 
 namespace {
 
-constexpr float kLog2e = 1.4426950408889634f;
+using namespace b2p;
 
 struct WeightParams {
-    b2p::Batch bt;
+    Batch bt;
     const uint16_t* k;
     long long page_stride, head_stride, row_stride;
     const __half* q16;
@@ -22,6 +22,9 @@ struct WeightParams {
     float* weights;
     const float* prev;
     long long ldw;
+    int short_rows;  // sequences with at most this many (token, head) rows per kv head are the short kernel's
+    int after_long;  // the long kernel was launched before the short one
+    int* err;
 };
 
 // ─── few rows per sequence ───
@@ -38,14 +41,19 @@ template <int HD>
 __global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightParams p) {
     __shared__ int pre[B2_PAGED_MAX_SEQS + 1];
     b2::pdl_trigger();
-    b2::pdl_wait();
+    // Behind the long kernel this grid starts once that one's CTAs have seen the
+    // kernels before them complete, works beside them and waits for them at the end.
+    if (!p.after_long) b2::pdl_wait();
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c4 = lane & 3;
-    b2p::prefix_work(pre, p.bt.n_seqs, [&](int s) { return (p.bt.seq(s).len + kBlk - 1) / kBlk * p.nkv; });
+    prefix_work(pre, p.bt.n_seqs, [&](int s) {
+        const Seq q = p.bt.seq(s);
+        return min(q.Q, p.max_q) * p.G > p.short_rows ? 0 : cdiv(q.len, kBlk) * p.nkv;
+    });
     const int W = pre[p.bt.n_seqs];
     const float scale = kLog2e / sqrtf((float)HD);
     for (int x = blockIdx.x; x < W; x += gridDim.x) {
-        const int s = b2p::prefix_find(pre, p.bt.n_seqs, x);
-        const b2p::Seq sq = p.bt.seq(s);
+        const int s = prefix_find(pre, p.bt.n_seqs, x);
+        const Seq sq = p.bt.seq(s);
         const int nb = (sq.len + kBlk - 1) / kBlk, g = (x - pre[s]) / nb, j0 = (x - pre[s]) % nb * kBlk + warp * 16;
         if (j0 >= sq.len) continue;
         const int page = p.bt.page(s, j0);
@@ -84,13 +92,13 @@ __global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightPar
                 for (int u = 0; u < HD / 32; u++) {
                     const uint32_t f0[4] = {a[0][u].x, a[1][u].x, a[0][u].y, a[1][u].y};
                     const uint32_t f1[4] = {a[0][u].z, a[1][u].z, a[0][u].w, a[1][u].w};
-                    b2p::mma16816(sc, f0, b[u].x, b[u].y);
-                    b2p::mma16816(sc, f1, b[u].z, b[u].w);
+                    mma16816(sc, f0, b[u].x, b[u].y);
+                    mma16816(sc, f1, b[u].z, b[u].w);
                 }
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
-                    if (ja <= lim[e]) acc[0] += b2p::ex2(fmaf(sc[e], scale, -l2[e]));
-                    if (jb <= lim[e]) acc[1] += b2p::ex2(fmaf(sc[e + 2], scale, -l2[e]));
+                    if (ja <= lim[e]) acc[0] += ex2(fmaf(sc[e], scale, -l2[e]));
+                    if (jb <= lim[e]) acc[1] += ex2(fmaf(sc[e + 2], scale, -l2[e]));
                 }
             }
         }
@@ -105,7 +113,366 @@ __global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightPar
             p.weights[o] = (p.prev ? p.prev[o] : 0.f) + (c4 == 0 ? acc[0] : acc[1]);
         }
     }
+    if (p.after_long) b2::pdl_wait();
 }
+
+// ─── many rows per sequence: chunks ───
+//
+// Bound by the exponentials (16 per clock and SM), before the product (2 hd FLOP
+// per pair).  A unit is 256 slots of one kv head: two K tiles of 128 slots, each
+// the A operand of S^T_t = K_t Q^T (tcgen05, N = 128 rows: T tokens x the G heads
+// of the group), so a thread owns a slot and adds its columns in registers, and a
+// Q tile brought in once serves both K tiles.  The CTAs of a cluster take every
+// S-th Q tile of a unit; their sums meet in the first one's shared memory and are
+// added in rank order.
+//   warp 8      producer: the unit's K tiles (double-buffered), Q tiles and their
+//               rows' -lse;
+//   warp 9      tensor cores;
+//   warps 0-3, 4-7   the exponentials of K tile 0 and 1, one slot per thread.
+constexpr int kUnit = 256;
+constexpr int kLongThreads = 320;
+constexpr int kRowsT = 128;  // rows of a Q tile
+constexpr int kMaxCluster = 4;
+
+template <int HD>
+struct LongSmem {
+    static constexpr int kTile = 128 * HD * 2;
+    alignas(1024) unsigned char k[2][2][kTile];  // [buffer][tile]
+    alignas(1024) unsigned char q[2][kTile];
+    alignas(16) float nl[8][kRowsT];             // -lse log2(e) of the rows of Q tile (count % 8)
+    float part[2][kMaxCluster - 1][kUnit];       // first CTA: the others' sums, by unit parity
+    uint64_t k_full[2], k_empty[2], q_full[2], q_empty[2];
+    uint64_t s_full[2][2], s_free[2][2];         // [K tile][buffer]
+    uint64_t sum_full[2], sum_free[2];
+    uint64_t drain;
+    uint32_t tmem;
+    int failed;
+    int pre[B2_PAGED_MAX_SEQS + 1];
+};
+
+struct Unit {
+    int s, g, j0;       // sequence, kv head, first slot
+    int tiles, first;   // Q tiles of the sequence, and the first that sees a slot of the unit
+    int rows;           // (token, head) rows
+    Seq sq;
+};
+
+__device__ __forceinline__ Unit find_unit(const WeightParams& p, const int* pre, int T, int x) {
+    Unit u;
+    u.s = prefix_find(pre, p.bt.n_seqs, x);
+    u.sq = p.bt.seq(u.s);
+    const int nb = cdiv(u.sq.len, kUnit), off = x - pre[u.s];
+    u.g = off / nb;
+    u.j0 = off % nb * kUnit;
+    const int toks = min(u.sq.Q, p.max_q);
+    u.rows = toks * p.G;
+    u.tiles = cdiv(toks, T);
+    u.first = max(0, u.j0 - u.sq.base) / T;
+    return u;
+}
+
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ uint32_t in_rank(const void* p, uint32_t rank) {
+    uint32_t r;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(smem_u32(p)), "r"(rank));
+    return r;
+}
+__device__ __forceinline__ void remote_arrive(uint32_t bar) {
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+// mbar_wait whose barrier other CTAs of the cluster arrive on.
+__device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+    for (long long it = 0;; it++) {
+        uint32_t ok;
+        asm volatile(
+            "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, "
+            "0, p;\n}\n"
+            : "=r"(ok)
+            : "r"(smem_u32(bar)), "r"(parity)
+            : "memory");
+        if (ok) return true;
+        if (it > kWaitLimit || *failed) {
+            *failed = 1;
+            return false;
+        }
+    }
+}
+
+template <int HD>
+__global__ void __launch_bounds__(kLongThreads, 1)
+    weights_long_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const WeightParams p,
+                        int S) {
+    using Sm = LongSmem<HD>;
+    constexpr int kHalves = HD / 64;
+    extern __shared__ unsigned char smem_raw[];
+    Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int rank = S > 1 ? (int)cluster_rank() : 0;
+    volatile int* failed = &sm.failed;
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; i++) {
+            mbar_init(&sm.k_full[i], 1);
+            mbar_init(&sm.k_empty[i], 1);
+            mbar_init(&sm.q_full[i], 1);
+            mbar_init(&sm.q_empty[i], 1);
+            for (int t = 0; t < 2; t++) {
+                mbar_init(&sm.s_full[t][i], 1);
+                mbar_init(&sm.s_free[t][i], 128);
+            }
+            mbar_init(&sm.sum_full[i], 256 * (S - 1) + (S == 1));
+            mbar_init(&sm.sum_free[i], 256);
+        }
+        mbar_init(&sm.drain, 1);
+        sm.failed = 0;
+        mbar_init_fence();
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tq) : "memory");
+        asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
+    }
+    if (warp == 9) tmem_alloc512(&sm.tmem);
+    b2::pdl_wait();
+    b2::pdl_trigger();  // only now: the kernel behind this one does not wait for those before it
+    const int T = kRowsT / p.G;
+    prefix_work(sm.pre, p.bt.n_seqs, [&](int s) {
+        const Seq q = p.bt.seq(s);
+        return min(q.Q, p.max_q) * p.G > p.short_rows ? cdiv(q.len, kUnit) * p.nkv : 0;
+    });
+    tc_fence_before();
+    __syncthreads();
+    if (S > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    tc_fence_after();
+    const uint32_t tmem = sm.tmem;
+    const int W = sm.pre[p.bt.n_seqs], step = gridDim.x / S;
+    bool ok = true;
+
+    if (warp == 8) {
+        // ── producer ──
+        const int page_rows = 1 << p.bt.page_shift, box_rows = min(page_rows, 128), boxes = 128 / box_rows;
+        const int box = lane / kHalves, half = lane % kHalves;
+        int nu = 0, nq = 0;  // units and Q tiles loaded
+        for (int x = blockIdx.x / S; x < W && ok; x += step) {
+            const Unit u = find_unit(p, sm.pre, T, x);
+            if (u.first + rank >= u.tiles) continue;
+            const int kb = nu & 1;
+            if (nu >= 2 && !mbar_wait(&sm.k_empty[kb], (nu / 2 - 1) & 1, failed)) ok = false;
+            ok = __all_sync(0xffffffffu, ok);
+            if (!ok) break;
+            nu++;
+            if (lane == 0) mbar_expect_tx(&sm.k_full[kb], 2 * Sm::kTile);
+            __syncwarp();
+            if (box < boxes)
+                for (int t = 0; t < 2; t++) {
+                    const int j = u.j0 + t * 128 + box * box_rows;
+                    const int page = j < u.sq.len ? p.bt.page(u.s, j) : -1;
+                    tma_load_5d(sm.k[kb][t] + half * 16384 + box * box_rows * 128, &tk, 0, j & (page_rows - 1), half, u.g,
+                                page >= 0 ? page : p.bt.n_pages, &sm.k_full[kb]);
+                }
+            for (int i = u.first + rank; i < u.tiles; i += S, nq++) {
+                const int qb = nq & 1;
+                float nl[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int r = i * T * p.G + 32 * e + lane;  // rows of tile i are T G consecutive ones
+                    const bool in = 32 * e + lane < T * p.G && r < u.rows;
+                    const float l = in ? p.lse[(size_t)(u.sq.row0 + r / p.G) * p.nq + u.g * p.G + r % p.G] : -INFINITY;
+                    nl[e] = l == -INFINITY ? -INFINITY : -l * kLog2e;
+                }
+                if (nq >= 2 && !mbar_wait(&sm.q_empty[qb], (nq / 2 - 1) & 1, failed)) ok = false;
+                ok = __all_sync(0xffffffffu, ok);
+                if (!ok) break;
+#pragma unroll
+                for (int e = 0; e < 4; e++) sm.nl[nq & 7][32 * e + lane] = nl[e];
+                __syncwarp();
+                if (lane == 0) mbar_expect_tx(&sm.q_full[qb], T * p.G * HD * 2);
+                __syncwarp();
+                if (lane < kHalves)
+                    tma_load_5d(sm.q[qb] + lane * 16384, &tq, 0, 0, u.sq.row0 + i * T, lane, u.g, &sm.q_full[qb]);
+            }
+        }
+        if (!ok && lane == 0) {  // let the copies in flight land (bounded) before the CTA ends
+            for (int i = max(0, nu - 2); i < nu; i++)
+                for (long long it = 0; it <= kWaitLimit; it++)
+                    if (mbar_try_wait(&sm.k_full[i & 1], (i / 2) & 1)) break;
+            for (int i = max(0, nq - 2); i < nq; i++)
+                for (long long it = 0; it <= kWaitLimit; it++)
+                    if (mbar_try_wait(&sm.q_full[i & 1], (i / 2) & 1)) break;
+        }
+    } else if (warp == 9) {
+        // ── tensor cores ──
+        if (lane == 0) {
+            constexpr uint32_t id = idesc_f16(128, kRowsT, false);
+            int nu = 0, nq = 0;
+            for (int x = blockIdx.x / S; x < W && ok; x += step) {
+                const Unit u = find_unit(p, sm.pre, T, x);
+                if (u.first + rank >= u.tiles) continue;
+                const int kb = nu & 1;
+                ok = mbar_wait(&sm.k_full[kb], (nu / 2) & 1, failed);
+                nu++;
+                for (int i = u.first + rank; i < u.tiles && ok; i += S, nq++) {
+                    const int b = nq & 1;
+                    ok = mbar_wait(&sm.q_full[b], (nq / 2) & 1, failed);
+                    for (int t = 0; t < 2 && ok; t++) {
+                        if (nq >= 2) ok = mbar_wait(&sm.s_free[t][b], (nq / 2 - 1) & 1, failed);
+                        if (!ok) break;
+                        tc_fence_after();
+                        const uint32_t ka = smem_u32(sm.k[kb][t]), qa = smem_u32(sm.q[b]);
+#pragma unroll
+                        for (int e = 0; e < HD / 16; e++) {
+                            const uint32_t o = (e >> 2) * 16384 + (e & 3) * 32;
+                            umma_ss(tmem + (2 * t + b) * 128, sw128_desc(ka + o, 16), sw128_desc(qa + o, 16), id, e != 0);
+                        }
+                        umma_commit(&sm.s_full[t][b]);
+                    }
+                    umma_commit(&sm.q_empty[b]);
+                }
+                umma_commit(&sm.k_empty[kb]);
+            }
+            if (!ok) {  // nothing of the tensor cores may be left running
+                umma_commit(&sm.drain);
+                for (long long it = 0; it <= kWaitLimit; it++)
+                    if (mbar_try_wait(&sm.drain, 0)) break;
+            }
+        }
+    } else {
+        // ── exponentials of K tile t: thread = slot ──
+        const int t = warp >> 2, slot = threadIdx.x;
+        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
+        const float scale = kLog2e / sqrtf((float)HD);
+        int nq = 0, done = 0;  // Q tiles; units (all of them, with work here or not)
+        for (int x = blockIdx.x / S; x < W && ok; x += step, done++) {
+            const Unit u = find_unit(p, sm.pre, T, x);
+            const int j = u.j0 + slot;
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+            for (int i = u.first + rank; i < u.tiles; i += S, nq++) {
+                const int b = nq & 1;
+                ok = mbar_wait(&sm.s_full[t][b], (nq / 2) & 1, failed);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                tc_fence_after();
+                const uint32_t ts = tmem + lanes + (2 * t + b) * 128;
+                uint32_t sv[128];
+                tmem_ld32<0>(ts, sv);
+                tmem_ld32<32>(ts + 32, sv);
+                tmem_ld32<64>(ts + 64, sv);
+                tmem_ld32<96>(ts + 96, sv);
+                tmem_wait_ld();
+                tc_fence_before();
+                mbar_arrive(&sm.s_free[t][b]);
+                // columns of tokens from the slot's own on, and rows that exist
+                const int c0 = min(j - u.sq.base - i * T, kRowsT) * p.G, c1 = min(T * p.G, u.rows - i * T * p.G);
+                const float* nl = sm.nl[nq & 7];
+                if (__any_sync(0xffffffffu, c0 > 0 || c1 < kRowsT)) {
+#pragma unroll
+                    for (int c = 0; c < kRowsT; c++)
+                        if (c < c0 || c >= c1) sv[c] = 0xff800000u;  // -inf
+                }
+#pragma unroll
+                for (int c = 0; c < kRowsT; c += 4) {
+                    const float4 n4 = *reinterpret_cast<const float4*>(nl + c);
+                    acc[0] += ex2(fmaf(__uint_as_float(sv[c]), scale, n4.x));
+                    acc[1] += ex2(fmaf(__uint_as_float(sv[c + 1]), scale, n4.y));
+                    acc[2] += ex2(fmaf(__uint_as_float(sv[c + 2]), scale, n4.z));
+                    acc[3] += ex2(fmaf(__uint_as_float(sv[c + 3]), scale, n4.w));
+                }
+            }
+            if (!ok) break;
+            float total = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+            const int par = done & 1;
+            if (rank > 0) {
+                // to the first CTA, once it has read what this buffer held two units ago
+                if (done >= 2) ok = cluster_wait(&sm.sum_free[par], (done / 2 - 1) & 1, failed);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_rank(&sm.part[par][rank - 1][slot], 0)), "f"(total)
+                             : "memory");
+                remote_arrive(in_rank(&sm.sum_full[par], 0));
+                continue;
+            }
+            if (S > 1) {
+                ok = cluster_wait(&sm.sum_full[par], (done / 2) & 1, failed);
+                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                for (int e = 1; e < S; e++) total += sm.part[par][e - 1][slot];
+                for (int e = 1; e < S; e++) remote_arrive(in_rank(&sm.sum_free[par], e));
+            }
+            if (j < u.sq.len && j < p.ldw) {
+                const size_t o = ((size_t)u.s * p.nkv + u.g) * p.ldw + j;
+                p.weights[o] = (p.prev ? p.prev[o] : 0.f) + (p.bt.page(u.s, j) >= 0 ? total : 0.f);
+            }
+        }
+    }
+    if (!ok && lane == 0) atomicExch(p.err, 1);
+    tc_fence_before();
+    __syncthreads();
+    // the others may still write to or arrive at this CTA's shared memory
+    if (S > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    if (warp == 9) {
+        tc_fence_after();
+        tmem_free512(tmem);
+    }
+}
+
+// Clusters of S CTAs that fit the device at once.
+template <int HD>
+int max_clusters(int S, int dev, int sms, size_t smem) {
+    if (S == 1) return sms;
+    static std::atomic<int> known[64][kMaxCluster + 1];
+    std::atomic<int>& c = known[dev & 63][S];
+    int n = c.load(std::memory_order_relaxed);
+    if (n == 0) {
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3(S);
+        cfg.blockDim = dim3(kLongThreads);
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute at[1];
+        at[0].id = cudaLaunchAttributeClusterDimension;
+        at[0].val.clusterDim.x = S;
+        at[0].val.clusterDim.y = at[0].val.clusterDim.z = 1;
+        cfg.attrs = at;
+        cfg.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&n, weights_long_kernel<HD>, &cfg) != cudaSuccess || n < 1) {
+            cudaGetLastError();
+            return 0;
+        }
+        c.store(n, std::memory_order_relaxed);
+    }
+    return n;
+}
+
+template <int HD>
+int launch_long(const WeightParams& p, const B2PagedKV* kv, int dev, int sms, cudaStream_t s) {
+    static std::atomic<unsigned long long> allowed{0};
+    constexpr size_t smem = sizeof(LongSmem<HD>) + 1024;
+    cudaError_t e = allow_smem(weights_long_kernel<HD>, smem, allowed, dev);
+    if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged_weights smem: %s", cudaGetErrorString(e));
+    CUtensorMap tq, tk;
+    const int box = kv->page_size < 128 ? kv->page_size : 128, T = kRowsT / p.G;
+    int rc = b2_paged_map(&tk, kv->k_pages, kv, p.nkv, HD, box, 1);
+    if (!rc) rc = q_map(&tq, p.q16, p.ldq, p.bt.M, p.nkv, p.G, HD, T);
+    if (rc) return rc;
+    // as many CTAs per unit as Q tiles can keep busy
+    const int tiles = cdiv(p.max_q, T);
+    int S = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1, clusters = max_clusters<HD>(S, dev, sms, smem);
+    if (clusters == 0) clusters = sms, S = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(clusters * S);
+    cfg.blockDim = dim3(kLongThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = S;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = S > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, weights_long_kernel<HD>, tq, tk, p, S);
+    if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged_weights: %s", cudaGetErrorString(e));
+    return 0;
+}
+
+constexpr int kShortRows = 64;
 
 }  // namespace
 
@@ -129,8 +496,15 @@ extern "C" int b2_attention_paged_weights(float* weights, const float* prev, lon
     int dev = 0, sms = 148;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    const WeightParams p{b2p::make_batch(kv, M), kv->k_pages, kv->page_stride, kv->head_stride, kv->row_stride,
-                         reinterpret_cast<const __half*>(q16), ldq, lse, max_q, nq, nkv, nq / nkv, weights, prev, ldw};
+    if (max_q > M) max_q = M;
+    WeightParams p{make_batch(kv, M), kv->k_pages, kv->page_stride, kv->head_stride, kv->row_stride,
+                         reinterpret_cast<const __half*>(q16), ldq, lse, max_q, nq, nkv, nq / nkv, weights, prev, ldw,
+                   kShortRows, 0, err};
+    if ((long long)max_q * p.G > kShortRows) {
+        rc = hd == 128 ? launch_long<128>(p, kv, dev, sms, (cudaStream_t)s) : launch_long<64>(p, kv, dev, sms, (cudaStream_t)s);
+        if (rc) return rc;
+        p.after_long = 1;
+    }
     const long long grid = blocks < sms * 8 ? blocks : sms * 8;
     const cudaError_t e = b2::launch_pdl(hd == 128 ? weights_short_kernel<128> : weights_short_kernel<64>,
                                          dim3((unsigned)grid), dim3(kThreads), 0, (cudaStream_t)s, p);
