@@ -153,12 +153,19 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(
 
 // ─── b2_kv_evict_paged ───
 //
-// Selection per (sequence, kv head): the slots become keys that order as the
-// contract does (0: not mapped, the largest: always kept, else the weight's
-// order), and the k-th largest key is found 8 bits at a time from histograms.
+// Selection: a cluster of S CTAs per (sequence, kv head), each with an S-th of
+// the slots.  A slot becomes a key that orders as the contract does (0: not
+// mapped, the largest: always kept, else the weight's order), held in shared
+// memory, and the k-th largest key is found 8 bits at a time from histograms that
+// the CTAs add up through distributed shared memory (one cluster barrier a digit).
 // Slots above it are kept, and as many of those equal to it as are missing,
-// lowest first; block-wide scans give their places in slot order.
-constexpr int kSelThreads = 1024;
+// lowest first.  A warp owns a contiguous run of its CTA's slots, 32 at a time, so
+// ballots give the places in slot order and one scan over the warps joins them.
+// Bound by latency: four digits of a few microseconds.
+constexpr int kSelThreads = 512;  // two CTAs per SM
+constexpr int kSelWarps = kSelThreads / 32;
+constexpr int kMaxKeys = 48 * 1024;  // keys a CTA holds; more are formed again for every digit
+constexpr int kMaxSplit = 8;
 
 __device__ __forceinline__ uint32_t evict_key(const b2p::Batch& bt, const float* w, long long ldw, int s, int j, int len,
                                               int sink, int recent) {
@@ -169,92 +176,182 @@ __device__ __forceinline__ uint32_t evict_key(const b2p::Batch& bt, const float*
     return min(max(k, 1u), 0xFFFFFFFEu);
 }
 
-// Inclusive scan over the CTA of one int per thread; total in *sum.
-__device__ __forceinline__ int block_scan(int v, int* ws, int* sum) {
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int t = __shfl_up_sync(0xffffffffu, v, o);
-        if (lane >= o) v += t;
-    }
-    if (lane == 31) ws[warp] = v;
-    __syncthreads();
-    int before = 0, all = 0;
-    for (int i = 0; i < kSelThreads / 32; i++) {
-        if (i < warp) before += ws[i];
-        all += ws[i];
-    }
-    __syncthreads();
-    *sum = all;
-    return v + before;
+__device__ __forceinline__ int ld_rank(const int* p, int rank) {
+    uint32_t a;
+    int v;
+    asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(b2p::smem_u32(p)), "r"(rank));
+    asm volatile("ld.shared::cluster.s32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+    return v;
+}
+__device__ __forceinline__ void sync_cluster(int S) {
+    if (S > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    else __syncthreads();
 }
 
-__global__ void __launch_bounds__(kSelThreads) evict_select_kernel(b2p::Batch bt, const float* __restrict__ weights,
+// S = gridDim.x.
+__global__ void __launch_bounds__(kSelThreads, 2) evict_select_kernel(b2p::Batch bt, const float* __restrict__ weights,
                                                                    long long ldw, int nkv, int budget, int sink,
-                                                                   int recent, int* __restrict__ kept,
+                                                                   int recent, int held, int* __restrict__ kept,
                                                                    float* __restrict__ dst_weights,
                                                                    int* __restrict__ new_len) {
-    __shared__ int hist[256];
-    __shared__ int ws[kSelThreads / 32];
-    __shared__ int sh[2];
+    extern __shared__ uint32_t keys[];
+    __shared__ int hist[2][257];  // [digit parity]; [256]: unmapped slots
+    __shared__ int sum[256];
+    __shared__ int counts[2];     // slots above the k-th key, and equal to it
+    __shared__ int warp_gt[kSelWarps], warp_eq[kSelWarps];
+    __shared__ int found[2], before[2], unmapped;
+    const int S = gridDim.x, rank = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     b2::pdl_trigger();
     b2::pdl_wait();
-    const int s = blockIdx.y, g = blockIdx.x, tid = threadIdx.x;
-    const int n = bt.kv_len[s];
+    const int n = max(bt.kv_len[s], 0);
     const long long cap = (long long)bt.max_pages << bt.page_shift;
-    const int len = n < 0 ? 0 : (int)((long long)n < cap ? n : cap);
+    const int len = (int)((long long)n < cap ? n : cap);
+    // this CTA's slots, and this warp's: whole groups of 32
+    const int groups = b2p::cdiv(len, 32), cta_g = b2p::cdiv(groups, S), warp_g = b2p::cdiv(cta_g, kSelWarps);
+    const int g0 = min(groups, rank * cta_g), g1 = min(groups, g0 + cta_g);
+    const int w0 = min(g1, g0 + warp * warp_g), w1 = min(g1, w0 + warp_g);
+    const bool cached = cta_g * 32 <= held;
     const float* w = weights + ((size_t)s * nkv + g) * ldw;
-    // mapped slots
-    int cnt = 0, mapped;
-    for (int j = tid; j < len; j += kSelThreads) cnt += bt.page(s, j) >= 0;
-    block_scan(cnt, ws, &mapped);
-    const int k = min(mapped, budget);
-    if (g == 0 && tid == 0) new_len[s] = k;
-    if (k == 0) return;
-    uint32_t prefix = 0;
-    int need = k;  // slots still to take among those that match the prefix
-    for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
-        for (int j = tid; j < len; j += kSelThreads) {
-            const uint32_t key = evict_key(bt, w, ldw, s, j, len, sink, recent);
-            if (shift == 24 || (key >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&hist[(key >> shift) & 255], 1);
+    auto make_key = [&](int j) { return j < len ? evict_key(bt, w, ldw, s, j, len, sink, recent) : 0u; };
+    auto key_of = [&](int q) { return cached ? keys[(q - g0) * 32 + lane] : make_key(q * 32 + lane); };
+    for (int i = tid; i < 2 * 257; i += kSelThreads) (&hist[0][0])[i] = 0;
+    if (cached) {
+#pragma unroll 4
+        for (int q = w0; q < w1; q++) keys[(q - g0) * 32 + lane] = make_key(q * 32 + lane);
+    }
+    __syncthreads();
+    uint32_t prefix = 0;  // the digits found so far of the k-th largest key
+    int need = 0, k = 0;  // slots still to take among those that share them; slots kept
+    for (int d = 0; d < 4; d++) {
+        const int shift = 24 - 8 * d;
+        int* h = hist[d & 1];
+        int none = 0;
+        for (int q = w0; q < w1; q++) {
+            const uint32_t key = key_of(q);
+            const bool in = key != 0 && (d == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+            if (d == 0) none += q * 32 + lane < len && key == 0;
+            // one addition per distinct digit of the warp: weights share exponents
+            const unsigned same = __match_any_sync(0xffffffffu, in ? (key >> shift) & 255 : 256u);
+            if (in && lane == __ffs(same) - 1) atomicAdd(&h[(key >> shift) & 255], __popc(same));
+        }
+        if (d == 0) {
+            none = __reduce_add_sync(0xffffffffu, none);
+            if (lane == 0 && none) atomicAdd(&h[256], none);
+        }
+        sync_cluster(S);
+        if (tid < 256) {
+            int v = 0;
+            for (int r = 0; r < S; r++) v += S > 1 ? ld_rank(&h[tid], r) : h[tid];
+            sum[tid] = v;
+        }
+        if (d == 0 && tid == 256) {
+            int v = 0;
+            for (int r = 0; r < S; r++) v += S > 1 ? ld_rank(&h[256], r) : h[256];
+            unmapped = v;
         }
         __syncthreads();
+        if (d == 0) {
+            k = min(len - unmapped, budget);
+            need = k;
+            if (k == 0 || k == len - unmapped) break;  // nothing to choose
+        }
+        if (warp == 0) {
+            // from the top: lane l has bins 255 - 8 l - 7 .. 255 - 8 l
+            int c[8], t = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) t += c[e] = sum[255 - 8 * lane - e];
+            int incl = t;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, incl, o);
+                if (lane >= o) incl += u;
+            }
+            int over = incl - t;  // slots in higher bins
+            if (over < need && incl >= need) {
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    if (over < need && over + c[e] >= need) {
+                        found[0] = 255 - 8 * lane - e;
+                        found[1] = need - over;
+                    }
+                    over += c[e];
+                }
+            }
+        }
+        // the other parity's bins were read behind the barrier before this one
+        if (d > 0)
+            for (int i = tid; i < 256; i += kSelThreads) hist[(d + 1) & 1][i] = 0;
+        __syncthreads();
+        prefix |= (uint32_t)found[0] << shift;
+        need = found[1];
+    }
+    if (rank == 0 && g == 0 && tid == 0) new_len[s] = k;
+    const bool every = k == len - unmapped;
+    const uint32_t bar = every ? 0u : prefix;  // kept: keys above, and `need` of those equal
+    if (every) need = 0;
+    if (k > 0) {  // the same for every CTA of the cluster
+        int gt = 0, eq = 0;
+        for (int q = w0; q < w1; q++) {
+            const uint32_t key = key_of(q);
+            gt += key > bar;
+            eq += key == bar && !every;
+        }
+        gt = __reduce_add_sync(0xffffffffu, gt);
+        eq = __reduce_add_sync(0xffffffffu, eq);
+        if (lane == 0) {
+            warp_gt[warp] = gt;
+            warp_eq[warp] = eq;
+        }
+        __syncthreads();
+        if (warp == 0) {  // exclusive sums over the warps
+            int a = lane < kSelWarps ? warp_gt[lane] : 0, b = lane < kSelWarps ? warp_eq[lane] : 0;
+            const int a0 = a, b0 = b;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int u = __shfl_up_sync(0xffffffffu, a, o), v = __shfl_up_sync(0xffffffffu, b, o);
+                if (lane >= o) a += u, b += v;
+            }
+            if (lane < kSelWarps) {
+                warp_gt[lane] = a - a0;
+                warp_eq[lane] = b - b0;
+            }
+            if (lane == 31) counts[0] = a, counts[1] = b;
+        }
+        sync_cluster(S);
         if (tid == 0) {
-            int b = 255, sum = 0;
-            while (b > 0 && sum + hist[b] < need) sum += hist[b--];
-            sh[0] = b;
-            sh[1] = need - sum;
+            int a = 0, b = 0;
+            for (int r = 0; r < rank; r++) {
+                a += ld_rank(&counts[0], r);
+                b += ld_rank(&counts[1], r);
+            }
+            before[0] = a;
+            before[1] = b;
         }
         __syncthreads();
-        prefix |= (uint32_t)sh[0] << shift;
-        need = sh[1];
-        __syncthreads();
-    }
-    // prefix is the k-th largest key; `need` of the slots that equal it are kept
-    int ties = 0, out = 0;
-    const size_t o0 = ((size_t)s * nkv + g) * budget;
-    for (int b = 0; b < len; b += kSelThreads) {
-        const int j = b + tid;
-        const uint32_t key = j < len ? evict_key(bt, w, ldw, s, j, len, sink, recent) : 0u;
-        const bool eq = j < len && key == prefix;
-        int all;
-        const int rank = ties + block_scan(eq ? 1 : 0, ws, &all);
-        ties += all;
-        const bool take = (j < len && key > prefix) || (eq && rank <= need);
-        const int at = out + block_scan(take ? 1 : 0, ws, &all) - 1;
-        out += all;
-        if (take) {
-            kept[o0 + at] = j;
-            if (dst_weights) dst_weights[o0 + at] = j < ldw ? w[j] : 0.f;
+        int above = before[0] + warp_gt[warp], equal = before[1] + warp_eq[warp];  // in slots before this group
+        const size_t o0 = ((size_t)s * nkv + g) * budget;
+        const unsigned below = (1u << lane) - 1;
+        for (int q = w0; q < w1; q++) {
+            const uint32_t key = key_of(q);
+            const unsigned bg = __ballot_sync(0xffffffffu, key > bar), be = __ballot_sync(0xffffffffu, key == bar && !every);
+            const int eq_rank = equal + __popc(be & below);
+            if (key > bar || (key == bar && !every && eq_rank < need)) {
+                const int j = q * 32 + lane, at = above + __popc(bg & below) + min(eq_rank, need);
+                kept[o0 + at] = j;
+                if (dst_weights) dst_weights[o0 + at] = j < ldw ? w[j] : 0.f;
+            }
+            above += __popc(bg);
+            equal += __popc(be);
         }
     }
+    if (S > 1) sync_cluster(S);  // the others may still read this CTA's counts
 }
 
 // Moves the kept rows: 16 bytes per thread, K and V of a row by neighbouring
-// threads.
+// threads, four rows in flight per thread.  Bound by HBM.
 constexpr int kMoveThreads = 256;
+constexpr int kMoveRows = 4;
 
 template <int HD>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(b2p::Batch bt, PageStrides pg, int budget,
@@ -267,18 +364,28 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(b2p::Batch bt,
     b2::pdl_wait();
     const int s = blockIdx.z, g = blockIdx.y, nkv = gridDim.y, n = new_len[s];
     const int c = threadIdx.x % C, which = threadIdx.x / C % 2;
-    uint16_t* pool = which ? pg.v : pg.k;
+    uint16_t* pool = (which ? pg.v : pg.k) + g * pg.head + c * 8;
     const int mask = (1 << bt.page_shift) - 1;
-    for (int j = blockIdx.x * kRows + threadIdx.x / (2 * C); j < n; j += gridDim.x * kRows) {
-        const int dp = j >> bt.page_shift;
-        if (dp >= dst_max_pages) break;
-        const int to = dst_table[(size_t)s * dst_max_pages + dp];
-        const int from = kept[((size_t)s * nkv + g) * budget + j];
-        if (to < 0 || to >= bt.n_pages) continue;
-        const int p = bt.page(s, from);
-        if (p < 0) continue;
-        const uint4 v = *reinterpret_cast<const uint4*>(pool + p * pg.page + g * pg.head + (from & mask) * pg.row + c * 8);
-        *reinterpret_cast<uint4*>(pool + to * pg.page + g * pg.head + (j & mask) * pg.row + c * 8) = v;
+    const int* from_of = kept + ((size_t)s * nkv + g) * budget;
+    for (int j0 = blockIdx.x * kRows * kMoveRows + threadIdx.x / (2 * C); j0 < n; j0 += gridDim.x * kRows * kMoveRows) {
+        int from[kMoveRows], to[kMoveRows], page[kMoveRows];
+        uint4 v[kMoveRows];
+#pragma unroll
+        for (int i = 0; i < kMoveRows; i++) {
+            const int j = j0 + i * kRows, dp = j >> bt.page_shift;
+            from[i] = j < n ? from_of[j] : -1;
+            to[i] = j < n && dp < dst_max_pages ? dst_table[(size_t)s * dst_max_pages + dp] : -1;
+        }
+#pragma unroll
+        for (int i = 0; i < kMoveRows; i++)
+            page[i] = from[i] >= 0 && to[i] >= 0 && to[i] < bt.n_pages ? bt.page(s, from[i]) : -1;
+#pragma unroll
+        for (int i = 0; i < kMoveRows; i++)
+            if (page[i] >= 0)
+                v[i] = b2::ld_stream16(pool + page[i] * pg.page + (from[i] & mask) * pg.row);
+#pragma unroll
+        for (int i = 0; i < kMoveRows; i++)
+            if (page[i] >= 0) *reinterpret_cast<uint4*>(pool + to[i] * pg.page + ((j0 + i * kRows) & mask) * pg.row) = v[i];
     }
 }
 
@@ -322,10 +429,35 @@ extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const flo
     const b2p::Batch bt = b2p::make_batch(kv, 0);
     const PageStrides pg{kv->k_pages, kv->v_pages, kv->page_stride, kv->head_stride, kv->row_stride};
     cudaStream_t st = (cudaStream_t)s;
-    cudaError_t e = b2::launch_pdl(evict_select_kernel, dim3(nkv, kv->n_seqs), dim3(kSelThreads), 0, st, bt, weights, ldw,
-                                   nkv, budget, sink, recent, kept, dst_weights, new_len);
+    // CTAs per (sequence, kv head): as many as have 2048 slots each when the table is
+    // full, and as two per SM have room for.
+    const long long cap = (long long)kv->max_pages * kv->page_size, heads = (long long)kv->n_seqs * nkv;
+    int dev = 0, sms = 148, S = 1;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    while (S < kMaxSplit && cap > 2048ll * S && heads * S * 2 <= 2 * sms) S *= 2;
+    long long held = ((cap + 31) / 32 + S - 1) / S * 32;
+    if (held > kMaxKeys) held = kMaxKeys;
+    static std::atomic<unsigned long long> allowed{0};
+    cudaError_t e = b2p::allow_smem(evict_select_kernel, kMaxKeys * 4, allowed, dev);
+    if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_kv_evict_paged smem: %s", cudaGetErrorString(e));
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(S, nkv, kv->n_seqs);
+    cfg.blockDim = dim3(kSelThreads);
+    cfg.dynamicSmemBytes = (size_t)held * 4;
+    cfg.stream = st;
+    cudaLaunchAttribute at[2];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    at[1].id = cudaLaunchAttributeClusterDimension;
+    at[1].val.clusterDim.x = S;
+    at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = S > 1 ? 2 : 1;
+    e = cudaLaunchKernelEx(&cfg, evict_select_kernel, bt, weights, ldw, nkv, budget, sink, recent, (int)held, kept,
+                           dst_weights, new_len);
     if (e == cudaSuccess && budget > 0) {
-        const int rows = kMoveThreads / (2 * (hd / 8));
+        const int rows = kMoveThreads / (2 * (hd / 8)) * kMoveRows;
         const int want = (budget + rows - 1) / rows;
         const dim3 grid(want < 4096 ? want : 4096, nkv, kv->n_seqs);
         e = b2::launch_pdl(hd == 128 ? evict_move_kernel<128> : evict_move_kernel<64>, grid, dim3(kMoveThreads), 0, st, bt,
