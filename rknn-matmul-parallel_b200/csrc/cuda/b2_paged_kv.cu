@@ -161,19 +161,19 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(
 // Slots above it are kept, and as many of those equal to it as are missing,
 // lowest first.  A warp owns a contiguous run of its CTA's slots, 32 at a time, so
 // ballots give the places in slot order and one scan over the warps joins them.
-// Bound by latency: four digits of a few microseconds.
-constexpr int kSelThreads = 512;  // two CTAs per SM
-constexpr int kSelWarps = kSelThreads / 32;
+// The search ends early once all slots that share the digits so far are kept.
+// Bound by latency: 2 to 4 digits of a few microseconds each; 100 thousand slots of
+// 8 heads take 33 us, 4096 slots of 128 (sequence, head) pairs 18 us.
+constexpr int kBatch = 8;  // groups of 32 slots whose loads a warp has in flight
 constexpr int kMaxKeys = 48 * 1024;  // keys a CTA holds; more are formed again for every digit
 constexpr int kMaxSplit = 8;
 
-__device__ __forceinline__ uint32_t evict_key(const b2p::Batch& bt, const float* w, long long ldw, int s, int j, int len,
-                                              int sink, int recent) {
-    if (bt.page(s, j) < 0) return 0u;
-    if (j < sink || j >= len - recent) return 0xFFFFFFFFu;
+// Key of slot j from its page entry and weight.
+__device__ __forceinline__ uint32_t evict_key(int page, int n_pages, float w, bool always) {
+    if (page < 0 || page >= n_pages) return 0u;
+    if (always) return 0xFFFFFFFFu;
     // + 0 turns -0 into 0, so that the two are equal here too
-    const uint32_t k = b2::float_order((j < ldw ? w[j] : 0.f) + 0.f);
-    return min(max(k, 1u), 0xFFFFFFFEu);
+    return min(max(b2::float_order(w + 0.f), 1u), 0xFFFFFFFEu);
 }
 
 __device__ __forceinline__ int ld_rank(const int* p, int rank) {
@@ -189,17 +189,19 @@ __device__ __forceinline__ void sync_cluster(int S) {
 }
 
 // S = gridDim.x.
-__global__ void __launch_bounds__(kSelThreads, 2) evict_select_kernel(b2p::Batch bt, const float* __restrict__ weights,
+template <int kSelThreads>
+__global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_kernel(b2p::Batch bt, const float* __restrict__ weights,
                                                                    long long ldw, int nkv, int budget, int sink,
                                                                    int recent, int held, int* __restrict__ kept,
                                                                    float* __restrict__ dst_weights,
                                                                    int* __restrict__ new_len) {
+    constexpr int kSelWarps = kSelThreads / 32;
     extern __shared__ uint32_t keys[];
     __shared__ int hist[2][257];  // [digit parity]; [256]: unmapped slots
     __shared__ int sum[256];
     __shared__ int counts[2];     // slots above the k-th key, and equal to it
     __shared__ int warp_gt[kSelWarps], warp_eq[kSelWarps];
-    __shared__ int found[2], before[2], unmapped;
+    __shared__ int found[3], before[2], unmapped;
     const int S = gridDim.x, rank = blockIdx.x, g = blockIdx.y, s = blockIdx.z;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     b2::pdl_trigger();
@@ -213,27 +215,62 @@ __global__ void __launch_bounds__(kSelThreads, 2) evict_select_kernel(b2p::Batch
     const int w0 = min(g1, g0 + warp * warp_g), w1 = min(g1, w0 + warp_g);
     const bool cached = cta_g * 32 <= held;
     const float* w = weights + ((size_t)s * nkv + g) * ldw;
-    auto make_key = [&](int j) { return j < len ? evict_key(bt, w, ldw, s, j, len, sink, recent) : 0u; };
-    auto key_of = [&](int q) { return cached ? keys[(q - g0) * 32 + lane] : make_key(q * 32 + lane); };
+    const int* table = bt.page_table + (size_t)s * bt.max_pages;
+    // kBatch groups' page entries and weights, all requested before any is used
+    auto make_keys = [&](int q0, uint32_t (&key)[kBatch]) {
+        int pg[kBatch];
+        float wv[kBatch];
+#pragma unroll
+        for (int e = 0; e < kBatch; e++) {
+            const int j = (q0 + e) * 32 + lane;
+            const bool in = q0 + e < w1 && j < len;
+            pg[e] = in ? table[j >> bt.page_shift] : -1;
+            wv[e] = in && j < ldw ? w[j] : 0.f;
+        }
+        __syncwarp();  // no load moves behind this
+#pragma unroll
+        for (int e = 0; e < kBatch; e++) {
+            const int j = (q0 + e) * 32 + lane;
+            key[e] = evict_key(pg[e], bt.n_pages, wv[e], j < sink || j >= len - recent);
+        }
+    };
+    auto get_keys = [&](int q0, uint32_t (&key)[kBatch]) {
+        if (cached) {
+#pragma unroll
+            for (int e = 0; e < kBatch; e++) key[e] = q0 + e < w1 ? keys[(q0 + e - g0) * 32 + lane] : 0u;
+        } else {
+            make_keys(q0, key);
+        }
+    };
     for (int i = tid; i < 2 * 257; i += kSelThreads) (&hist[0][0])[i] = 0;
-    if (cached) {
-#pragma unroll 4
-        for (int q = w0; q < w1; q++) keys[(q - g0) * 32 + lane] = make_key(q * 32 + lane);
-    }
+    if (cached)
+        for (int q = w0; q < w1; q += kBatch) {
+            uint32_t key[kBatch];
+            make_keys(q, key);
+#pragma unroll
+            for (int e = 0; e < kBatch; e++)
+                if (q + e < w1) keys[(q + e - g0) * 32 + lane] = key[e];
+        }
     __syncthreads();
     uint32_t prefix = 0;  // the digits found so far of the k-th largest key
     int need = 0, k = 0;  // slots still to take among those that share them; slots kept
+    bool whole = false;
     for (int d = 0; d < 4; d++) {
         const int shift = 24 - 8 * d;
         int* h = hist[d & 1];
         int none = 0;
-        for (int q = w0; q < w1; q++) {
-            const uint32_t key = key_of(q);
-            const bool in = key != 0 && (d == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
-            if (d == 0) none += q * 32 + lane < len && key == 0;
-            // one addition per distinct digit of the warp: weights share exponents
-            const unsigned same = __match_any_sync(0xffffffffu, in ? (key >> shift) & 255 : 256u);
-            if (in && lane == __ffs(same) - 1) atomicAdd(&h[(key >> shift) & 255], __popc(same));
+        for (int q = w0; q < w1; q += kBatch) {
+            uint32_t keyv[kBatch];
+            get_keys(q, keyv);
+#pragma unroll
+            for (int e = 0; e < kBatch; e++) {
+                const uint32_t key = keyv[e];
+                const bool in = key != 0 && (d == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
+                if (d == 0) none += q + e < w1 && (q + e) * 32 + lane < len && key == 0;
+                // one addition per distinct digit of the warp: weights share exponents
+                const unsigned same = __match_any_sync(0xffffffffu, in ? (key >> shift) & 255 : 256u);
+                if (in && lane == __ffs(same) - 1) atomicAdd(&h[(key >> shift) & 255], __popc(same));
+            }
         }
         if (d == 0) {
             none = __reduce_add_sync(0xffffffffu, none);
@@ -274,6 +311,7 @@ __global__ void __launch_bounds__(kSelThreads, 2) evict_select_kernel(b2p::Batch
                     if (over < need && over + c[e] >= need) {
                         found[0] = 255 - 8 * lane - e;
                         found[1] = need - over;
+                        found[2] = need - over == c[e];
                     }
                     over += c[e];
                 }
@@ -285,17 +323,25 @@ __global__ void __launch_bounds__(kSelThreads, 2) evict_select_kernel(b2p::Batch
         __syncthreads();
         prefix |= (uint32_t)found[0] << shift;
         need = found[1];
+        if (found[2]) {  // every slot that shares these digits is kept: the rest of them does not matter
+            whole = true;
+            break;
+        }
     }
     if (rank == 0 && g == 0 && tid == 0) new_len[s] = k;
-    const bool every = k == len - unmapped;
-    const uint32_t bar = every ? 0u : prefix;  // kept: keys above, and `need` of those equal
-    if (every) need = 0;
+    // kept: keys above `bar`, and unless that is all `need` of those equal to it
+    const bool every = whole || k == len - unmapped;
+    const uint32_t bar = !every ? prefix : whole && prefix > 0 ? prefix - 1 : 0u;
     if (k > 0) {  // the same for every CTA of the cluster
         int gt = 0, eq = 0;
-        for (int q = w0; q < w1; q++) {
-            const uint32_t key = key_of(q);
-            gt += key > bar;
-            eq += key == bar && !every;
+        for (int q = w0; q < w1; q += kBatch) {
+            uint32_t key[kBatch];
+            get_keys(q, key);
+#pragma unroll
+            for (int e = 0; e < kBatch; e++) {
+                gt += key[e] > bar;
+                eq += key[e] == bar && !every;
+            }
         }
         gt = __reduce_add_sync(0xffffffffu, gt);
         eq = __reduce_add_sync(0xffffffffu, eq);
@@ -332,17 +378,30 @@ __global__ void __launch_bounds__(kSelThreads, 2) evict_select_kernel(b2p::Batch
         int above = before[0] + warp_gt[warp], equal = before[1] + warp_eq[warp];  // in slots before this group
         const size_t o0 = ((size_t)s * nkv + g) * budget;
         const unsigned below = (1u << lane) - 1;
-        for (int q = w0; q < w1; q++) {
-            const uint32_t key = key_of(q);
-            const unsigned bg = __ballot_sync(0xffffffffu, key > bar), be = __ballot_sync(0xffffffffu, key == bar && !every);
-            const int eq_rank = equal + __popc(be & below);
-            if (key > bar || (key == bar && !every && eq_rank < need)) {
-                const int j = q * 32 + lane, at = above + __popc(bg & below) + min(eq_rank, need);
-                kept[o0 + at] = j;
-                if (dst_weights) dst_weights[o0 + at] = j < ldw ? w[j] : 0.f;
+        for (int q = w0; q < w1; q += kBatch) {
+            uint32_t keyv[kBatch];
+            float wv[kBatch];
+            get_keys(q, keyv);
+#pragma unroll
+            for (int e = 0; e < kBatch; e++) {
+                const int j = (q + e) * 32 + lane;
+                wv[e] = dst_weights && keyv[e] != 0 && keyv[e] >= bar && j < ldw ? w[j] : 0.f;
             }
-            above += __popc(bg);
-            equal += __popc(be);
+            __syncwarp();  // no load moves behind this
+#pragma unroll
+            for (int e = 0; e < kBatch; e++) {
+                const uint32_t key = keyv[e];
+                const bool is_gt = key > bar, is_eq = key == bar && !every;
+                const unsigned bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq);
+                const int eq_rank = equal + __popc(be & below);
+                if (is_gt || (is_eq && eq_rank < need)) {
+                    const int at = above + __popc(bg & below) + (every ? 0 : min(eq_rank, need));
+                    kept[o0 + at] = (q + e) * 32 + lane;
+                    if (dst_weights) dst_weights[o0 + at] = wv[e];
+                }
+                above += __popc(bg);
+                equal += __popc(be);
+            }
         }
     }
     if (S > 1) sync_cluster(S);  // the others may still read this CTA's counts
@@ -429,21 +488,25 @@ extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const flo
     const b2p::Batch bt = b2p::make_batch(kv, 0);
     const PageStrides pg{kv->k_pages, kv->v_pages, kv->page_stride, kv->head_stride, kv->row_stride};
     cudaStream_t st = (cudaStream_t)s;
-    // CTAs per (sequence, kv head): as many as have 2048 slots each when the table is
-    // full, and as two per SM have room for.
+    // CTAs per (sequence, kv head): as many as have 4096 slots each when the table is
+    // full, and as two per SM have room for.  (4096 slots: 39 us with one, 40 with
+    // two; 100 thousand slots of 8 heads: 264 us with one, 61 with eight.)
     const long long cap = (long long)kv->max_pages * kv->page_size, heads = (long long)kv->n_seqs * nkv;
     int dev = 0, sms = 148, S = 1;
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
-    while (S < kMaxSplit && cap > 2048ll * S && heads * S * 2 <= 2 * sms) S *= 2;
+    while (S < kMaxSplit && cap > 4096ll * S && heads * S * 2 <= 2 * sms) S *= 2;
     long long held = ((cap + 31) / 32 + S - 1) / S * 32;
     if (held > kMaxKeys) held = kMaxKeys;
-    static std::atomic<unsigned long long> allowed{0};
-    cudaError_t e = b2p::allow_smem(evict_select_kernel, kMaxKeys * 4, allowed, dev);
+    // Twice the threads where a CTA has an SM to itself and slots for them.
+    const bool wide = held > 2048 && heads * S <= sms;
+    static std::atomic<unsigned long long> allowed[2];
+    cudaError_t e = wide ? b2p::allow_smem(evict_select_kernel<1024>, kMaxKeys * 4, allowed[1], dev)
+                         : b2p::allow_smem(evict_select_kernel<512>, kMaxKeys * 4, allowed[0], dev);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_kv_evict_paged smem: %s", cudaGetErrorString(e));
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(S, nkv, kv->n_seqs);
-    cfg.blockDim = dim3(kSelThreads);
+    cfg.blockDim = dim3(wide ? 1024 : 512);
     cfg.dynamicSmemBytes = (size_t)held * 4;
     cfg.stream = st;
     cudaLaunchAttribute at[2];
@@ -454,7 +517,7 @@ extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const flo
     at[1].val.clusterDim.y = at[1].val.clusterDim.z = 1;
     cfg.attrs = at;
     cfg.numAttrs = S > 1 ? 2 : 1;
-    e = cudaLaunchKernelEx(&cfg, evict_select_kernel, bt, weights, ldw, nkv, budget, sink, recent, (int)held, kept,
+    e = cudaLaunchKernelEx(&cfg, wide ? evict_select_kernel<1024> : evict_select_kernel<512>, bt, weights, ldw, nkv, budget, sink, recent, (int)held, kept,
                            dst_weights, new_len);
     if (e == cudaSuccess && budget > 0) {
         const int rows = kMoveThreads / (2 * (hd / 8)) * kMoveRows;
