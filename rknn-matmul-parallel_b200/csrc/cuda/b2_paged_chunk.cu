@@ -58,7 +58,7 @@ struct Smem {
     alignas(1024) unsigned char ring[Cfg<HD>::kStages][Cfg<HD>::kTile];
     uint64_t full[Cfg<HD>::kStages], empty[Cfg<HD>::kStages];
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_ready[2], o_done[2], o_free[2], drain;
+    uint64_t s_full[2], p_ready[2][2], o_done[2], o_free[2], drain;  // p_ready: [tile][half of the slots]
     uint32_t tmem;
     int failed;
     int mapped[8];  // bit w of entry (block count % 8): slots 16 w .. 16 w + 15 are mapped
@@ -137,7 +137,8 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(&sm.drain, 1);
         for (int t = 0; t < 2; t++) {
             mbar_init(&sm.s_full[t], 1);
-            mbar_init(&sm.p_ready[t], 128);
+            mbar_init(&sm.p_ready[t][0], 128);
+            mbar_init(&sm.p_ready[t][1], 128);
             mbar_init(&sm.o_done[t], 1);
             mbar_init(&sm.o_free[t], 128);
         }
@@ -227,71 +228,74 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (mbar_try_wait(&sm.q_full, (seg - 1) & 1)) break;
         } else if (warp == 9) {
             // ── tensor cores ──
-            if (lane == 0) {
-                constexpr uint32_t id_s = idesc_f16(128, 128, false), id_o = idesc_f16(128, HD, true);
-                int k = 0, seg = 0;
-                int np[2] = {0, 0};  // P tiles consumed
-                int no[2] = {0, 0};  // segments whose O the tile has summed
-                auto mma_s = [&](int t, int st) {
-                    const uint32_t a = smem_u32(sm.q[t]), b = smem_u32(sm.ring[st]);
+            constexpr uint32_t id_s = idesc_f16(128, 128, false), id_o = idesc_f16(128, HD, true);
+            const uint32_t lead = lane == 0, tm = (uint32_t)uniform((int)tmem);
+            int k = 0, seg = 0;
+            int np0 = 0, np1 = 0;  // P tiles consumed of either tile
+            int no0 = 0, no1 = 0;  // segments whose O the tile has summed
+            auto wait = [&](uint64_t* bar, int parity) {
+                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+                tc_fence_after();
+                return ok;
+            };
+            // descriptors of the first element; later ones add to the 14-bit address field
+            const uint64_t dq = sw128_desc(smem_u32(sm.q[0]), 16), dk = sw128_desc(smem_u32(sm.ring[0]), 16),
+                           dv = sw128_desc(smem_u32(sm.ring[0]), 16384);
+            auto mma_s = [&](int t, int st) {
+                const uint64_t a = dq + t * (C::kTile >> 4), b = dk + st * (C::kTile >> 4);
 #pragma unroll
-                    for (int i = 0; i < HD / 16; i++) {
-                        const uint32_t o = (i >> 2) * 16384 + (i & 3) * 32;
-                        umma_ss(tmem + C::kS + 128 * t, sw128_desc(a + o, 16), sw128_desc(b + o, 16), id_s, i != 0);
-                    }
-                    umma_commit(&sm.s_full[t]);
-                };
-                for (int x = x0; x < x1 && ok;) {
-                    const Seg g = find_seg<HD>(p, sm, items, x, x1);
-                    x += g.b1 - g.b0;
-                    const int e = g.end();
-                    if (e <= g.b0) continue;
-                    ok = mbar_wait(&sm.q_full, seg & 1, failed);
-                    seg++;
-                    if (!ok) break;
-                    ok = mbar_wait(&sm.full[k % C::kStages], (k / C::kStages) & 1, failed);
-                    if (!ok) break;
-                    tc_fence_after();
-                    for (int t = 0; t < 2; t++)
-                        if (g.b0 < g.live[t]) mma_s(t, k % C::kStages);
-                    umma_commit(&sm.empty[k % C::kStages]);
-                    if (g.b0 + 1 == e) umma_commit(&sm.q_empty);
-                    for (int b = g.b0; b < e && ok; b++, k += 2) {
-                        const int sv = (k + 1) % C::kStages, sk = (k + 2) % C::kStages;
-                        bool have_k = false;
-                        ok = mbar_wait(&sm.full[sv], ((k + 1) / C::kStages) & 1, failed);
-                        for (int t = 0; t < 2 && ok; t++) {
-                            if (b < g.live[t]) {
-                                // the segment before's O has been read
-                                if (b == g.b0 && no[t]++) ok = mbar_wait(&sm.o_free[t], no[t] & 1, failed);
-                                ok = ok && mbar_wait(&sm.p_ready[t], np[t] & 1, failed);
-                                np[t]++;
-                                if (!ok) break;
-                                tc_fence_after();
+                for (int i = 0; i < HD / 16; i++) {
+                    const uint32_t o = ((i >> 2) * 16384 + (i & 3) * 32) >> 4;
+                    umma_ss(tm + C::kS + 128 * t, a + o, b + o, id_s, i != 0, lead);
+                }
+                umma_commit(&sm.s_full[t], lead);
+            };
+            // O_t += P_t V for one block; first: the segment's first, once the segment before's O has been read
+            auto mma_o = [&](int t, int st, bool first, int& np, int& no) {
+                if (first && no++ && !wait(&sm.o_free[t], no & 1)) return false;
+                const uint64_t v = dv + st * (C::kTile >> 4);
 #pragma unroll
-                                for (int i = 0; i < kBlk / 16; i++)
-                                    umma_ts(tmem + C::kO + HD * t, tmem + C::kS + 128 * t + 8 * i,
-                                            sw128_desc(smem_u32(sm.ring[sv]) + 2048 * i, 16384), id_o, b > g.b0 || i > 0);
-                                umma_commit(&sm.o_done[t]);
-                            }
-                            if (b + 1 < g.live[t]) {
-                                if (!have_k) ok = mbar_wait(&sm.full[sk], ((k + 2) / C::kStages) & 1, failed);
-                                if (!ok) break;
-                                have_k = true;
-                                tc_fence_after();
-                                mma_s(t, sk);
-                            }
-                        }
-                        umma_commit(&sm.empty[sv]);
-                        if (b + 1 < e) umma_commit(&sm.empty[sk]);
-                        if (b + 2 == e) umma_commit(&sm.q_empty);
-                    }
+                for (int h = 0; h < 2; h++) {
+                    if (!wait(&sm.p_ready[t][h], np & 1)) return false;
+#pragma unroll
+                    for (int i = 4 * h; i < 4 * h + 4; i++)
+                        umma_ts(tm + C::kO + HD * t, tm + C::kS + 128 * t + 8 * i, v + i * (2048 >> 4), id_o,
+                                !first || i > 0, lead);
                 }
-                if (!ok) {  // nothing of the tensor cores may be left running
-                    umma_commit(&sm.drain);
-                    for (long long it = 0; it <= kWaitLimit; it++)
-                        if (mbar_try_wait(&sm.drain, 0)) break;
+                np++;
+                umma_commit(&sm.o_done[t], lead);
+                return true;
+            };
+            for (int x = x0; x < x1 && ok;) {
+                const Seg g = find_seg<HD>(p, sm, items, x, x1);
+                x = uniform(x + g.b1 - g.b0);
+                const int b0 = uniform(g.b0), live0 = uniform(g.live[0]), live1 = uniform(g.live[1]);
+                const int e = max(live0, live1);
+                if (e <= b0) continue;
+                if (!wait(&sm.q_full, seg & 1)) break;
+                seg++;
+                if (!wait(&sm.full[k % C::kStages], (k / C::kStages) & 1)) break;
+                if (b0 < live0) mma_s(0, k % C::kStages);
+                if (b0 < live1) mma_s(1, k % C::kStages);
+                umma_commit(&sm.empty[k % C::kStages], lead);
+                if (b0 + 1 == e) umma_commit(&sm.q_empty, lead);
+                for (int b = b0; b < e; b++, k += 2) {
+                    const int sv = (k + 1) % C::kStages, sk = (k + 2) % C::kStages;
+                    if (!wait(&sm.full[sv], ((k + 1) / C::kStages) & 1)) break;
+                    if (b < live0 && !mma_o(0, sv, b == b0, np0, no0)) break;
+                    if (b + 1 < e && !wait(&sm.full[sk], ((k + 2) / C::kStages) & 1)) break;
+                    if (b + 1 < live0) mma_s(0, sk);
+                    if (b < live1 && !mma_o(1, sv, b == b0, np1, no1)) break;
+                    umma_commit(&sm.empty[sv], lead);
+                    if (b + 1 < live1) mma_s(1, sk);
+                    if (b + 1 < e) umma_commit(&sm.empty[sk], lead);
+                    if (b + 2 == e) umma_commit(&sm.q_empty, lead);
                 }
+            }
+            if (!ok) {  // nothing of the tensor cores may be left running
+                umma_commit(&sm.drain, lead);
+                for (long long it = 0; it <= kWaitLimit; it++)
+                    if (mbar_try_wait(&sm.drain, 0)) break;
             }
         }
     } else {
@@ -310,7 +314,8 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int tok = r / p.a.G, first = g.b0;
             const bool live = tok < g.tok[t];
             const int lim = live ? min(g.sq.len - 1, g.sq.base + g.i0 + t * p.T + tok) : -1;
-            float m = -INFINITY, l0 = 0.f, l1 = 0.f;
+            float m = -INFINITY;
+            uint64_t l2[2] = {pack_f2(0.f, 0.f), pack_f2(0.f, 0.f)};  // sums, two slots at a time
             for (int b = first; b < g.live[t]; b++, ns++) {
                 const int j0 = b * kBlk, n = nblk + (b - first);
                 ok = mbar_wait(&sm.s_full[t], ns & 1, failed);
@@ -319,19 +324,30 @@ __global__ void __launch_bounds__(kThreads, 1)
                 uint32_t sv[128];
                 tmem_ld32<0>(ts, sv);
                 tmem_ld32<32>(ts + 32, sv);
+                tmem_wait_ld();
                 tmem_ld32<64>(ts + 64, sv);
                 tmem_ld32<96>(ts + 96, sv);
-                tmem_wait_ld();
                 const int bits = *(volatile int*)&sm.mapped[n & 7];
-                if (bits != 0xff || __any_sync(0xffffffffu, live && lim < j0 + kBlk - 1)) {
+                const bool masked = bits != 0xff || __any_sync(0xffffffffu, live && lim < j0 + kBlk - 1);
+                auto mask = [&](int c0) {
 #pragma unroll
-                    for (int c = 0; c < 128; c++)
+                    for (int c = c0; c < c0 + 64; c++)
                         if (j0 + c > lim || !(bits >> (c >> 4) & 1)) sv[c] = 0xff800000u;  // -inf
-                }
-                float mx = -INFINITY;
+                };
+                float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto top = [&](int c0) {
 #pragma unroll
-                for (int c = 0; c < 128; c++) mx = fmaxf(mx, __uint_as_float(sv[c]));
-                mx *= scale;
+                    for (int c = c0; c < c0 + 64; c += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            mx4[e] = max3(mx4[e], __uint_as_float(sv[c + 2 * e]), __uint_as_float(sv[c + 2 * e + 1]));
+                };
+                if (masked) mask(0);
+                top(0);
+                tmem_wait_ld();
+                if (masked) mask(64);
+                top(64);
+                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
                 // a new reference for rows that outgrew theirs
                 const bool grow = live && (mx > m + kLazy || (m == -INFINITY && mx > m));
                 if (b == first) {
@@ -350,23 +366,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int i = 0; i < 32; i++) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
                         tmem_st32(to + c, ov);
                     }
-                    l0 *= f;
-                    l1 *= f;
+                    l2[0] = fma_f2(l2[0], pack_f2(f, f), pack_f2(0.f, 0.f));
+                    l2[1] = fma_f2(l2[1], pack_f2(f, f), pack_f2(0.f, 0.f));
                     if (grow) m = mx;
-                }
-                const float bias = m == -INFINITY ? 0.f : kUp - m;
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const float a = ex2(fmaf(__uint_as_float(sv[64 * h + 2 * i]), scale, bias));
-                        const float c = ex2(fmaf(__uint_as_float(sv[64 * h + 2 * i + 1]), scale, bias));
-                        l0 += a;
-                        l1 += c;
-                        pk[i] = pack_h2(a, c);
-                    }
-                    tmem_st32(ts + 32 * h, pk);
                 }
                 if (g.sq.len < j0 + kBlk) {
                     // V rows past kv_len may hold anything: zero them (their P is zero, and 0 x inf is not)
@@ -380,9 +382,26 @@ __global__ void __launch_bounds__(kThreads, 1)
                     }
                     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
-                tmem_wait_st();
-                tc_fence_before();
-                mbar_arrive(&sm.p_ready[t]);
+                const float bias = m == -INFINITY ? 0.f : kUp - m;
+                const uint64_t scale2 = pack_f2(scale, scale), bias2 = pack_f2(bias, bias);
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    uint32_t pk[32];
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const int c = 64 * h + 2 * i;
+                        float x, y;
+                        unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, bias2), x, y);
+                        x = ex2(x);
+                        y = ex2(y);
+                        l2[i & 1] = add_f2(l2[i & 1], pack_f2(x, y));
+                        pk[i] = pack_h2(x, y);
+                    }
+                    tmem_st32(ts + 32 * h, pk);
+                    tmem_wait_st();
+                    tc_fence_before();
+                    mbar_arrive(&sm.p_ready[t][h]);
+                }
             }
             if (!ok) break;
             nblk += max(0, g.end() - first);
@@ -393,7 +412,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
                 tc_fence_after();
             }
-            const float l = l0 + l1;
+            float la, lb;
+            unpack_f2(add_f2(l2[0], l2[1]), la, lb);
+            const float l = la + lb;
             const size_t row = (size_t)(g.sq.row0 + g.i0 + t * p.T + tok);
             const int h = g.g * p.a.G + r % p.a.G;
             float* part = p.a.long_part + (size_t)(2 * blockIdx.x + (g.b0 == 0 ? 1 : 0)) * long_piece_floats(HD);

@@ -302,39 +302,45 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         }
     } else if (warp == 9) {
         // ── tensor cores ──
-        if (lane == 0) {
-            constexpr uint32_t id = idesc_f16(128, kRowsT, false);
-            int nu = 0, nq = 0;
-            for (int x = blockIdx.x / S; x < W && ok; x += step) {
-                const Unit u = find_unit(p, sm.pre, T, x);
-                if (u.first + rank >= u.tiles) continue;
-                const int kb = nu & 1;
-                ok = mbar_wait(&sm.k_full[kb], (nu / 2) & 1, failed);
-                nu++;
-                for (int i = u.first + rank; i < u.tiles && ok; i += S, nq++) {
-                    const int b = nq & 1;
-                    ok = mbar_wait(&sm.q_full[b], (nq / 2) & 1, failed);
-                    for (int t = 0; t < 2 && ok; t++) {
-                        if (nq >= 2) ok = mbar_wait(&sm.s_free[t][b], (nq / 2 - 1) & 1, failed);
-                        if (!ok) break;
-                        tc_fence_after();
-                        const uint32_t ka = smem_u32(sm.k[kb][t]), qa = smem_u32(sm.q[b]);
+        constexpr uint32_t id = idesc_f16(128, kRowsT, false);
+        const uint32_t lead = lane == 0, tm = (uint32_t)uniform((int)tmem);
+        auto wait = [&](uint64_t* bar, int parity) {
+            ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+            tc_fence_after();
+            return ok;
+        };
+        // descriptors of the first element; later ones add to the 14-bit address field
+        const uint64_t dk = sw128_desc(smem_u32(sm.k[0][0]), 16), dq = sw128_desc(smem_u32(sm.q[0]), 16);
+        int nu = 0, nq = 0;
+        for (int x = blockIdx.x / S; x < W && ok; x += step) {
+            const Unit u = find_unit(p, sm.pre, T, x);
+            const int first = uniform(u.first) + rank, tiles = uniform(u.tiles);
+            if (first >= tiles) continue;
+            const int kb = nu & 1;
+            if (!wait(&sm.k_full[kb], (nu / 2) & 1)) break;
+            nu++;
+            for (int i = first; i < tiles && ok; i += S, nq++) {
+                const int b = nq & 1;
+                if (!wait(&sm.q_full[b], (nq / 2) & 1)) break;
 #pragma unroll
-                        for (int e = 0; e < HD / 16; e++) {
-                            const uint32_t o = (e >> 2) * 16384 + (e & 3) * 32;
-                            umma_ss(tmem + (2 * t + b) * 128, sw128_desc(ka + o, 16), sw128_desc(qa + o, 16), id, e != 0);
-                        }
-                        umma_commit(&sm.s_full[t][b]);
+                for (int t = 0; t < 2; t++) {
+                    if (nq >= 2 && !wait(&sm.s_free[t][b], (nq / 2 - 1) & 1)) break;
+                    const uint64_t a = dk + (2 * kb + t) * (Sm::kTile >> 4), q = dq + b * (Sm::kTile >> 4);
+#pragma unroll
+                    for (int e = 0; e < HD / 16; e++) {
+                        const uint32_t o = ((e >> 2) * 16384 + (e & 3) * 32) >> 4;
+                        umma_ss(tm + (2 * t + b) * 128, a + o, q + o, id, e != 0, lead);
                     }
-                    umma_commit(&sm.q_empty[b]);
+                    umma_commit(&sm.s_full[t][b], lead);
                 }
-                umma_commit(&sm.k_empty[kb]);
+                umma_commit(&sm.q_empty[b], lead);
             }
-            if (!ok) {  // nothing of the tensor cores may be left running
-                umma_commit(&sm.drain);
-                for (long long it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.drain, 0)) break;
-            }
+            umma_commit(&sm.k_empty[kb], lead);
+        }
+        if (!ok) {  // nothing of the tensor cores may be left running
+            umma_commit(&sm.drain, lead);
+            for (long long it = 0; it <= kWaitLimit; it++)
+                if (mbar_try_wait(&sm.drain, 0)) break;
         }
     } else {
         // ── exponentials of K tile t: thread = slot ──
