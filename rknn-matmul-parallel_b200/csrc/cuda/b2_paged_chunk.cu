@@ -10,8 +10,10 @@
 //               table into a ring of shared-memory stages; unmapped pages and
 //               pages past kv_len are fetched from outside the tensor, which
 //               fills zeros;
-//   warp 9      one thread issues tcgen05.mma: S_t = Q_t K^T (128 x 128, FP32 in
-//               tensor memory) and O_t += P_t V with P_t read from tensor memory;
+//   warps 9, 10 the tensor cores for tile 0 and tile 1: S_t = Q_t K^T (128 x 128,
+//               FP32 in tensor memory) and O_t += P_t V with P_t read from tensor
+//               memory.  One warp for both spent 5000 cycles a block on waiting
+//               and issuing in turn, where the products take 2048;
 //   warps 0-3, 4-7   the softmax of tile 0 and of tile 1, one row per thread:
 //               maximum, exponentials, sum, P_t as FP16 over S_t's columns.
 //
@@ -26,19 +28,21 @@
 // The work of the call is one line of blocks, cut into equal stretches for the
 // CTAs; pairs that a cut divides leave pieces (maximum, sum, unnormalised O) in
 // the workspace, which the kernel launched behind this one merges.
+#include <type_traits>
+
 #include "b2_tc.cuh"
 
 namespace {
 
 using namespace b2p;
 
-constexpr int kBlk = 128;
-// Three warpgroups; the third's last two warps only fill it up.  Launched with 168
+constexpr int kBlk = 64;
+// Three warpgroups; the third's last warp only fills it up.  Launched with 168
 // registers a thread; the softmax warpgroups, which hold a row of 128 scores, go to
 // 208 and the third gives them up: 208 + 208 + 88 = 3 x 168.
 constexpr int kThreads = 384;
 constexpr int kMaxItems = 2048;  // entries of the line's prefix in shared memory
-constexpr int kMinBlocks = 2;    // shortest stretch of a CTA
+constexpr int kMinBlocks = 4;    // shortest stretch of a CTA
 constexpr float kLazy = 8.f;     // growth of the maximum (log2) that O tolerates without rescaling
 // Weights are 2^(s - m + kUp) <= 2^(kLazy + kUp) = 2^15 in FP16; kUp keeps small
 // ones out of FP16's subnormals down to 2^-21 of the reference.
@@ -47,21 +51,26 @@ constexpr float kUp = 7.f;
 template <int HD>
 struct Cfg {
     static constexpr int kHalves = HD / 64;
-    static constexpr int kTile = 128 * HD * 2;  // one Q tile, K block or V block, bytes
-    static constexpr int kStages = HD == 128 ? 4 : 8;
-    static constexpr uint32_t kS = 0, kO = 256;  // tensor-memory columns: S_t at 128 t, O_t at 256 + HD t
+    static constexpr int kQTile = 128 * HD * 2;  // bytes
+    static constexpr int kTile = kBlk * HD * 2;  // K block or V block, bytes
+    static constexpr int kStages = HD == 128 ? 4 : 8;  // of a K block and its V block
+    static constexpr int kQHalf = 128 * 128, kHalf = kBlk * 128;  // 64 dims of a Q tile, of a block
+    // tensor-memory columns: buffer i of S_t at 128 t + 64 i (P_t over its first half), O_t at 256 + HD t
+    static constexpr uint32_t kS = 0, kO = 256;
 };
 
 template <int HD>
 struct Smem {
-    alignas(1024) unsigned char q[2][Cfg<HD>::kTile];
-    alignas(1024) unsigned char ring[Cfg<HD>::kStages][Cfg<HD>::kTile];
+    alignas(1024) unsigned char q[2][Cfg<HD>::kQTile];
+    alignas(1024) unsigned char ring[Cfg<HD>::kStages][2][Cfg<HD>::kTile];  // [stage][K, V]
     uint64_t full[Cfg<HD>::kStages], empty[Cfg<HD>::kStages];
     uint64_t q_full, q_empty;
-    uint64_t s_full[2], p_ready[2][2], o_done[2], o_free[2], drain;  // p_ready: [tile][half of the slots]
+    // [tile][buffer of S and P]; o_done too: two products may be under way, and a wait tells two phases apart
+    uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];
+    uint64_t o_free[2], drain[2];
     uint32_t tmem;
     int failed;
-    int mapped[8];  // bit w of entry (block count % 8): slots 16 w .. 16 w + 15 are mapped
+    int mapped[16];  // bit w of entry (block count % 16): slots 16 w .. 16 w + 15 are mapped
     int pre_seq[B2_PAGED_MAX_SEQS + 1];
     int pre[kMaxItems + 1];
 };
@@ -69,11 +78,14 @@ struct Smem {
 // A stretch's part of one tile pair: blocks [b0, b1) of its nb.
 struct Seg {
     int s, g, i0;
-    int tok[2];   // tokens of each tile
-    int live[2];  // end of the stretch's blocks that some row of the tile sees
+    int tok0, tok1;    // tokens of each tile
+    int live0, live1;  // end of the stretch's blocks that some row of the tile sees
     int b0, b1, nb, x0;
     Seq sq;
-    __device__ __forceinline__ int end() const { return max(live[0], live[1]); }
+    __device__ __forceinline__ int end() const { return max(live0, live1); }
+    // (selected, not indexed: an indexed member lives in local memory, a load in every block)
+    __device__ __forceinline__ int tok(int t) const { return t ? tok1 : tok0; }
+    __device__ __forceinline__ int live(int t) const { return t ? live1 : live0; }
 };
 
 struct LongParams {
@@ -108,12 +120,10 @@ __device__ __forceinline__ Seg find_seg(const LongParams& p, const Smem<HD>& sm,
     r.g = item % p.a.nkv;
     r.i0 = (first + item / p.a.nkv) * 2 * p.T;
     const int rest = min(r.sq.Q, p.a.max_q) - r.i0;
-#pragma unroll
-    for (int t = 0; t < 2; t++) {
-        r.tok[t] = max(0, min(p.T, rest - t * p.T));
-        const int end = r.tok[t] ? min(r.sq.len, max(0, r.sq.base + r.i0 + t * p.T + r.tok[t])) : 0;
-        r.live[t] = min(r.b1, cdiv(end, kBlk));
-    }
+    r.tok0 = min(p.T, rest);
+    r.tok1 = max(0, min(p.T, rest - p.T));
+    r.live0 = min(r.b1, cdiv(min(r.sq.len, max(0, r.sq.base + r.i0 + r.tok0)), kBlk));
+    r.live1 = r.tok1 ? min(r.b1, cdiv(min(r.sq.len, max(0, r.sq.base + r.i0 + p.T + r.tok1)), kBlk)) : 0;
     return r;
 }
 
@@ -130,17 +140,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kStages; i++) {
             mbar_init(&sm.full[i], 1);
-            mbar_init(&sm.empty[i], 1);
+            mbar_init(&sm.empty[i], 2);
         }
         mbar_init(&sm.q_full, 1);
-        mbar_init(&sm.q_empty, 1);
-        mbar_init(&sm.drain, 1);
+        mbar_init(&sm.q_empty, 2);
         for (int t = 0; t < 2; t++) {
-            mbar_init(&sm.s_full[t], 1);
-            mbar_init(&sm.p_ready[t][0], 128);
-            mbar_init(&sm.p_ready[t][1], 128);
-            mbar_init(&sm.o_done[t], 1);
-            mbar_init(&sm.o_free[t], 128);
+            mbar_init(&sm.drain[t], 1);
+            for (int i = 0; i < 2; i++) {
+                mbar_init(&sm.s_full[t][i], 1);
+                mbar_init(&sm.p_ready[t][i], 4);
+                mbar_init(&sm.o_done[t][i], 1);
+            }
+            mbar_init(&sm.o_free[t], 4);
         }
         sm.failed = 0;
         mbar_init_fence();
@@ -175,127 +186,136 @@ __global__ void __launch_bounds__(kThreads, 1)
         asm volatile("setmaxnreg.dec.sync.aligned.u32 88;" ::: "memory");
         if (warp == 8) {
             // ── producer ──
+            // Lanes copy the boxes of a block: K's, then V's, a box holding every half of the head's dims
+            // where a page has all rows of the block.
             const int page_rows = 1 << bt.page_shift, box_rows = min(page_rows, kBlk), boxes = kBlk / box_rows;
-            const int box = lane / C::kHalves, half = lane % C::kHalves;
-            int k = 0, n = 0, seg = 0;  // ring entries, blocks, segments with work
+            const int halves = boxes == 1 ? 1 : C::kHalves, per_kv = boxes * halves;
+            const int is_v = lane >= per_kv, box = (lane - is_v * per_kv) / halves, half = lane % halves;
+            const CUtensorMap* map = is_v ? &tv : &tk;
+            unsigned char* to = sm.ring[0][is_v] + half * C::kHalf + box * box_rows * 128;
+            int n = 0, seg = 0;  // blocks, segments with work
             for (int x = x0; x < x1 && ok;) {
                 const Seg g = find_seg<HD>(p, sm, items, x, x1);
-                x += g.b1 - g.b0;
-                if (g.end() <= g.b0) continue;
-                if (seg && !mbar_wait(&sm.q_empty, (seg - 1) & 1, failed)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
+                x = uniform(x + g.b1 - g.b0);
+                const int b0 = uniform(g.b0), e = uniform(g.end());
+                if (e <= b0) continue;
+                // page ids of the next 32 boxes, one per lane, asked for before they are needed
+                int ids_from = b0, id = -1, next = -1;
+                auto load_ids = [&](int from) {
+                    const int j = from * kBlk + lane * box_rows;
+                    return j < g.sq.len && from + lane / boxes < e ? bt.page(g.s, j) : -1;
+                };
+                id = load_ids(b0);
+                next = load_ids(b0 + 32 / boxes);
+                if (seg) ok = warp_wait(&sm.q_empty, (seg - 1) & 1, failed);
                 if (!ok) break;
-                const int tiles = g.tok[1] ? 2 : 1, rows = p.T * p.a.G;
+                const int tiles = g.tok1 ? 2 : 1, rows = p.T * p.a.G;
                 if (lane == 0) mbar_expect_tx(&sm.q_full, tiles * rows * HD * 2);
                 __syncwarp();
                 if (lane < tiles * C::kHalves) {
-                    const int t = lane / C::kHalves;
+                    const int t = lane / C::kHalves, h = lane % C::kHalves;
                     // (64 dims, q heads of the group, tokens, halves, kv heads): rows land as token * G + head
-                    tma_load_5d(sm.q[t] + half * 16384, &tq, 0, 0, g.sq.row0 + g.i0 + t * p.T, half, g.g, &sm.q_full);
+                    tma_load_5d(sm.q[t] + h * C::kQHalf, &tq, 0, 0, g.sq.row0 + g.i0 + t * p.T, h, g.g, &sm.q_full);
                 }
                 seg++;
-                for (int b = g.b0; b < g.end() && ok; b++, n++) {
-                    const int j = b * kBlk + box * box_rows;
-                    const int page = box < boxes && j < g.sq.len ? bt.page(g.s, j) : -1;
-                    const unsigned have = __ballot_sync(0xffffffffu, page >= 0);
-#pragma unroll
-                    for (int kv = 0; kv < 2; kv++, k++) {
-                        const int st = k % C::kStages;
-                        if (k >= C::kStages && !mbar_wait(&sm.empty[st], (k / C::kStages - 1) & 1, failed)) ok = false;
-                        ok = __all_sync(0xffffffffu, ok);
-                        if (!ok) break;
-                        if (lane == 0) {
-                            if (kv == 0) {
-                                int bits = 0;
-                                for (int w = 0; w < 8; w++) bits |= (have >> (w * 16 / box_rows * C::kHalves) & 1) << w;
-                                sm.mapped[n & 7] = bits;
-                            }
-                            mbar_expect_tx(&sm.full[st], C::kTile);
-                        }
-                        __syncwarp();
-                        if (box < boxes)
-                            tma_load_5d(sm.ring[st] + half * 16384 + box * box_rows * 128, kv ? &tv : &tk, 0, j & (page_rows - 1),
-                                        half, g.g, page >= 0 ? page : bt.n_pages, &sm.full[st]);
+                for (int b = b0; b < e; b++, n++) {
+                    if ((b - ids_from) * boxes == 32) {
+                        ids_from = b;
+                        id = next;
+                        next = load_ids(b + 32 / boxes);
                     }
+                    const int at = (b - ids_from) * boxes, st = n % C::kStages;
+                    const unsigned have = __ballot_sync(0xffffffffu, id >= 0) >> at;
+                    const int page = __shfl_sync(0xffffffffu, id, (at + box) & 31);
+                    if (n >= C::kStages) ok = warp_wait(&sm.empty[st], (n / C::kStages - 1) & 1, failed);
+                    if (!ok) break;
+                    if (lane == 0) {
+                        int bits = 0;
+                        for (int w = 0; w < kBlk / 16; w++) bits |= (have >> (w * 16 / box_rows) & 1) << w;
+                        sm.mapped[n & 15] = bits;
+                        mbar_expect_tx(&sm.full[st], 2 * C::kTile);
+                    }
+                    __syncwarp();
+                    if (lane < 2 * per_kv)
+                        tma_load_5d(to + st * 2 * C::kTile, map, 0, (b * kBlk + box * box_rows) & (page_rows - 1), half, g.g,
+                                    page >= 0 ? page : bt.n_pages, &sm.full[st]);
                 }
             }
             if (!ok && lane == 0)  // let the copies in flight land (bounded) before the CTA ends
-                for (int i = max(0, k - C::kStages); i < k; i++)
-                    for (long long it = 0; it <= kWaitLimit; it++)
+                for (int i = max(0, n - C::kStages); i < n; i++)
+                    for (int it = 0; it <= kWaitLimit; it++)
                         if (mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
             if (!ok && lane == 0 && seg)
-                for (long long it = 0; it <= kWaitLimit; it++)
+                for (int it = 0; it <= kWaitLimit; it++)
                     if (mbar_try_wait(&sm.q_full, (seg - 1) & 1)) break;
-        } else if (warp == 9) {
-            // ── tensor cores ──
-            constexpr uint32_t id_s = idesc_f16(128, 128, false), id_o = idesc_f16(128, HD, true);
+        } else if (warp < 11) {
+            // ── tensor cores, for tile t ──
+            constexpr uint32_t id_s = idesc_f16(128, kBlk, false), id_o = idesc_f16(128, HD, true);
+            const int t = uniform(warp - 9);
             const uint32_t lead = lane == 0, tm = (uint32_t)uniform((int)tmem);
-            int k = 0, seg = 0;
-            int np0 = 0, np1 = 0;  // P tiles consumed of either tile
-            int no0 = 0, no1 = 0;  // segments whose O the tile has summed
+            const uint32_t ts = tm + C::kS + 128 * t, to = tm + C::kO + HD * t;
+            int k = 0, seg = 0;  // blocks, segments with work
+            int np = 0;  // P tiles consumed
+            int no = 0;  // segments whose O has been summed
             auto wait = [&](uint64_t* bar, int parity) {
-                ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+                ok = warp_wait(bar, parity, failed);
                 tc_fence_after();
                 return ok;
             };
             // descriptors of the first element; later ones add to the 14-bit address field
-            const uint64_t dq = sw128_desc(smem_u32(sm.q[0]), 16), dk = sw128_desc(smem_u32(sm.ring[0]), 16),
-                           dv = sw128_desc(smem_u32(sm.ring[0]), 16384);
-            auto mma_s = [&](int t, int st) {
-                const uint64_t a = dq + t * (C::kTile >> 4), b = dk + st * (C::kTile >> 4);
+            const uint64_t dq = sw128_desc(smem_u32(sm.q[t]), 16), dk = sw128_desc(smem_u32(sm.ring[0][0]), 16),
+                           dv = sw128_desc(smem_u32(sm.ring[0][1]), C::kHalf);
+            int ns = 0;  // S tiles made
+            auto mma_s = [&](int st) {
+                const uint64_t k0 = dk + st * (2 * C::kTile >> 4);
+                const uint32_t d = ts + 64 * (ns & 1);
 #pragma unroll
-                for (int i = 0; i < HD / 16; i++) {
-                    const uint32_t o = ((i >> 2) * 16384 + (i & 3) * 32) >> 4;
-                    umma_ss(tm + C::kS + 128 * t, a + o, b + o, id_s, i != 0, lead);
-                }
-                umma_commit(&sm.s_full[t], lead);
-            };
-            // O_t += P_t V for one block; first: the segment's first, once the segment before's O has been read
-            auto mma_o = [&](int t, int st, bool first, int& np, int& no) {
-                if (first && no++ && !wait(&sm.o_free[t], no & 1)) return false;
-                const uint64_t v = dv + st * (C::kTile >> 4);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if (!wait(&sm.p_ready[t][h], np & 1)) return false;
-#pragma unroll
-                    for (int i = 4 * h; i < 4 * h + 4; i++)
-                        umma_ts(tm + C::kO + HD * t, tm + C::kS + 128 * t + 8 * i, v + i * (2048 >> 4), id_o,
-                                !first || i > 0, lead);
-                }
-                np++;
-                umma_commit(&sm.o_done[t], lead);
-                return true;
+                for (int i = 0; i < HD / 16; i++)
+                    umma_ss(d, dq + (((i >> 2) * C::kQHalf + (i & 3) * 32) >> 4), k0 + (((i >> 2) * C::kHalf + (i & 3) * 32) >> 4),
+                            id_s, i != 0, lead);
+                umma_commit(&sm.s_full[t][ns & 1], lead);
+                ns++;
             };
             for (int x = x0; x < x1 && ok;) {
                 const Seg g = find_seg<HD>(p, sm, items, x, x1);
                 x = uniform(x + g.b1 - g.b0);
-                const int b0 = uniform(g.b0), live0 = uniform(g.live[0]), live1 = uniform(g.live[1]);
-                const int e = max(live0, live1);
+                const int b0 = uniform(g.b0), live = uniform(g.live(t)), e = uniform(g.end());
                 if (e <= b0) continue;
                 if (!wait(&sm.q_full, seg & 1)) break;
                 seg++;
                 if (!wait(&sm.full[k % C::kStages], (k / C::kStages) & 1)) break;
-                if (b0 < live0) mma_s(0, k % C::kStages);
-                if (b0 < live1) mma_s(1, k % C::kStages);
-                umma_commit(&sm.empty[k % C::kStages], lead);
+                if (b0 < live) mma_s(k % C::kStages);
                 if (b0 + 1 == e) umma_commit(&sm.q_empty, lead);
-                for (int b = b0; b < e; b++, k += 2) {
-                    const int sv = (k + 1) % C::kStages, sk = (k + 2) % C::kStages;
-                    if (!wait(&sm.full[sv], ((k + 1) / C::kStages) & 1)) break;
-                    if (b < live0 && !mma_o(0, sv, b == b0, np0, no0)) break;
-                    if (b + 1 < e && !wait(&sm.full[sk], ((k + 2) / C::kStages) & 1)) break;
-                    if (b + 1 < live0) mma_s(0, sk);
-                    if (b < live1 && !mma_o(1, sv, b == b0, np1, no1)) break;
-                    umma_commit(&sm.empty[sv], lead);
-                    if (b + 1 < live1) mma_s(1, sk);
-                    if (b + 1 < e) umma_commit(&sm.empty[sk], lead);
-                    if (b + 2 == e) umma_commit(&sm.q_empty, lead);
+                for (int b = b0; b < e; b++, k++) {
+                    const int st = k % C::kStages;
+                    if (b + 1 < e) {
+                        // The next scores, into the buffer of the last P: the products of one tile run in
+                        // order, so that P has been read by then.
+                        const int next = (k + 1) % C::kStages;
+                        if (B2_RARE(!wait(&sm.full[next], ((k + 1) / C::kStages) & 1))) break;
+                        if (b + 1 < live) mma_s(next);
+                        if (b + 2 == e) umma_commit(&sm.q_empty, lead);
+                    }
+                    if (b < live) {
+                        const bool first = b == b0;
+                        // the segment before's O has been read
+                        if (B2_RARE(first && no++ && !wait(&sm.o_free[t], no & 1))) break;
+                        const uint64_t v = dv + st * (2 * C::kTile >> 4);
+                        if (B2_RARE(!wait(&sm.p_ready[t][np & 1], (np >> 1) & 1))) break;
+                        const uint32_t pt = ts + 64 * (np & 1);
+#pragma unroll
+                        for (int i = 0; i < kBlk / 16; i++)
+                            umma_ts(to, pt + 8 * i, v + i * (2048 >> 4), id_o, !first || i > 0, lead);
+                        umma_commit(&sm.o_done[t][np & 1], lead);
+                        np++;
+                    }
+                    umma_commit(&sm.empty[st], lead);
                 }
             }
             if (!ok) {  // nothing of the tensor cores may be left running
-                umma_commit(&sm.drain, lead);
-                for (long long it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.drain, 0)) break;
+                umma_commit(&sm.drain[t], lead);
+                for (int it = 0; it <= kWaitLimit; it++)
+                    if (mbar_try_wait(&sm.drain[t], 0)) break;
             }
         }
     } else {
@@ -303,7 +323,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         // ── softmax of tile t: thread = row ──
         const int t = warp >> 2, r = threadIdx.x & 127;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t ts = tmem + lanes + C::kS + 128 * t, to = tmem + lanes + C::kO + HD * t;
+        const uint32_t s0 = tmem + lanes + C::kS + 128 * t, to = tmem + lanes + C::kO + HD * t;
         const float scale = kLog2e / sqrtf((float)HD);
         int nblk = 0;  // blocks of all segments so far (the producer's count)
         int ns = 0;    // of them this tile's
@@ -311,109 +331,117 @@ __global__ void __launch_bounds__(kThreads, 1)
         for (int x = x0; x < x1 && ok;) {
             const Seg g = find_seg<HD>(p, sm, items, x, x1);
             x += g.b1 - g.b0;
-            const int tok = r / p.a.G, first = g.b0;
-            const bool live = tok < g.tok[t];
-            const int lim = live ? min(g.sq.len - 1, g.sq.base + g.i0 + t * p.T + tok) : -1;
+            const int tok = r / p.a.G, first = uniform(g.b0), last = uniform(g.live(t)), len = uniform(g.sq.len);
+            const bool live = tok < g.tok(t);
+            const int lim = live ? min(len - 1, g.sq.base + g.i0 + t * p.T + tok) : -1;
             float m = -INFINITY;
-            uint64_t l2[2] = {pack_f2(0.f, 0.f), pack_f2(0.f, 0.f)};  // sums, two slots at a time
-            for (int b = first; b < g.live[t]; b++, ns++) {
-                const int j0 = b * kBlk, n = nblk + (b - first);
-                ok = mbar_wait(&sm.s_full[t], ns & 1, failed);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+            uint64_t l2 = pack_f2(0.f, 0.f);  // sum of even and of odd slots
+            uint32_t sv[kBlk];
+            // the scores of block number i of this tile, asked for while the block before is put away
+            auto load_s = [&](int i) {
+                ok = warp_wait(&sm.s_full[t][i & 1], (i >> 1) & 1, failed);
+                if (!ok) return;
                 tc_fence_after();
-                uint32_t sv[128];
-                tmem_ld32<0>(ts, sv);
-                tmem_ld32<32>(ts + 32, sv);
+                tmem_ld32<0>(s0 + 64 * (i & 1), sv);
+                tmem_ld32<32>(s0 + 64 * (i & 1) + 32, sv);
+            };
+            if (first < last) load_s(ns);
+            if (!ok) break;
+            // blocks from here on hold slots that some row of the warp does not see, or that are not
+            // cached (whose V rows the four warps zero together)
+            const int edge_from = __reduce_min_sync(0xffffffffu, live ? max(lim + 1, 0) : len) / kBlk;
+            const uint64_t scale2 = pack_f2(scale, scale);
+            // One block; edge: with slots that are not seen.  Two copies, because a path beside the common
+            // one costs that one a fifth of its time even where it is not taken.
+            auto step = [&](auto edge, int b, int bits) {
+                const int j0 = b * kBlk, n = nblk + (b - first);
+                const uint32_t ts = s0 + 64 * (ns & 1);
                 tmem_wait_ld();
-                tmem_ld32<64>(ts + 64, sv);
-                tmem_ld32<96>(ts + 96, sv);
-                const int bits = *(volatile int*)&sm.mapped[n & 7];
-                const bool masked = bits != 0xff || __any_sync(0xffffffffu, live && lim < j0 + kBlk - 1);
-                auto mask = [&](int c0) {
+                if constexpr (decltype(edge)::value) {
+                    // bit c of the pair: the row sees slot j0 + c
+                    const int seen = lim - j0 + 1;
+                    uint32_t lo = (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
+                    uint32_t hi = (bits & 4 ? 0xffffu : 0u) | (bits & 8 ? 0xffff0000u : 0u);
+                    if (seen < 32) lo &= (1u << max(seen, 0)) - 1;
+                    if (seen < 64) hi &= (1u << max(seen - 32, 0)) - 1;
 #pragma unroll
-                    for (int c = c0; c < c0 + 64; c++)
-                        if (j0 + c > lim || !(bits >> (c >> 4) & 1)) sv[c] = 0xff800000u;  // -inf
-                };
+                    for (int c = 0; c < kBlk; c++)
+                        if (!((c < 32 ? lo : hi) >> (c & 31) & 1)) sv[c] = 0xff800000u;  // -inf
+                    if (len < j0 + kBlk) {
+                        // V rows past kv_len may hold anything: zero them (their P is zero, and 0 x inf is not)
+                        // (S from this stage's K is there, so its V is)
+                        unsigned char* v = sm.ring[n % C::kStages][1];
+                        for (int i = r; i < (j0 + kBlk - len) * (HD / 8); i += 128) {
+                            const int row = len - j0 + i / (HD / 8), c = i % (HD / 8);
+                            *reinterpret_cast<uint4*>(v + (c >> 3) * C::kHalf + row * 128 + (c & 7) * 16) =
+                                make_uint4(0, 0, 0, 0);
+                        }
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                }
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-                auto top = [&](int c0) {
 #pragma unroll
-                    for (int c = c0; c < c0 + 64; c += 8)
-#pragma unroll
-                        for (int e = 0; e < 4; e++)
-                            mx4[e] = max3(mx4[e], __uint_as_float(sv[c + 2 * e]), __uint_as_float(sv[c + 2 * e + 1]));
-                };
-                if (masked) mask(0);
-                top(0);
-                tmem_wait_ld();
-                if (masked) mask(64);
-                top(64);
-                const float mx = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])) * scale;
+                for (int i = 0; i < kBlk / 2; i++)
+                    mx4[i & 3] = max3(mx4[i & 3], __uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1]));
+                const float mx = max3(fmaxf(mx4[0], mx4[1]), mx4[2], mx4[3]) * scale;
                 // a new reference for rows that outgrew theirs
                 const bool grow = live && (mx > m + kLazy || (m == -INFINITY && mx > m));
-                if (b == first) {
-                    m = mx;
-                } else if (__any_sync(0xffffffffu, grow)) {
+                if (B2_RARE(__any_sync(0xffffffffu, grow))) {
                     const float f = grow ? ex2(m - mx) : 1.f;
-                    ok = mbar_wait(&sm.o_done[t], (ns - 1) & 1, failed);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    tc_fence_after();
-#pragma unroll 1
-                    for (int c = 0; c < HD; c += 32) {
-                        uint32_t ov[32];
-                        tmem_ld32<0>(to + c, ov);
-                        tmem_wait_ld();
-#pragma unroll
-                        for (int i = 0; i < 32; i++) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
-                        tmem_st32(to + c, ov);
-                    }
-                    l2[0] = fma_f2(l2[0], pack_f2(f, f), pack_f2(0.f, 0.f));
-                    l2[1] = fma_f2(l2[1], pack_f2(f, f), pack_f2(0.f, 0.f));
                     if (grow) m = mx;
-                }
-                if (g.sq.len < j0 + kBlk) {
-                    // V rows past kv_len may hold anything: zero them (their P is zero, and 0 x inf is not)
-                    const int kvn = 2 * n + 1;
-                    ok = mbar_wait(&sm.full[kvn % C::kStages], (kvn / C::kStages) & 1, failed);
-                    if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
-                    unsigned char* v = sm.ring[kvn % C::kStages];
-                    for (int i = r; i < (j0 + kBlk - g.sq.len) * (HD / 8); i += 128) {
-                        const int row = g.sq.len - j0 + i / (HD / 8), c = i % (HD / 8);
-                        *reinterpret_cast<uint4*>(v + (c >> 3) * 16384 + row * 128 + (c & 7) * 16) = make_uint4(0, 0, 0, 0);
+                    if (b > first) {
+                        l2 = fma_f2(l2, pack_f2(f, f), pack_f2(0.f, 0.f));
+                        ok = warp_wait(&sm.o_done[t][(ns - 1) & 1], ((ns - 1) >> 1) & 1, failed);
+                        tc_fence_after();
+#pragma unroll 1
+                        for (int c = 0; c < HD && ok; c += 32) {
+                            uint32_t ov[32];
+                            tmem_ld32<0>(to + c, ov);
+                            tmem_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; i++) ov[i] = __float_as_uint(__uint_as_float(ov[i]) * f);
+                            tmem_st32(to + c, ov);
+                        }
                     }
-                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 }
+                uint32_t pk[kBlk / 2];
+                uint64_t add[2] = {pack_f2(0.f, 0.f), pack_f2(0.f, 0.f)};
                 const float bias = m == -INFINITY ? 0.f : kUp - m;
-                const uint64_t scale2 = pack_f2(scale, scale), bias2 = pack_f2(bias, bias);
+                const uint64_t bias2 = pack_f2(bias, bias);
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    uint32_t pk[32];
-#pragma unroll
-                    for (int i = 0; i < 32; i++) {
-                        const int c = 64 * h + 2 * i;
-                        float x, y;
-                        unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[c]), __uint_as_float(sv[c + 1])), scale2, bias2), x, y);
-                        x = ex2(x);
-                        y = ex2(y);
-                        l2[i & 1] = add_f2(l2[i & 1], pack_f2(x, y));
-                        pk[i] = pack_h2(x, y);
-                    }
-                    tmem_st32(ts + 32 * h, pk);
-                    tmem_wait_st();
-                    tc_fence_before();
-                    mbar_arrive(&sm.p_ready[t][h]);
+                for (int i = 0; i < kBlk / 2; i++) {
+                    float x, y;
+                    unpack_f2(fma_f2(pack_f2(__uint_as_float(sv[2 * i]), __uint_as_float(sv[2 * i + 1])), scale2, bias2), x, y);
+                    x = ex2(x);
+                    y = ex2(y);
+                    add[i & 1] = add_f2(add[i & 1], pack_f2(x, y));
+                    pk[i] = pack_h2(x, y);
                 }
+                tmem_st32(ts, pk);
+                l2 = add_f2(l2, add_f2(add[0], add[1]));
+                if (b + 1 < last) load_s(ns + 1);
+                tmem_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.p_ready[t][ns & 1]);
+            };
+            for (int b = first; b < last; b++, ns++) {
+                const int bits = *(volatile int*)&sm.mapped[(nblk + b - first) & 15];
+                if (B2_RARE(b >= edge_from || bits != (1 << kBlk / 16) - 1)) step(std::true_type{}, b, bits);
+                else step(std::false_type{}, b, bits);
+                if (B2_RARE(!ok)) break;
             }
             if (!ok) break;
             nblk += max(0, g.end() - first);
             // the pair's result, or this stretch's piece of it
-            const bool whole = g.b0 == 0 && g.b1 == g.nb, any = g.live[t] > first;
+            const bool whole = g.b0 == 0 && g.b1 == g.nb, any = last > first;
             if (any) {
-                ok = mbar_wait(&sm.o_done[t], (ns - 1) & 1, failed);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ok = warp_wait(&sm.o_done[t][(ns - 1) & 1], ((ns - 1) >> 1) & 1, failed);
+                if (!ok) break;
                 tc_fence_after();
             }
             float la, lb;
-            unpack_f2(add_f2(l2[0], l2[1]), la, lb);
+            unpack_f2(l2, la, lb);
             const float l = la + lb;
             const size_t row = (size_t)(g.sq.row0 + g.i0 + t * p.T + tok);
             const int h = g.g * p.a.G + r % p.a.G;
@@ -455,12 +483,13 @@ __global__ void __launch_bounds__(kThreads, 1)
                     p.a.lse[row * p.a.nq + h] = l == 0.f ? -INFINITY : (m - kUp) * kLn2 + logf(l);
             }
             tc_fence_before();
-            if (any) mbar_arrive(&sm.o_free[t]);
+            __syncwarp();
+            if (any && lane == 0) mbar_arrive(&sm.o_free[t]);
             if (!whole && g.b0 == 0) {
                 owns = true;
                 if (threadIdx.x == 0)
                     p.a.cuts[blockIdx.x] =
-                        Cut{(g.x0 + g.nb - 1) / per - (int)blockIdx.x + 1, g.sq.row0 + g.i0, g.tok[0] + g.tok[1], g.g};
+                        Cut{(g.x0 + g.nb - 1) / per - (int)blockIdx.x + 1, g.sq.row0 + g.i0, g.tok0 + g.tok1, g.g};
             }
         }
         if (threadIdx.x == 0 && !owns) p.a.cuts[blockIdx.x] = Cut{0, 0, 0, 0};
@@ -482,8 +511,9 @@ int launch_long(LongParams& p, const B2PagedKV* kv, int dev, int sms, cudaStream
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged smem: %s", cudaGetErrorString(e));
     CUtensorMap tq, tk, tv;
     const int box = kv->page_size < kBlk ? kv->page_size : kBlk;
-    int rc = b2_paged_map(&tk, kv->k_pages, kv, p.a.nkv, HD, box, 1);
-    if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, p.a.nkv, HD, box, 1);
+    const int halves = box == kBlk ? HD / 64 : 1;
+    int rc = b2_paged_map(&tk, kv->k_pages, kv, p.a.nkv, HD, box, halves);
+    if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, p.a.nkv, HD, box, halves);
     if (!rc) rc = q_map(&tq, p.a.q16, p.a.ldq, p.a.bt.M, p.a.nkv, p.a.G, HD, p.T);
     if (rc) return rc;
     e = b2::launch_pdl(attn_long_kernel<HD>, dim3(sms), dim3(kThreads), smem, s, tq, tk, tv, p);

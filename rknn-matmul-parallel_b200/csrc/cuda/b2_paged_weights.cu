@@ -184,9 +184,9 @@ __device__ __forceinline__ uint32_t in_rank(const void* p, uint32_t rank) {
 __device__ __forceinline__ void remote_arrive(uint32_t bar) {
     asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// mbar_wait whose barrier other CTAs of the cluster arrive on.
+// warp_wait for a barrier that other CTAs of the cluster arrive on.
 __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
-    for (long long it = 0;; it++) {
+    for (int it = 0;; it++) {
         uint32_t ok;
         asm volatile(
             "{\n .reg .pred p;\n mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n selp.u32 %0, 1, "
@@ -194,8 +194,8 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, vol
             : "=r"(ok)
             : "r"(smem_u32(bar)), "r"(parity)
             : "memory");
-        if (ok) return true;
-        if (it > kWaitLimit || *failed) {
+        if (__all_sync(0xffffffffu, ok)) return true;
+        if (__any_sync(0xffffffffu, it > kWaitLimit || *failed)) {
             *failed = 1;
             return false;
         }
@@ -221,7 +221,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             mbar_init(&sm.q_empty[i], 1);
             for (int t = 0; t < 2; t++) {
                 mbar_init(&sm.s_full[t][i], 1);
-                mbar_init(&sm.s_free[t][i], 128);
+                mbar_init(&sm.s_free[t][i], 4);
             }
             mbar_init(&sm.sum_full[i], 256 * (S - 1) + (S == 1));
             mbar_init(&sm.sum_free[i], 256);
@@ -257,8 +257,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             const Unit u = find_unit(p, sm.pre, T, x);
             if (u.first + rank >= u.tiles) continue;
             const int kb = nu & 1;
-            if (nu >= 2 && !mbar_wait(&sm.k_empty[kb], (nu / 2 - 1) & 1, failed)) ok = false;
-            ok = __all_sync(0xffffffffu, ok);
+            if (nu >= 2) ok = warp_wait(&sm.k_empty[kb], (nu / 2 - 1) & 1, failed);
             if (!ok) break;
             nu++;
             if (lane == 0) mbar_expect_tx(&sm.k_full[kb], 2 * Sm::kTile);
@@ -280,8 +279,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                     const float l = in ? p.lse[(size_t)(u.sq.row0 + r / p.G) * p.nq + u.g * p.G + r % p.G] : -INFINITY;
                     nl[e] = l == -INFINITY ? -INFINITY : -l * kLog2e;
                 }
-                if (nq >= 2 && !mbar_wait(&sm.q_empty[qb], (nq / 2 - 1) & 1, failed)) ok = false;
-                ok = __all_sync(0xffffffffu, ok);
+                if (nq >= 2) ok = warp_wait(&sm.q_empty[qb], (nq / 2 - 1) & 1, failed);
                 if (!ok) break;
 #pragma unroll
                 for (int e = 0; e < 4; e++) sm.nl[nq & 7][32 * e + lane] = nl[e];
@@ -294,10 +292,10 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         }
         if (!ok && lane == 0) {  // let the copies in flight land (bounded) before the CTA ends
             for (int i = max(0, nu - 2); i < nu; i++)
-                for (long long it = 0; it <= kWaitLimit; it++)
+                for (int it = 0; it <= kWaitLimit; it++)
                     if (mbar_try_wait(&sm.k_full[i & 1], (i / 2) & 1)) break;
             for (int i = max(0, nq - 2); i < nq; i++)
-                for (long long it = 0; it <= kWaitLimit; it++)
+                for (int it = 0; it <= kWaitLimit; it++)
                     if (mbar_try_wait(&sm.q_full[i & 1], (i / 2) & 1)) break;
         }
     } else if (warp == 9) {
@@ -305,7 +303,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         constexpr uint32_t id = idesc_f16(128, kRowsT, false);
         const uint32_t lead = lane == 0, tm = (uint32_t)uniform((int)tmem);
         auto wait = [&](uint64_t* bar, int parity) {
-            ok = __all_sync(0xffffffffu, mbar_wait(bar, parity, failed));
+            ok = warp_wait(bar, parity, failed);
             tc_fence_after();
             return ok;
         };
@@ -339,7 +337,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         }
         if (!ok) {  // nothing of the tensor cores may be left running
             umma_commit(&sm.drain, lead);
-            for (long long it = 0; it <= kWaitLimit; it++)
+            for (int it = 0; it <= kWaitLimit; it++)
                 if (mbar_try_wait(&sm.drain, 0)) break;
         }
     } else {
@@ -354,8 +352,8 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             float acc[4] = {0.f, 0.f, 0.f, 0.f};
             for (int i = u.first + rank; i < u.tiles; i += S, nq++) {
                 const int b = nq & 1;
-                ok = mbar_wait(&sm.s_full[t][b], (nq / 2) & 1, failed);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                ok = warp_wait(&sm.s_full[t][b], (nq / 2) & 1, failed);
+                if (!ok) break;
                 tc_fence_after();
                 const uint32_t ts = tmem + lanes + (2 * t + b) * 128;
                 uint32_t sv[128];
@@ -365,7 +363,8 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 tmem_ld32<96>(ts + 96, sv);
                 tmem_wait_ld();
                 tc_fence_before();
-                mbar_arrive(&sm.s_free[t][b]);
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sm.s_free[t][b]);
                 // columns of tokens from the slot's own on, and rows that exist
                 const int c0 = min(j - u.sq.base - i * T, kRowsT) * p.G, c1 = min(T * p.G, u.rows - i * T * p.G);
                 const float* nl = sm.nl[nq & 7];
@@ -389,7 +388,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             if (rank > 0) {
                 // to the first CTA, once it has read what this buffer held two units ago
                 if (done >= 2) ok = cluster_wait(&sm.sum_free[par], (done / 2 - 1) & 1, failed);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                if (!ok) break;
                 asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_rank(&sm.part[par][rank - 1][slot], 0)), "f"(total)
                              : "memory");
                 remote_arrive(in_rank(&sm.sum_full[par], 0));
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             }
             if (S > 1) {
                 ok = cluster_wait(&sm.sum_full[par], (done / 2) & 1, failed);
-                if (!__all_sync(0xffffffffu, ok)) { ok = false; break; }
+                if (!ok) break;
                 for (int e = 1; e < S; e++) total += sm.part[par][e - 1][slot];
                 for (int e = 1; e < S; e++) remote_arrive(in_rank(&sm.sum_free[par], e));
             }
