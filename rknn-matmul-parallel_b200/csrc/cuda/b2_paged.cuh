@@ -215,6 +215,7 @@ struct Cut {
 // (maximum, sum)[2][128].  CTA c's slot 2 c holds a piece that continues a
 // pair, slot 2 c + 1 one that begins it.
 constexpr int kLongRows = 128;
+constexpr int kMaxLongCtas = 256;
 __host__ __device__ constexpr int long_piece_floats(int hd) { return 2 * kLongRows * (hd + 2); }
 
 constexpr float kLn2 = 0.69314718055994531f;
@@ -226,6 +227,24 @@ constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float piece_weight(float m, float M) { return m == -INFINITY ? 1.f : ex2(m - M); }
 
 __host__ __device__ __forceinline__ int cdiv(int a, int b) { return (a + b - 1) / b; }
+
+// The line of work and its cuts.  CTA c's stretch begins at place c per, or at the
+// near end of the tile there (nb blocks, the place being b into it) when that is
+// within snap_of blocks: a piece costs about as much as six blocks of 64 slots, so
+// short stretches rather take a tile of up to 16 blocks whole, and long ones stay
+// even.
+__device__ __forceinline__ int snap_of(int per) { return per <= 8 ? 8 : min(8, max(3, per / 8)); }
+__device__ __forceinline__ int snap_to(int x, int b, int nb, int per) {
+    const int snap = snap_of(per);
+    return b <= snap && b <= nb - b ? x - b : nb - b <= snap ? x - b + nb : x;
+}
+// The CTAs own .. last whose stretches share the tile of nb blocks at place x0: it
+// is whole where own >= last.
+__device__ __forceinline__ void cut_of(int x0, int nb, int per, int& own, int& last) {
+    const int snap = snap_of(per);
+    own = (x0 + snap) / per;
+    last = cdiv(x0 + nb - snap, per) - 1;
+}
 
 // Host: dynamic shared memory opt-in, once per kernel and device.
 template <typename K>

@@ -40,8 +40,7 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
 // blocks.  Every CTA takes an equal stretch of that line, so sequences of any
 // mix of lengths load the SMs evenly; a tile that a stretch boundary cuts is
 // summed in pieces, which the last CTA to arrive merges in the line's order.
-// A boundary near a tile's end moves there (snap_of): a piece costs about as
-// much as six blocks.
+// A boundary near a tile's end moves there.
 //
 // A producer warp walks the stretch: for each tile it copies the Q rows, then
 // the K and V blocks through the page table into a ring of stages, across tile
@@ -94,17 +93,13 @@ struct ShortSmem {
     int pre[B2_PAGED_MAX_SEQS + 1];
 };
 
-// Blocks within which a boundary moves to a tile's end: short stretches rather
-// take a tile of up to 16 blocks whole than split it.
-__device__ __forceinline__ int snap_of(int per) { return per <= 8 ? 8 : max(3, per / 8); }
-
 // Where the stretch of CTA c begins.  T: tokens of one tile.
 __device__ __forceinline__ int stretch_start(const AttnParams& p, const int* pre, int W, int per, int c) {
     const long long at = (long long)c * per;
     if (at >= W) return W;
     const int x = (int)at, s = prefix_find(pre, p.bt.n_seqs, x);
-    const int nb = max(1, cdiv(p.bt.seq(s).len, kBlk)), b = (x - pre[s]) % nb, snap = snap_of(per);
-    return b <= snap && b <= nb - b ? x - b : nb - b <= snap ? x - b + nb : x;
+    const int nb = max(1, cdiv(p.bt.seq(s).len, kBlk));
+    return snap_to(x, (x - pre[s]) % nb, nb, per);
 }
 
 __device__ __forceinline__ Seg find_seg(const AttnParams& p, int T, const int* pre, int x, int x1) {
@@ -193,34 +188,52 @@ __device__ __forceinline__ void merge_pieces(const AttnParams& p, const Seg& sg,
 //
 // Tile pairs that it left in pieces, by the four computing warps, one row per
 // thread.  A task is CC chunks of four dims of one tile; the tasks of all pairs
-// go round the CTAs.
-template <int HD, int CC>
+// go round the CTAs.  NB pieces are in flight at a time: bound by reading them.
+template <int HD, int CC, int NB>
 __device__ __forceinline__ void merge_task(const AttnParams& p, int owner, const Cut& cut, int t, int c0) {
     const int r = threadIdx.x, T = kLongRows / p.G, tok = r / p.G;
-    if (tok >= min(T, cut.tokens - t * T)) return;
-    auto piece = [&](int i) { return p.long_part + (size_t)(2 * (owner + i) + (i == 0)) * long_piece_floats(HD); };
-    const int ml = 2 * kLongRows * HD + 2 * (t * kLongRows + r);
-    float M = -INFINITY;
-    for (int i = 0; i < cut.pieces; i++) M = fmaxf(M, __ldcg(piece(i) + ml));
-    float l = 0.f;
+    const bool live = tok < min(T, cut.tokens - t * T);
+    if (!__any_sync(0xffffffffu, live)) return;
+    const int ml0 = 2 * kLongRows * HD + 2 * (t * kLongRows + r), o0 = (t * (HD / 4) + c0) * kLongRows * 4 + 4 * r;
+    float M = -INFINITY, l = 0.f;
     float4 acc[CC];
 #pragma unroll
     for (int c = 0; c < CC; c++) acc[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll(CC == 1 ? 8 : 2)
-    for (int i = 0; i < cut.pieces; i++) {
-        const float* q = piece(i);
-        const float2 v = __ldcg(reinterpret_cast<const float2*>(q + ml));
-        const float w = piece_weight(v.x, M);
-        l = fmaf(v.y, w, l);
+    for (int j0 = 0; j0 < cut.pieces; j0 += NB) {
+        float2 ml[NB];
+        float4 o[NB][CC];
 #pragma unroll
-        for (int c = 0; c < CC; c++) {
-            const float4 o = __ldcg(reinterpret_cast<const float4*>(q + ((size_t)(t * (HD / 4) + c0 + c) * kLongRows + r) * 4));
-            acc[c].x = fmaf(o.x, w, acc[c].x);
-            acc[c].y = fmaf(o.y, w, acc[c].y);
-            acc[c].z = fmaf(o.z, w, acc[c].z);
-            acc[c].w = fmaf(o.w, w, acc[c].w);
+        for (int j = 0; j < NB; j++) {
+            const int i = min(j0 + j, cut.pieces - 1);
+            const float* q = p.long_part + (size_t)(2 * (owner + i) + (i == 0)) * long_piece_floats(HD);
+            ml[j] = ld_cg2(q + ml0);
+#pragma unroll
+            for (int c = 0; c < CC; c++) o[j][c] = ld_cg4(q + o0 + c * kLongRows * 4);
+        }
+        __syncwarp();  // no load moves behind this
+        float top = M;
+#pragma unroll
+        for (int j = 0; j < NB; j++) top = fmaxf(top, ml[j].x);
+        const float f = piece_weight(M, top);
+        M = top;
+        l *= f;
+#pragma unroll
+        for (int c = 0; c < CC; c++) acc[c].x *= f, acc[c].y *= f, acc[c].z *= f, acc[c].w *= f;
+#pragma unroll
+        for (int j = 0; j < NB; j++) {
+            if (j0 + j >= cut.pieces) break;
+            const float w = piece_weight(ml[j].x, M);
+            l = fmaf(ml[j].y, w, l);
+#pragma unroll
+            for (int c = 0; c < CC; c++) {
+                acc[c].x = fmaf(o[j][c].x, w, acc[c].x);
+                acc[c].y = fmaf(o[j][c].y, w, acc[c].y);
+                acc[c].z = fmaf(o[j][c].z, w, acc[c].z);
+                acc[c].w = fmaf(o[j][c].w, w, acc[c].w);
+            }
         }
     }
+    if (!live) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const size_t row = (size_t)(cut.row0 + t * T + tok);
     const int h = cut.g * p.G + r % p.G;
@@ -237,31 +250,45 @@ __device__ __forceinline__ void merge_task(const AttnParams& p, int owner, const
 
 template <int HD>
 __device__ __forceinline__ void merge_long(const AttnParams& p, int* scratch) {
-    constexpr int kBatch = 256;  // cuts read at a time
-    static_assert(kBatch * 4 <= B2_PAGED_MAX_SEQS, "scratch");
-    constexpr int kFew = 16;  // pieces up to which a task takes 8 chunks; more pieces, more tasks
-    Cut* cuts = reinterpret_cast<Cut*>(scratch);
-    int next = 0;  // tasks before
-    for (int base = 0; base < p.long_ctas; base += kBatch) {
-        const int n = min(kBatch, p.long_ctas - base);
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        for (int i = threadIdx.x; i < n; i += 128) {
-            const int4 v = __ldcg(reinterpret_cast<const int4*>(p.cuts + base + i));
-            cuts[i] = Cut{v.x, v.y, v.z, v.w};
-        }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        for (int i = 0; i < n; i++) {
-            const Cut cut = cuts[i];
-            if (cut.pieces == 0) continue;
-            const bool few = cut.pieces <= kFew;
-            const int per_tile = few ? HD / 32 : HD / 4, tasks = per_tile * (cut.tokens * p.G > kLongRows / p.G * p.G ? 2 : 1);
-            const int grid = gridDim.x;
-            for (int k = ((int)blockIdx.x - next % grid + grid) % grid; k < tasks; k += grid) {
-                if (few) merge_task<HD, 8>(p, base + i, cut, k / per_tile, k % per_tile * 8);
-                else merge_task<HD, 1>(p, base + i, cut, k / per_tile, k % per_tile);
-            }
-            next += tasks;
-        }
+    constexpr int kMaxCuts = kMaxLongCtas;
+    static_assert(kMaxCuts == 2 * 128, "two cuts per thread");
+    static_assert(kMaxCuts + 1 + 4 <= B2_PAGED_MAX_SEQS, "scratch");
+    constexpr int kFew = 16;  // pieces up to which a task takes four chunks; more pieces, more tasks
+    int* before = scratch;    // tasks of the cuts before each
+    int* sums = scratch + kMaxCuts + 1;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    auto tasks_of = [&](const Cut& c) {
+        if (c.pieces == 0) return 0;
+        const int tiles = c.tokens > kLongRows / p.G ? 2 : 1;
+        return tiles * (c.pieces <= kFew ? HD / 16 : HD / 4);
+    };
+    auto cut_at = [&](int i) {
+        const int4 v = i < p.long_ctas ? __ldcg(reinterpret_cast<const int4*>(p.cuts + i)) : make_int4(0, 0, 0, 0);
+        return Cut{v.x, v.y, v.z, v.w};
+    };
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const int a = tasks_of(cut_at(2 * tid)), b = tasks_of(cut_at(2 * tid + 1));
+    int incl = a + b;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int t = __shfl_up_sync(0xffffffffu, incl, o);
+        if (lane >= o) incl += t;
+    }
+    if (lane == 31) sums[warp] = incl;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    for (int w = 0; w < warp; w++) incl += sums[w];
+    before[2 * tid] = incl - a - b;
+    before[2 * tid + 1] = incl - b;
+    if (tid == 127) before[kMaxCuts] = incl;
+    asm volatile("bar.sync 1, 128;" ::: "memory");
+    const int total = before[kMaxCuts];
+    for (int k = blockIdx.x; k < total; k += gridDim.x) {
+        const int i = prefix_find(before, kMaxCuts, k), rest = k - before[i];
+        const Cut cut = cut_at(i);
+        const bool few = cut.pieces <= kFew;
+        const int per_tile = few ? HD / 16 : HD / 4;
+        if (few) merge_task<HD, 4, 4>(p, i, cut, rest / per_tile, rest % per_tile * 4);
+        else merge_task<HD, 1, 16>(p, i, cut, rest / per_tile, rest % per_tile);
     }
 }
 
@@ -577,11 +604,9 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
             }
         }
         sync4();
-        // A boundary strictly inside the tile, away from its ends, cuts it.
-        const int snap = snap_of(per);
-        const int c_lo = (sg.x0 + snap) / per + 1, c_hi = (sg.x0 + sg.nb - snap + per - 1) / per - 1;
-        const bool whole = c_lo > c_hi;
-        const int own = c_lo - 1, last = c_hi;  // CTAs of the pieces
+        int own, last;  // CTAs of the tile's pieces
+        cut_of(sg.x0, sg.nb, per, own, last);
+        const bool whole = own >= last;
         float* part = p.part + (size_t)(2 * blockIdx.x + (sg.b0 == 0 ? 1 : 0)) * C::kTile;
         for (int i = tid; i < rows * (HD / 8); i += 128) {
             const int r = i / (HD / 8), c = i % (HD / 8) * 8;
@@ -641,7 +666,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
 
 constexpr int kMaxGroup = 16;
 constexpr int kShortRows = 16;  // (token, head) rows of a kv head that the short kernel takes, at most
-constexpr size_t kCounterBytes = 4096, kCutBytes = 4096;
+constexpr size_t kCounterBytes = 4096, kCutBytes = kMaxLongCtas * sizeof(Cut);
 
 // CTAs of a launch: one or two per SM.
 template <int HD, int NT>

@@ -105,6 +105,17 @@ __device__ __forceinline__ int blocks_of(const LongParams& p, const Seq& q, int 
     return max(1, cdiv(min(q.len, max(0, q.base + last)), kBlk));
 }
 
+// Where the stretch of CTA c begins.
+template <int HD>
+__device__ __forceinline__ int stretch_start(const LongParams& p, const Smem<HD>& sm, int items, int W, int per, int c) {
+    const long long at = (long long)c * per;
+    if (at >= W) return W;
+    const int x = (int)at, e = prefix_find(sm.pre, items, x), s = prefix_find(sm.pre_seq, p.a.bt.n_seqs, e);
+    const Seq q = p.a.bt.seq(s);
+    const int first = (e - sm.pre_seq[s]) * p.group, nb = blocks_of(p, q, first + min(p.group, pairs_of(p, q) - first) - 1);
+    return snap_to(x, (x - sm.pre[e]) % nb, nb, per);
+}
+
 template <int HD>
 __device__ __forceinline__ Seg find_seg(const LongParams& p, const Smem<HD>& sm, int items, int x, int x1) {
     Seg r;
@@ -179,7 +190,8 @@ __global__ void __launch_bounds__(kThreads, 1)
     const uint32_t tmem = sm.tmem;
     const int W = items ? sm.pre[items] : 0;
     const int per = max(kMinBlocks, cdiv(W, gridDim.x));
-    const int x0 = (int)min((long long)W, (long long)blockIdx.x * per), x1 = min(W, x0 + per);
+    const int x0 = stretch_start<HD>(p, sm, items, W, per, blockIdx.x),
+              x1 = stretch_start<HD>(p, sm, items, W, per, blockIdx.x + 1);
     bool ok = true;
 
     if (warp >= 8) {
@@ -434,7 +446,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (!ok) break;
             nblk += max(0, g.end() - first);
             // the pair's result, or this stretch's piece of it
-            const bool whole = g.b0 == 0 && g.b1 == g.nb, any = last > first;
+            int own, end;  // CTAs of the pair's pieces
+            cut_of(g.x0, g.nb, per, own, end);
+            const bool whole = own >= end, any = last > first;
             if (any) {
                 ok = warp_wait(&sm.o_done[t][(ns - 1) & 1], ((ns - 1) >> 1) & 1, failed);
                 if (!ok) break;
@@ -489,7 +503,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 owns = true;
                 if (threadIdx.x == 0)
                     p.a.cuts[blockIdx.x] =
-                        Cut{(g.x0 + g.nb - 1) / per - (int)blockIdx.x + 1, g.sq.row0 + g.i0, g.tok0 + g.tok1, g.g};
+                        Cut{end - own + 1, g.sq.row0 + g.i0, g.tok0 + g.tok1, g.g};
             }
         }
         if (threadIdx.x == 0 && !owns) p.a.cuts[blockIdx.x] = Cut{0, 0, 0, 0};
@@ -516,7 +530,7 @@ int launch_long(LongParams& p, const B2PagedKV* kv, int dev, int sms, cudaStream
     if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, p.a.nkv, HD, box, halves);
     if (!rc) rc = q_map(&tq, p.a.q16, p.a.ldq, p.a.bt.M, p.a.nkv, p.a.G, HD, p.T);
     if (rc) return rc;
-    e = b2::launch_pdl(attn_long_kernel<HD>, dim3(sms), dim3(kThreads), smem, s, tq, tk, tv, p);
+    e = b2::launch_pdl(attn_long_kernel<HD>, dim3(p.a.long_ctas), dim3(kThreads), smem, s, tq, tk, tv, p);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged: %s", cudaGetErrorString(e));
     return 0;
 }
@@ -531,6 +545,6 @@ int b2_paged_attention_long(b2p::AttnParams& a, const B2PagedKV* kv, int hd, int
     const long long cap = ((long long)kv->max_pages * kv->page_size + kBlk - 1) / kBlk;
     if (pairs * a.nkv * cap >= (1ll << 31) - 65536)
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_attention_paged: %lld blocks of work in one call", pairs * a.nkv * cap);
-    a.long_ctas = p.a.long_ctas = sms;
+    a.long_ctas = p.a.long_ctas = sms < kMaxLongCtas ? sms : kMaxLongCtas;
     return hd == 128 ? launch_long<128>(p, kv, dev, sms, s) : launch_long<64>(p, kv, dev, sms, s);
 }
