@@ -5,6 +5,8 @@
 // over the new rows i that see slot j, from q, K and the row sums that the
 // attention left.  Every slot belongs to one warp, which adds its rows in
 // their order: no atomics, and the result does not depend on timing.
+#include <type_traits>
+
 #include "b2_tc.cuh"
 
 namespace {
@@ -122,9 +124,9 @@ __global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightPar
 // per pair).  A unit is 256 slots of one kv head: two K tiles of 128 slots, each
 // the A operand of S^T_t = K_t Q^T (tcgen05, N = 128 rows: T tokens x the G heads
 // of the group), so a thread owns a slot and adds its columns in registers, and a
-// Q tile brought in once serves both K tiles.  The CTAs of a cluster take every
-// S-th Q tile of a unit; their sums meet in the first one's shared memory and are
-// added in rank order.
+// Q tile brought in once serves both K tiles.  Where there are too few units to
+// go round, S CTAs of a cluster take every S-th Q tile of one; their sums meet in
+// the first one's shared memory and are added in rank order.
 //   warp 8      producer: the unit's K tiles (double-buffered), Q tiles and their
 //               rows' -lse;
 //   warp 9      tensor cores;
@@ -205,13 +207,12 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, vol
 template <int HD>
 __global__ void __launch_bounds__(kLongThreads, 1)
     weights_long_kernel(const __grid_constant__ CUtensorMap tq, const __grid_constant__ CUtensorMap tk, const WeightParams p,
-                        int S) {
+                        int cluster) {
     using Sm = LongSmem<HD>;
     constexpr int kHalves = HD / 64;
     extern __shared__ unsigned char smem_raw[];
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int rank = S > 1 ? (int)cluster_rank() : 0;
     volatile int* failed = &sm.failed;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
@@ -223,12 +224,10 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 mbar_init(&sm.s_full[t][i], 1);
                 mbar_init(&sm.s_free[t][i], 4);
             }
-            mbar_init(&sm.sum_full[i], 256 * (S - 1) + (S == 1));
             mbar_init(&sm.sum_free[i], 256);
         }
         mbar_init(&sm.drain, 1);
         sm.failed = 0;
-        mbar_init_fence();
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tq) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
     }
@@ -240,12 +239,25 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         const Seq q = p.bt.seq(s);
         return min(q.Q, p.max_q) * p.G > p.short_rows ? cdiv(q.len, kUnit) * p.nkv : 0;
     });
+    // CTAs per unit: the fewest that give the shortest schedule, a unit costing its Q
+    // tiles and about one more for its K tiles.
+    const int W = sm.pre[p.bt.n_seqs], all_tiles = cdiv(p.max_q, T);
+    int S = 1;
+    for (int c = 2; c <= cluster; c *= 2) {
+        auto cost = [&](int n) { return (long long)cdiv(W, gridDim.x / n) * (cdiv(all_tiles, n) + 1); };
+        if (cost(c) < cost(S)) S = c;
+    }
+    const int step = gridDim.x / S, rank = (int)blockIdx.x % S;
+    const uint32_t lead_cta = cluster > 1 ? cluster_rank() - rank : 0;  // this unit's first CTA, in the cluster
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; i++) mbar_init(&sm.sum_full[i], S > 1 ? 256 * (S - 1) : 1);
+        mbar_init_fence();
+    }
     tc_fence_before();
     __syncthreads();
-    if (S > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    if (cluster > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     tc_fence_after();
     const uint32_t tmem = sm.tmem;
-    const int W = sm.pre[p.bt.n_seqs], step = gridDim.x / S;
     bool ok = true;
 
     if (warp == 8) {
@@ -345,60 +357,84 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         const int t = warp >> 2, slot = threadIdx.x;
         const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
         const float scale = kLog2e / sqrtf((float)HD);
+        const uint64_t scale2 = pack_f2(scale, scale);
         int nq = 0, done = 0;  // Q tiles; units (all of them, with work here or not)
         for (int x = blockIdx.x / S; x < W && ok; x += step, done++) {
             const Unit u = find_unit(p, sm.pre, T, x);
             const int j = u.j0 + slot;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
-            for (int i = u.first + rank; i < u.tiles; i += S, nq++) {
+            uint64_t acc[2] = {pack_f2(0.f, 0.f), pack_f2(0.f, 0.f)};
+            const int first = uniform(u.first) + rank, tiles = uniform(u.tiles);
+            // One Q tile; edge: with columns that the slot is not seen by.  Two copies, because a path beside
+            // the common one costs that one time even where it is not taken.
+            auto step = [&](auto edge, int c0, int c1) {
                 const int b = nq & 1;
                 ok = warp_wait(&sm.s_full[t][b], (nq / 2) & 1, failed);
-                if (!ok) break;
                 tc_fence_after();
                 const uint32_t ts = tmem + lanes + (2 * t + b) * 128;
-                uint32_t sv[128];
-                tmem_ld32<0>(ts, sv);
-                tmem_ld32<32>(ts + 32, sv);
-                tmem_ld32<64>(ts + 64, sv);
-                tmem_ld32<96>(ts + 96, sv);
+                const float4* nl = reinterpret_cast<const float4*>(sm.nl[nq & 7]);
+                uint32_t va[32], vb[32];
+                // 32 columns from c0 on, the next ones on their way
+                auto add = [&](uint32_t (&v)[32], int col) {
+                    if constexpr (decltype(edge)::value) {
+#pragma unroll
+                        for (int c = 0; c < 32; c++)
+                            if (col + c < c0 || col + c >= c1) v[c] = 0xff800000u;  // -inf
+                    }
+#pragma unroll
+                    for (int c = 0; c < 32; c += 4) {
+                        const float4 n4 = nl[(col + c) / 4];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            float x, y;
+                            unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), scale2,
+                                             e ? pack_f2(n4.z, n4.w) : pack_f2(n4.x, n4.y)),
+                                      x, y);
+                            acc[e] = add_f2(acc[e], pack_f2(ex2(x), ex2(y)));
+                        }
+                    }
+                };
+                tmem_ld32<0>(ts, va);
+                tmem_wait_ld();
+                tmem_ld32<0>(ts + 32, vb);
+                add(va, 0);
+                tmem_wait_ld();
+                tmem_ld32<0>(ts + 64, va);
+                add(vb, 32);
+                tmem_wait_ld();
+                tmem_ld32<0>(ts + 96, vb);
+                add(va, 64);
                 tmem_wait_ld();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sm.s_free[t][b]);
+                add(vb, 96);
+            };
+            for (int i = first; i < tiles; i += S, nq++) {
                 // columns of tokens from the slot's own on, and rows that exist
                 const int c0 = min(j - u.sq.base - i * T, kRowsT) * p.G, c1 = min(T * p.G, u.rows - i * T * p.G);
-                const float* nl = sm.nl[nq & 7];
-                if (__any_sync(0xffffffffu, c0 > 0 || c1 < kRowsT)) {
-#pragma unroll
-                    for (int c = 0; c < kRowsT; c++)
-                        if (c < c0 || c >= c1) sv[c] = 0xff800000u;  // -inf
-                }
-#pragma unroll
-                for (int c = 0; c < kRowsT; c += 4) {
-                    const float4 n4 = *reinterpret_cast<const float4*>(nl + c);
-                    acc[0] += ex2(fmaf(__uint_as_float(sv[c]), scale, n4.x));
-                    acc[1] += ex2(fmaf(__uint_as_float(sv[c + 1]), scale, n4.y));
-                    acc[2] += ex2(fmaf(__uint_as_float(sv[c + 2]), scale, n4.z));
-                    acc[3] += ex2(fmaf(__uint_as_float(sv[c + 3]), scale, n4.w));
-                }
+                if (B2_RARE(__any_sync(0xffffffffu, c0 > 0 || c1 < kRowsT))) step(std::true_type{}, c0, c1);
+                else step(std::false_type{}, c0, c1);
+                if (B2_RARE(!ok)) break;
             }
             if (!ok) break;
-            float total = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+            float total, odd;
+            unpack_f2(add_f2(acc[0], acc[1]), total, odd);
+            total += odd;
             const int par = done & 1;
             if (rank > 0) {
                 // to the first CTA, once it has read what this buffer held two units ago
                 if (done >= 2) ok = cluster_wait(&sm.sum_free[par], (done / 2 - 1) & 1, failed);
                 if (!ok) break;
-                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_rank(&sm.part[par][rank - 1][slot], 0)), "f"(total)
+                asm volatile("st.shared::cluster.f32 [%0], %1;" ::"r"(in_rank(&sm.part[par][rank - 1][slot], lead_cta)), "f"(total)
                              : "memory");
-                remote_arrive(in_rank(&sm.sum_full[par], 0));
+                remote_arrive(in_rank(&sm.sum_full[par], lead_cta));
                 continue;
             }
             if (S > 1) {
                 ok = cluster_wait(&sm.sum_full[par], (done / 2) & 1, failed);
                 if (!ok) break;
                 for (int e = 1; e < S; e++) total += sm.part[par][e - 1][slot];
-                for (int e = 1; e < S; e++) remote_arrive(in_rank(&sm.sum_free[par], e));
+                for (int e = 1; e < S; e++) remote_arrive(in_rank(&sm.sum_free[par], lead_cta + e));
             }
             if (j < u.sq.len && j < p.ldw) {
                 const size_t o = ((size_t)u.s * p.nkv + u.g) * p.ldw + j;
@@ -410,7 +446,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
     tc_fence_before();
     __syncthreads();
     // the others may still write to or arrive at this CTA's shared memory
-    if (S > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+    if (cluster > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     if (warp == 9) {
         tc_fence_after();
         tmem_free512(tmem);
@@ -455,7 +491,7 @@ int launch_long(const WeightParams& p, const B2PagedKV* kv, int dev, int sms, cu
     int rc = b2_paged_map(&tk, kv->k_pages, kv, p.nkv, HD, box, 1);
     if (!rc) rc = q_map(&tq, p.q16, p.ldq, p.bt.M, p.nkv, p.G, HD, T);
     if (rc) return rc;
-    // as many CTAs per unit as Q tiles can keep busy
+    // clusters of as many CTAs as the Q tiles of a unit can keep busy
     const int tiles = cdiv(p.max_q, T);
     int S = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1, clusters = max_clusters<HD>(S, dev, sms, smem);
     if (clusters == 0) clusters = sms, S = 1;
