@@ -127,8 +127,7 @@ __global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightPar
 // Q tile brought in once serves both K tiles.  Where there are too few units to
 // go round, S CTAs of a cluster take every S-th Q tile of one; their sums meet in
 // the first one's shared memory and are added in rank order.
-//   warp 8      producer: the unit's K tiles (double-buffered), Q tiles and their
-//               rows' -lse;
+//   warp 8      producer: the unit's K tiles, Q tiles and their rows' -lse;
 //   warp 9      tensor cores;
 //   warps 0-3, 4-7   the exponentials of K tile 0 and 1, one slot per thread.
 constexpr int kUnit = 256;
@@ -139,11 +138,12 @@ constexpr int kMaxCluster = 4;
 template <int HD>
 struct LongSmem {
     static constexpr int kTile = 128 * HD * 2;
-    alignas(1024) unsigned char k[2][2][kTile];  // [buffer][tile]
-    alignas(1024) unsigned char q[2][kTile];
-    alignas(16) float nl[8][kRowsT];             // -lse log2(e) of the rows of Q tile (count % 8)
+    static constexpr int kQStages = HD == 128 ? 4 : 8;
+    alignas(1024) unsigned char k[2][kTile];  // [tile]
+    alignas(1024) unsigned char q[kQStages][kTile];
+    alignas(16) float nl[16][kRowsT];            // -lse log2(e) of the rows of Q tile (count % 16)
     float part[2][kMaxCluster - 1][kUnit];       // first CTA: the others' sums, by unit parity
-    uint64_t k_full[2], k_empty[2], q_full[2], q_empty[2];
+    uint64_t k_full, k_empty, q_full[kQStages], q_empty[kQStages];
     uint64_t s_full[2][2], s_free[2][2];         // [K tile][buffer]
     uint64_t sum_full[2], sum_free[2];
     uint64_t drain;
@@ -216,16 +216,18 @@ __global__ void __launch_bounds__(kLongThreads, 1)
     volatile int* failed = &sm.failed;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
-            mbar_init(&sm.k_full[i], 1);
-            mbar_init(&sm.k_empty[i], 1);
-            mbar_init(&sm.q_full[i], 1);
-            mbar_init(&sm.q_empty[i], 1);
             for (int t = 0; t < 2; t++) {
                 mbar_init(&sm.s_full[t][i], 1);
                 mbar_init(&sm.s_free[t][i], 4);
             }
             mbar_init(&sm.sum_free[i], 256);
         }
+        for (int i = 0; i < Sm::kQStages; i++) {
+            mbar_init(&sm.q_full[i], 1);
+            mbar_init(&sm.q_empty[i], 1);
+        }
+        mbar_init(&sm.k_full, 1);
+        mbar_init(&sm.k_empty, 1);
         mbar_init(&sm.drain, 1);
         sm.failed = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tq) : "memory");
@@ -265,50 +267,64 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         const int page_rows = 1 << p.bt.page_shift, box_rows = min(page_rows, 128), boxes = 128 / box_rows;
         const int box = lane / kHalves, half = lane % kHalves;
         int nu = 0, nq = 0;  // units and Q tiles loaded
+        // this lane's four rows of a Q tile
+        int tok[4], head[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+            tok[e] = (32 * e + lane) / p.G;
+            head[e] = (32 * e + lane) % p.G;
+        }
         for (int x = blockIdx.x / S; x < W && ok; x += step) {
             const Unit u = find_unit(p, sm.pre, T, x);
-            if (u.first + rank >= u.tiles) continue;
-            const int kb = nu & 1;
-            if (nu >= 2) ok = warp_wait(&sm.k_empty[kb], (nu / 2 - 1) & 1, failed);
-            if (!ok) break;
-            nu++;
-            if (lane == 0) mbar_expect_tx(&sm.k_full[kb], 2 * Sm::kTile);
-            __syncwarp();
+            const int first = uniform(u.first) + rank, tiles = uniform(u.tiles), toks = u.rows / p.G;
+            if (first >= tiles) continue;
+            const float* lse = p.lse + (size_t)u.sq.row0 * p.nq + u.g * p.G;
+            float next[4];
+            auto load_lse = [&](int i) {
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    next[e] = tok[e] < T && i * T + tok[e] < toks ? lse[(size_t)(i * T + tok[e]) * p.nq + head[e]] : -INFINITY;
+            };
+            load_lse(first);
+            // K of the unit before is done with; its pages
+            int page[2] = {-1, -1};
             if (box < boxes)
+#pragma unroll
                 for (int t = 0; t < 2; t++) {
                     const int j = u.j0 + t * 128 + box * box_rows;
-                    const int page = j < u.sq.len ? p.bt.page(u.s, j) : -1;
-                    tma_load_5d(sm.k[kb][t] + half * 16384 + box * box_rows * 128, &tk, 0, j & (page_rows - 1), half, u.g,
-                                page >= 0 ? page : p.bt.n_pages, &sm.k_full[kb]);
+                    page[t] = j < u.sq.len ? p.bt.page(u.s, j) : -1;
                 }
-            for (int i = u.first + rank; i < u.tiles; i += S, nq++) {
-                const int qb = nq & 1;
-                float nl[4];
+            if (nu) ok = warp_wait(&sm.k_empty, (nu - 1) & 1, failed);
+            if (!ok) break;
+            nu++;
+            if (lane == 0) mbar_expect_tx(&sm.k_full, 2 * Sm::kTile);
+            __syncwarp();
+            if (box < boxes)
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const int r = i * T * p.G + 32 * e + lane;  // rows of tile i are T G consecutive ones
-                    const bool in = 32 * e + lane < T * p.G && r < u.rows;
-                    const float l = in ? p.lse[(size_t)(u.sq.row0 + r / p.G) * p.nq + u.g * p.G + r % p.G] : -INFINITY;
-                    nl[e] = l == -INFINITY ? -INFINITY : -l * kLog2e;
-                }
-                if (nq >= 2) ok = warp_wait(&sm.q_empty[qb], (nq / 2 - 1) & 1, failed);
+                for (int t = 0; t < 2; t++)
+                    tma_load_5d(sm.k[t] + half * 16384 + box * box_rows * 128, &tk, 0, (u.j0 + box * box_rows) & (page_rows - 1),
+                                half, u.g, page[t] >= 0 ? page[t] : p.bt.n_pages, &sm.k_full);
+            for (int i = first; i < tiles; i += S, nq++) {
+                const int qb = nq % Sm::kQStages;
+                if (nq >= Sm::kQStages) ok = warp_wait(&sm.q_empty[qb], (nq / Sm::kQStages - 1) & 1, failed);
                 if (!ok) break;
 #pragma unroll
-                for (int e = 0; e < 4; e++) sm.nl[nq & 7][32 * e + lane] = nl[e];
+                for (int e = 0; e < 4; e++)
+                    sm.nl[nq & 15][32 * e + lane] = next[e] == -INFINITY ? -INFINITY : -next[e] * kLog2e;
                 __syncwarp();
                 if (lane == 0) mbar_expect_tx(&sm.q_full[qb], T * p.G * HD * 2);
                 __syncwarp();
                 if (lane < kHalves)
                     tma_load_5d(sm.q[qb] + lane * 16384, &tq, 0, 0, u.sq.row0 + i * T, lane, u.g, &sm.q_full[qb]);
+                if (i + S < tiles) load_lse(i + S);
             }
         }
         if (!ok && lane == 0) {  // let the copies in flight land (bounded) before the CTA ends
-            for (int i = max(0, nu - 2); i < nu; i++)
+            for (int it = 0; nu && it <= kWaitLimit; it++)
+                if (mbar_try_wait(&sm.k_full, (nu - 1) & 1)) break;
+            for (int i = max(0, nq - Sm::kQStages); i < nq; i++)
                 for (int it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.k_full[i & 1], (i / 2) & 1)) break;
-            for (int i = max(0, nq - 2); i < nq; i++)
-                for (int it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.q_full[i & 1], (i / 2) & 1)) break;
+                    if (mbar_try_wait(&sm.q_full[i % Sm::kQStages], (i / Sm::kQStages) & 1)) break;
         }
     } else if (warp == 9) {
         // ── tensor cores ──
@@ -320,22 +336,21 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             return ok;
         };
         // descriptors of the first element; later ones add to the 14-bit address field
-        const uint64_t dk = sw128_desc(smem_u32(sm.k[0][0]), 16), dq = sw128_desc(smem_u32(sm.q[0]), 16);
+        const uint64_t dk = sw128_desc(smem_u32(sm.k[0]), 16), dq = sw128_desc(smem_u32(sm.q[0]), 16);
         int nu = 0, nq = 0;
         for (int x = blockIdx.x / S; x < W && ok; x += step) {
             const Unit u = find_unit(p, sm.pre, T, x);
             const int first = uniform(u.first) + rank, tiles = uniform(u.tiles);
             if (first >= tiles) continue;
-            const int kb = nu & 1;
-            if (!wait(&sm.k_full[kb], (nu / 2) & 1)) break;
+            if (!wait(&sm.k_full, nu & 1)) break;
             nu++;
             for (int i = first; i < tiles && ok; i += S, nq++) {
-                const int b = nq & 1;
-                if (!wait(&sm.q_full[b], (nq / 2) & 1)) break;
+                const int b = nq & 1, st = nq % Sm::kQStages;
+                if (!wait(&sm.q_full[st], (nq / Sm::kQStages) & 1)) break;
 #pragma unroll
                 for (int t = 0; t < 2; t++) {
                     if (nq >= 2 && !wait(&sm.s_free[t][b], (nq / 2 - 1) & 1)) break;
-                    const uint64_t a = dk + (2 * kb + t) * (Sm::kTile >> 4), q = dq + b * (Sm::kTile >> 4);
+                    const uint64_t a = dk + t * (Sm::kTile >> 4), q = dq + st * (Sm::kTile >> 4);
 #pragma unroll
                     for (int e = 0; e < HD / 16; e++) {
                         const uint32_t o = ((e >> 2) * 16384 + (e & 3) * 32) >> 4;
@@ -343,9 +358,9 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                     }
                     umma_commit(&sm.s_full[t][b], lead);
                 }
-                umma_commit(&sm.q_empty[b], lead);
+                umma_commit(&sm.q_empty[st], lead);
             }
-            umma_commit(&sm.k_empty[kb], lead);
+            umma_commit(&sm.k_empty, lead);
         }
         if (!ok) {  // nothing of the tensor cores may be left running
             umma_commit(&sm.drain, lead);
@@ -371,7 +386,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 ok = warp_wait(&sm.s_full[t][b], (nq / 2) & 1, failed);
                 tc_fence_after();
                 const uint32_t ts = tmem + lanes + (2 * t + b) * 128;
-                const float4* nl = reinterpret_cast<const float4*>(sm.nl[nq & 7]);
+                const float4* nl = reinterpret_cast<const float4*>(sm.nl[nq & 15]);
                 uint32_t va[32], vb[32];
                 // 32 columns from c0 on, the next ones on their way
                 auto add = [&](uint32_t (&v)[32], int col) {
