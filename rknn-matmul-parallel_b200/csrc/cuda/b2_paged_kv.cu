@@ -46,25 +46,48 @@ struct PageStrides {
 // the row's position, and the rounding to FP16: q for the tensor cores of the
 // attention, K and V as the cache keeps them.  FP32 throughout, the sum of
 // squares across the warp.  Bound by HBM: 4 bytes read and 2 written per
-// element.  A warp takes kHeads heads of one row at a time, so their loads are
-// in flight together and the row's angles are read once.
-constexpr int kAppendThreads = 256;
+// element.  A warp takes `steps` times kHeads heads of one row, kHeads at a time
+// and the next ones on their way: with many rows a whole row, so that its place
+// and angles are looked up once, with few rows kHeads, so that there are warps.
+constexpr int kAppendThreads = 128;
 constexpr int kHeads = 4;
 
+template <int E>
+__device__ __forceinline__ void load_vec(float (&v)[E], const float* p, bool aligned) {
+    if (!aligned) {
+#pragma unroll
+        for (int j = 0; j < E; j++) v[j] = p[j];
+    } else if constexpr (E == 4) {
+        const float4 u = *reinterpret_cast<const float4*>(p);
+        v[0] = u.x, v[1] = u.y, v[2] = u.z, v[3] = u.w;
+    } else {
+        const float2 u = *reinterpret_cast<const float2*>(p);
+        v[0] = u.x, v[1] = u.y;
+    }
+}
+
+// aligned: the angle tables and norm weights allow 16-byte loads.
 template <int HD>
-__global__ void __launch_bounds__(kAppendThreads) append_kernel(
+__global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(
     __half* __restrict__ q16, int ldq, const float* __restrict__ qkv, int ldqkv, int nq, int nkv,
     const float* __restrict__ q_norm_w, const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_tab,
     const float* __restrict__ sin_tab, int max_pos, int rope_style, const int* __restrict__ pos_of, b2p::Batch bt,
-    PageStrides pg) {
+    PageStrides pg, bool aligned, int steps) {
     constexpr int E = HD / 32;  // elements per lane
     b2::pdl_trigger();
     b2::pdl_wait();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int heads = nq + 2 * nkv, per_row = (heads + kHeads - 1) / kHeads;
+    const int heads = nq + 2 * nkv, per_row = (heads + kHeads * steps - 1) / (kHeads * steps);
     const long long job = (long long)blockIdx.x * (kAppendThreads / 32) + warp;
-    const int m = (int)(job / per_row), h0 = (int)(job % per_row) * kHeads;
+    const int m = (int)(job / per_row);
+    int h0 = (int)(job % per_row) * kHeads * steps;
+    const int h_end = min(heads, h0 + kHeads * steps);
     if (m >= bt.M || m >= bt.q_start[bt.n_seqs] || m < bt.q_start[0]) return;
+    // The first heads' elements are asked for before it is known where the row belongs.
+    float x[kHeads][E];
+    const float* src = qkv + (size_t)m * ldqkv + lane * E;
+#pragma unroll
+    for (int i = 0; i < kHeads; i++) load_vec(x[i], src + (size_t)min(h0 + i, heads - 1) * HD, true);
     // largest s with q_start[s] <= m: every lane tests one splitter per round
     int lo = 0, hi = bt.n_seqs;
     while (hi - lo > 1) {
@@ -80,74 +103,80 @@ __global__ void __launch_bounds__(kAppendThreads) append_kernel(
     const int page = slot >= 0 && slot < sq.len ? bt.page(lo, slot) : -1;
     const long long at = page >= 0 ? page * pg.page + (slot & ((1 << bt.page_shift) - 1)) * pg.row : 0;
 
-    float x[kHeads][E];
-    const float* src = qkv + (size_t)m * ldqkv + lane * E;
-#pragma unroll
-    for (int i = 0; i < kHeads; i++) {
-        if (h0 + i >= heads) break;
-        const float* p = src + (size_t)(h0 + i) * HD;
-        if constexpr (E == 4) {
-            const float4 v = *reinterpret_cast<const float4*>(p);
-            x[i][0] = v.x, x[i][1] = v.y, x[i][2] = v.z, x[i][3] = v.w;
-        } else {
-            const float2 v = *reinterpret_cast<const float2*>(p);
-            x[i][0] = v.x, x[i][1] = v.y;
-        }
-    }
-    // angle index of element j: pairs (2i, 2i+1), or i and i + HD/2
+    // angle of element j: that of the pair (2i, 2i+1), or (i, i + HD/2)
     float c[E], sn[E];
+    const float *ct = cos_tab + (size_t)pos * (HD / 2), *st = sin_tab + (size_t)pos * (HD / 2);
+    if (rope_style == 0) {
 #pragma unroll
-    for (int j = 0; j < E; j++) {
-        const int e = lane * E + j, i = rope_style == 0 ? e >> 1 : e & (HD / 2 - 1);
-        c[j] = cos_tab[(size_t)pos * (HD / 2) + i];
-        sn[j] = sin_tab[(size_t)pos * (HD / 2) + i];
+        for (int j = 0; j < E; j += 2) {
+            c[j] = c[j + 1] = ct[(lane * E + j) >> 1];
+            sn[j] = sn[j + 1] = st[(lane * E + j) >> 1];
+        }
+    } else {
+        load_vec(c, ct + (lane * E & (HD / 2 - 1)), aligned);
+        load_vec(sn, st + (lane * E & (HD / 2 - 1)), aligned);
     }
+    float wq[E], wk[E];
 #pragma unroll
-    for (int i = 0; i < kHeads; i++) {
-        const int h = h0 + i;
-        if (h >= heads) break;
-        const bool is_q = h < nq, is_v = h >= nq + nkv;
-        if (!is_v) {
-            const float* w = is_q ? q_norm_w : k_norm_w;
-            if (w) {
-                float ss = 0.f;
+    for (int j = 0; j < E; j++) wq[j] = wk[j] = 1.f;
+    if (q_norm_w && h0 < nq) load_vec(wq, q_norm_w + lane * E, aligned);
+    if (k_norm_w && h_end > nq && h0 < nq + nkv) load_vec(wk, k_norm_w + lane * E, aligned);
+    for (; h0 < h_end; h0 += kHeads) {
+        float nx[kHeads][E];  // the heads after these
+        if (h0 + kHeads < h_end) {
 #pragma unroll
-                for (int j = 0; j < E; j++) ss = fmaf(x[i][j], x[i][j], ss);
-                const float r = 1.0f / sqrtf(b2::warp_sum(ss) / (float)HD + eps);
+            for (int i = 0; i < kHeads; i++) load_vec(nx[i], src + (size_t)min(h0 + kHeads + i, heads - 1) * HD, true);
+        }
 #pragma unroll
-                for (int j = 0; j < E; j++) x[i][j] = (x[i][j] * r) * w[lane * E + j];
-            }
-            if (rope_style == 0) {
+        for (int i = 0; i < kHeads; i++) {
+            const int h = h0 + i;
+            if (h >= h_end) break;
+            const bool is_q = h < nq, is_v = h >= nq + nkv;
+            if (!is_v) {
+                if (is_q ? q_norm_w : k_norm_w) {
+                    float ss = 0.f;
 #pragma unroll
-                for (int j = 0; j < E; j += 2) {
-                    const float a = x[i][j], b = x[i][j + 1];
-                    x[i][j] = a * c[j] - b * sn[j];
-                    x[i][j + 1] = b * c[j] + a * sn[j];
+                    for (int j = 0; j < E; j++) ss = fmaf(x[i][j], x[i][j], ss);
+                    const float r = 1.0f / sqrtf(b2::warp_sum(ss) / (float)HD + eps);
+#pragma unroll
+                    for (int j = 0; j < E; j++) x[i][j] = (x[i][j] * r) * (is_q ? wq[j] : wk[j]);
                 }
+                if (rope_style == 0) {
+#pragma unroll
+                    for (int j = 0; j < E; j += 2) {
+                        const float a = x[i][j], b = x[i][j + 1];
+                        x[i][j] = a * c[j] - b * sn[j];
+                        x[i][j + 1] = b * c[j] + a * sn[j];
+                    }
+                } else {
+#pragma unroll
+                    for (int j = 0; j < E; j++) {
+                        const float o = __shfl_xor_sync(0xffffffffu, x[i][j], 16);
+                        x[i][j] = lane < 16 ? x[i][j] * c[j] - o * sn[j] : x[i][j] * c[j] + o * sn[j];
+                    }
+                }
+            }
+            __half* dst;
+            if (is_q) {
+                dst = q16 + (size_t)m * ldq + (size_t)h * HD;
             } else {
-#pragma unroll
-                for (int j = 0; j < E; j++) {
-                    const float o = __shfl_xor_sync(0xffffffffu, x[i][j], 16);
-                    x[i][j] = lane < 16 ? x[i][j] * c[j] - o * sn[j] : x[i][j] * c[j] + o * sn[j];
-                }
+                if (page < 0) continue;
+                const int g = is_v ? h - nq - nkv : h - nq;
+                dst = reinterpret_cast<__half*>(is_v ? pg.v : pg.k) + at + g * pg.head;
+            }
+            if constexpr (E == 4) {
+                uint2 u;
+                u.x = b2p::pack_h2(x[i][0], x[i][1]);
+                u.y = b2p::pack_h2(x[i][2], x[i][3]);
+                *reinterpret_cast<uint2*>(dst + lane * E) = u;
+            } else {
+                *reinterpret_cast<uint32_t*>(dst + lane * E) = b2p::pack_h2(x[i][0], x[i][1]);
             }
         }
-        __half* dst;
-        if (is_q) {
-            dst = q16 + (size_t)m * ldq + (size_t)h * HD;
-        } else {
-            if (page < 0) continue;
-            const int g = is_v ? h - nq - nkv : h - nq;
-            dst = reinterpret_cast<__half*>(is_v ? pg.v : pg.k) + at + g * pg.head;
-        }
-        if constexpr (E == 4) {
-            uint2 u;
-            u.x = b2p::pack_h2(x[i][0], x[i][1]);
-            u.y = b2p::pack_h2(x[i][2], x[i][3]);
-            *reinterpret_cast<uint2*>(dst + lane * E) = u;
-        } else {
-            *reinterpret_cast<uint32_t*>(dst + lane * E) = b2p::pack_h2(x[i][0], x[i][1]);
-        }
+#pragma unroll
+        for (int i = 0; i < kHeads; i++)
+#pragma unroll
+            for (int j = 0; j < E; j++) x[i][j] = nx[i][j];
     }
 }
 
@@ -464,14 +493,18 @@ extern "C" int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int
                             "b2_qk_rope_kv_paged: rows must be aligned (qkv 16 bytes, ldqkv %% 4; q16 8 bytes, ldq %% 4) "
                             "and hold every head");
     if (M == 0 || kv->n_seqs == 0) return 0;
-    const long long jobs = (long long)M * ((nq + 2 * nkv + kHeads - 1) / kHeads);
+    const int all = (nq + 2 * nkv + kHeads - 1) / kHeads;
+    const int steps = (long long)M * all > 148 * 64 ? all : 1;  // more than fits the SMs at once
+    const long long jobs = (long long)M * ((all + steps - 1) / steps);
     const long long grid = (jobs + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
     if (grid > 0x7fffffffll) return b2_set_error(B2_ERR_INVALID_ARG, "b2_qk_rope_kv_paged: too many rows");
     const PageStrides pg{kv->k_pages, kv->v_pages, kv->page_stride, kv->head_stride, kv->row_stride};
+    const bool aligned = ((reinterpret_cast<uintptr_t>(cos_tab) | reinterpret_cast<uintptr_t>(sin_tab) |
+                           reinterpret_cast<uintptr_t>(q_norm_w) | reinterpret_cast<uintptr_t>(k_norm_w)) & 15) == 0;
     const cudaError_t e =
         b2::launch_pdl(hd == 128 ? append_kernel<128> : append_kernel<64>, dim3((unsigned)grid), dim3(kAppendThreads), 0,
                        (cudaStream_t)s, reinterpret_cast<__half*>(q16), ldq, qkv, ldqkv, nq, nkv, q_norm_w, k_norm_w,
-                       eps, cos_tab, sin_tab, max_pos, rope_style, pos, b2p::make_batch(kv, M), pg);
+                       eps, cos_tab, sin_tab, max_pos, rope_style, pos, b2p::make_batch(kv, M), pg, aligned, steps);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_qk_rope_kv_paged: %s", cudaGetErrorString(e));
     return 0;
 }

@@ -31,16 +31,17 @@ struct WeightParams {
 
 // ─── few rows per sequence ───
 //
-// Bound by reading K once.  A warp owns 16 slots: S = K Q^T on mma m16n8k16
-// with the slots as M rows and eight (token, head) rows as N columns.  The dims
-// of the sum may go in any order as long as K and Q agree, so a lane takes 16
-// consecutive bytes of its row for two k steps and the fragments come straight
-// from global memory, a row's four lanes reading 64 consecutive bytes.
+// Bound by reading K once.  A warp owns 32 slots, two groups of 16: S = K Q^T on
+// mma m16n8k16 with the slots as M rows and eight (token, head) rows as N columns.
+// The dims of the sum may go in any order as long as K and Q agree, so a lane takes
+// 16 consecutive bytes of its row for two k steps and the fragments come straight
+// from global memory, a row's four lanes reading 64 consecutive bytes.  Everything
+// a block needs is asked for before any of it is used.
 constexpr int kThreads = 128;
-constexpr int kBlk = 64;
+constexpr int kBlk = 128;
 
 template <int HD>
-__global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightParams p) {
+__global__ void __launch_bounds__(kThreads, 4) weights_short_kernel(const WeightParams p) {
     __shared__ int pre[B2_PAGED_MAX_SEQS + 1];
     b2::pdl_trigger();
     // Behind the long kernel this grid starts once that one's CTAs have seen the
@@ -53,25 +54,33 @@ __global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightPar
     });
     const int W = pre[p.bt.n_seqs];
     const float scale = kLog2e / sqrtf((float)HD);
+    const int slot_mask = (1 << p.bt.page_shift) - 1;
     for (int x = blockIdx.x; x < W; x += gridDim.x) {
         const int s = prefix_find(pre, p.bt.n_seqs, x);
         const Seq sq = p.bt.seq(s);
-        const int nb = (sq.len + kBlk - 1) / kBlk, g = (x - pre[s]) / nb, j0 = (x - pre[s]) % nb * kBlk + warp * 16;
+        const int nb = cdiv(sq.len, kBlk), g = (x - pre[s]) / nb, j0 = (x - pre[s]) % nb * kBlk + warp * 32;
         if (j0 >= sq.len) continue;
-        const int page = p.bt.page(s, j0);
         const int rows = min(sq.Q, p.max_q) * p.G;
-        const int ja = j0 + n, jb = ja + 8;
-        float acc[2] = {0.f, 0.f};
         // first row that may see a slot of this warp, down to a column tile's start
         const int r_first = max(0, j0 - sq.base) * p.G / 8 * 8;
-        if (page >= 0 && r_first < rows) {
-            const uint16_t* kp = p.k + page * p.page_stride + g * p.head_stride +
-                                 (long long)((j0 & ((1 << p.bt.page_shift) - 1)) + n) * p.row_stride + 8 * c4;
-            uint4 a[2][HD / 32];
+        const size_t o = ((size_t)s * p.nkv + g) * p.ldw + j0 + lane;
+        const bool out = j0 + lane < sq.len && j0 + lane < p.ldw;
+        const float was = out && p.prev ? p.prev[o] : 0.f;  // lane = slot
+        int page[2];
 #pragma unroll
-            for (int u = 0; u < HD / 32; u++) {
-                a[0][u] = b2::ld_stream16(kp + 32 * u);
-                a[1][u] = b2::ld_stream16(kp + 8 * p.row_stride + 32 * u);
+        for (int t = 0; t < 2; t++) page[t] = j0 + 16 * t < sq.len ? p.bt.page(s, j0 + 16 * t) : -1;
+        float acc[2][2] = {{0.f, 0.f}, {0.f, 0.f}};
+        if (r_first < rows && (page[0] >= 0 || page[1] >= 0)) {
+            uint4 a[2][2][HD / 32];
+#pragma unroll
+            for (int t = 0; t < 2; t++) {
+                const uint16_t* kp = p.k + max(page[t], 0) * p.page_stride + g * p.head_stride +
+                                     (long long)(((j0 + 16 * t) & slot_mask) + n) * p.row_stride + 8 * c4;
+#pragma unroll
+                for (int u = 0; u < HD / 32; u++) {
+                    a[t][0][u] = page[t] >= 0 ? b2::ld_stream16(kp + 32 * u) : make_uint4(0, 0, 0, 0);
+                    a[t][1][u] = page[t] >= 0 ? b2::ld_stream16(kp + 8 * p.row_stride + 32 * u) : make_uint4(0, 0, 0, 0);
+                }
             }
             for (int r0 = r_first; r0 < rows; r0 += 8) {
                 const int rq = r0 + n;
@@ -80,40 +89,47 @@ __global__ void __launch_bounds__(kThreads) weights_short_kernel(const WeightPar
 #pragma unroll
                 for (int u = 0; u < HD / 32; u++)
                     b[u] = rq < rows ? *reinterpret_cast<const uint4*>(qp + 32 * u) : make_uint4(0, 0, 0, 0);
-                float l2[2];
-                int lim[2];
+                float l[2];
 #pragma unroll
                 for (int e = 0; e < 2; e++) {
                     const int r = r0 + 2 * c4 + e;
-                    const float l = r < rows ? p.lse[(size_t)(sq.row0 + r / p.G) * p.nq + g * p.G + r % p.G] : -INFINITY;
-                    lim[e] = l == -INFINITY ? -1 : min(sq.len - 1, sq.base + r / p.G);
-                    l2[e] = l * kLog2e;
+                    l[e] = r < rows ? p.lse[(size_t)(sq.row0 + r / p.G) * p.nq + g * p.G + r % p.G] : -INFINITY;
                 }
-                float sc[4] = {0.f, 0.f, 0.f, 0.f};
+                __syncwarp();  // no load moves behind this
 #pragma unroll
-                for (int u = 0; u < HD / 32; u++) {
-                    const uint32_t f0[4] = {a[0][u].x, a[1][u].x, a[0][u].y, a[1][u].y};
-                    const uint32_t f1[4] = {a[0][u].z, a[1][u].z, a[0][u].w, a[1][u].w};
-                    mma16816(sc, f0, b[u].x, b[u].y);
-                    mma16816(sc, f1, b[u].z, b[u].w);
-                }
+                for (int t = 0; t < 2; t++) {
+                    float sc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int e = 0; e < 2; e++) {
-                    if (ja <= lim[e]) acc[0] += ex2(fmaf(sc[e], scale, -l2[e]));
-                    if (jb <= lim[e]) acc[1] += ex2(fmaf(sc[e + 2], scale, -l2[e]));
+                    for (int u = 0; u < HD / 32; u++) {
+                        const uint32_t f0[4] = {a[t][0][u].x, a[t][1][u].x, a[t][0][u].y, a[t][1][u].y};
+                        const uint32_t f1[4] = {a[t][0][u].z, a[t][1][u].z, a[t][0][u].w, a[t][1][u].w};
+                        mma16816(sc, f0, b[u].x, b[u].y);
+                        mma16816(sc, f1, b[u].z, b[u].w);
+                    }
+                    const int ja = j0 + 16 * t + n;
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int lim = page[t] < 0 || l[e] == -INFINITY ? -1
+                                                                         : min(sq.len - 1, sq.base + (r0 + 2 * c4 + e) / p.G);
+                        const float l2 = l[e] * kLog2e;
+                        if (ja <= lim) acc[t][0] += ex2(fmaf(sc[e], scale, -l2));
+                        if (ja + 8 <= lim) acc[t][1] += ex2(fmaf(sc[e + 2], scale, -l2));
+                    }
                 }
             }
         }
 #pragma unroll
-        for (int e = 0; e < 2; e++) {
-            acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 1);
-            acc[e] += __shfl_xor_sync(0xffffffffu, acc[e], 2);
-        }
-        const int j = c4 == 0 ? ja : jb;
-        if (c4 < 2 && j < sq.len && j < p.ldw) {
-            const size_t o = ((size_t)s * p.nkv + g) * p.ldw + j;
-            p.weights[o] = (p.prev ? p.prev[o] : 0.f) + (c4 == 0 ? acc[0] : acc[1]);
-        }
+        for (int t = 0; t < 2; t++)
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                acc[t][e] += __shfl_xor_sync(0xffffffffu, acc[t][e], 1);
+                acc[t][e] += __shfl_xor_sync(0xffffffffu, acc[t][e], 2);
+            }
+        // slot j0 + lane: group lane / 16, row lane % 16, held by the lanes of row (lane % 8)
+        const float v00 = __shfl_sync(0xffffffffu, acc[0][0], (lane & 7) * 4), v01 = __shfl_sync(0xffffffffu, acc[0][1], (lane & 7) * 4);
+        const float v10 = __shfl_sync(0xffffffffu, acc[1][0], (lane & 7) * 4), v11 = __shfl_sync(0xffffffffu, acc[1][1], (lane & 7) * 4);
+        const float v = lane < 16 ? (lane < 8 ? v00 : v01) : (lane < 24 ? v10 : v11);
+        if (out) p.weights[o] = was + v;
     }
     if (p.after_long) b2::pdl_wait();
 }
