@@ -577,7 +577,7 @@ extern "C" int b2_attention_paged_weights(float* weights, const float* prev, lon
         if (rc) return rc;
         p.after_long = 1;
     }
-    const long long grid = blocks < sms * 8 ? blocks : sms * 8;
+    const long long grid = blocks < sms * 4 ? blocks : sms * 4;  // what is resident
     const cudaError_t e = b2::launch_pdl(hd == 128 ? weights_short_kernel<128> : weights_short_kernel<64>,
                                          dim3((unsigned)grid), dim3(kThreads), 0, (cudaStream_t)s, p);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged_weights: %s", cudaGetErrorString(e));
