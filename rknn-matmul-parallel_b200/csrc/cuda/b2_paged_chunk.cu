@@ -4,26 +4,32 @@
 //
 // A tile is 128 rows of one kv head: T = 128 / G tokens times the G q heads of
 // its group, so K and V are read once for the whole group.  A CTA works on a
-// pair of tiles (2 T tokens) against blocks of 128 slots:
+// pair of tiles (2 T tokens) against blocks of 64 slots:
 //
 //   warp 8      producer: Q tiles, then K and V blocks by TMA through the page
 //               table into a ring of shared-memory stages; unmapped pages and
 //               pages past kv_len are fetched from outside the tensor, which
 //               fills zeros;
-//   warps 9, 10 the tensor cores for tile 0 and tile 1: S_t = Q_t K^T (128 x 128,
+//   warps 9, 10 the tensor cores for tile 0 and tile 1: S_t = Q_t K^T (128 x 64,
 //               FP32 in tensor memory) and O_t += P_t V with P_t read from tensor
-//               memory.  One warp for both spent 5000 cycles a block on waiting
-//               and issuing in turn, where the products take 2048;
+//               memory;
+//   warp 11     looks for infinities and NaN in V where some rows may not see it;
 //   warps 0-3, 4-7   the softmax of tile 0 and of tile 1, one row per thread:
 //               maximum, exponentials, sum, P_t as FP16 over S_t's columns.
 //
-// While one tile's softmax runs, the tensor cores work on the other tile.  O_t is
+// S_t has two buffers, so that a tile's next scores are there when its softmax has
+// done the block before (blocks of 128 slots with one buffer: 534 us where this takes
+// 512, for 4096 new rows after 12288 at 16 q heads, 8 kv heads, hd 128).  O_t is
 // rescaled only when a row's maximum has grown by more than 2^8 since the last
 // time: until then the weights are taken relative to the older maximum, which
 // changes no result (the sum carries the same factor).
 //
 // Bound by the two products (4 hd FLOP per row and slot) and, at hd 128 just as
-// much, by the exponentials: 16 per clock and SM.
+// much, by the exponentials: 16 per clock and SM.  Those 4096 rows take 491 us,
+// 980 TFLOP/s, 0.59 of a library product's rate; the products and their barriers alone take 468,
+// the softmax without the products 460.  Every fourth exponential by a polynomial
+// instead made it 501: the softmax waits for the order of its steps, not for the
+// exponential unit.
 //
 // The work of the call is one line of blocks, cut into equal stretches for the
 // CTAs; pairs that a cut divides leave pieces (maximum, sum, unnormalised O) in
@@ -37,9 +43,9 @@ namespace {
 using namespace b2p;
 
 constexpr int kBlk = 64;
-// Three warpgroups; the third's last warp only fills it up.  Launched with 168
-// registers a thread; the softmax warpgroups, which hold a row of 128 scores, go to
-// 208 and the third gives them up: 208 + 208 + 88 = 3 x 168.
+// Three warpgroups, launched with 168 registers a thread; those of the softmax, which
+// hold a row's 64 scores and weights, go to 208 and the third gives them up:
+// 208 + 208 + 88 = 3 x 168.
 constexpr int kThreads = 384;
 constexpr int kMaxItems = 2048;  // entries of the line's prefix in shared memory
 constexpr int kMinBlocks = 4;    // shortest stretch of a CTA
@@ -70,6 +76,9 @@ struct Smem {
     uint64_t o_free[2], drain[2];
     uint32_t tmem;
     int failed;
+    int issued;      // blocks that the producer has asked for
+    int skip[2][2];  // [tile][buffer]: block count of a block whose product with V the softmax did itself
+    unsigned last_bad[16];  // entry (block count % 16): the count, and 1 + the last slot whose V is not finite
     int mapped[16];  // bit w of entry (block count % 16): slots 16 w .. 16 w + 15 are mapped
     int pre_seq[B2_PAGED_MAX_SEQS + 1];
     int pre[kMaxItems + 1];
@@ -93,6 +102,11 @@ struct LongParams {
     int T;      // tokens of one tile
     int group;  // tile pairs of one entry of the line's prefix
 };
+
+// Slots that every row of tile t sees, as far as they are mapped: those of its first token.
+__device__ __forceinline__ int seen_by_all(const LongParams& p, const Seg& g, int t) {
+    return max(0, min(g.sq.len, g.sq.base + g.i0 + t * p.T + 1));
+}
 
 // Tile pairs of a sequence (none when the short kernel takes it) and the blocks
 // that its pair t reaches.
@@ -165,6 +179,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             mbar_init(&sm.o_free[t], 4);
         }
         sm.failed = 0;
+        sm.issued = 0;
+        for (int i = 0; i < 4; i++) sm.skip[i >> 1][i & 1] = -1;
+        for (int i = 0; i < 16; i++) sm.last_bad[i] = ~0u;
         mbar_init_fence();
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tq) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
@@ -246,6 +263,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int w = 0; w < kBlk / 16; w++) bits |= (have >> (w * 16 / box_rows) & 1) << w;
                         sm.mapped[n & 15] = bits;
                         mbar_expect_tx(&sm.full[st], 2 * C::kTile);
+                        *(volatile int*)&sm.issued = n + 1;
                     }
                     __syncwarp();
                     if (lane < 2 * per_kv)
@@ -292,6 +310,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                 const Seg g = find_seg<HD>(p, sm, items, x, x1);
                 x = uniform(x + g.b1 - g.b0);
                 const int b0 = uniform(g.b0), live = uniform(g.live(t)), e = uniform(g.end());
+                const int edge_from = uniform(seen_by_all(p, g, t)) / kBlk;
                 if (e <= b0) continue;
                 if (!wait(&sm.q_full, seg & 1)) break;
                 seg++;
@@ -315,8 +334,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                         const uint64_t v = dv + st * (2 * C::kTile >> 4);
                         if (B2_RARE(!wait(&sm.p_ready[t][np & 1], (np >> 1) & 1))) break;
                         const uint32_t pt = ts + 64 * (np & 1);
+                        const bool skip = B2_RARE(b >= edge_from) && *(volatile int*)&sm.skip[t][np & 1] == k;
 #pragma unroll
-                        for (int i = 0; i < kBlk / 16; i++)
+                        for (int i = 0; i < kBlk / 16 && !skip; i++)
                             umma_ts(to, pt + 8 * i, v + i * (2048 >> 4), id_o, !first || i > 0, lead);
                         umma_commit(&sm.o_done[t][np & 1], lead);
                         np++;
@@ -328,6 +348,38 @@ __global__ void __launch_bounds__(kThreads, 1)
                 umma_commit(&sm.drain[t], lead);
                 for (int it = 0; it <= kWaitLimit; it++)
                     if (mbar_try_wait(&sm.drain[t], 0)) break;
+            }
+        } else {
+            // ── the last slot of each block that some rows may not see whose V is not finite ──
+            // (a stage of such a block is not given back before the softmax has this)
+            int n = 0;
+            for (int x = x0; x < x1 && ok;) {
+                const Seg g = find_seg<HD>(p, sm, items, x, x1);
+                x += g.b1 - g.b0;
+                const int e = uniform(g.end()), b0 = uniform(g.b0), len = uniform(g.sq.len);
+                const int seen_all = uniform(seen_by_all(p, g, 0));
+                for (int b = max(b0, seen_all / kBlk); b < e && b * kBlk < len; b++) {
+                    const int k = n + b - b0, from = max(0, seen_all - b * kBlk), to = min(kBlk, len - b * kBlk);
+                    // This warp waits for few of a stage's phases, so it first has to know that the one it
+                    // means has begun.  (The limit starts again with every block: it may be far away.)
+                    for (int it = 0, was = 0, now; (now = *(volatile int*)&sm.issued) <= k && ok; it++) {
+                        if (now != was) was = now, it = 0;
+                        if (it > kWaitLimit || *failed) *failed = 1, ok = false;
+                        __nanosleep(32);
+                    }
+                    ok = __all_sync(0xffffffffu, ok) && warp_wait(&sm.full[k % C::kStages], (k / C::kStages) & 1, failed);
+                    if (!ok) break;
+                    const unsigned char* v = sm.ring[k % C::kStages][1];
+                    int last = 0;  // slot + 1
+#pragma unroll 4
+                    for (int i = from * (HD / 8) + lane; i < to * (HD / 8); i += 32)
+                        if (non_finite8(*reinterpret_cast<const uint4*>(v + (i % (HD / 8) >> 3) * C::kHalf +
+                                                                        i / (HD / 8) * 128 + (i & 7) * 16)))
+                            last = i / (HD / 8) + 1;
+                    last = __reduce_max_sync(0xffffffffu, last);
+                    if (lane == 0) *(volatile unsigned*)&sm.last_bad[k & 15] = (unsigned)k << 8 | (unsigned)last;
+                }
+                n += max(0, e - b0);
             }
         }
     } else {
@@ -359,21 +411,22 @@ __global__ void __launch_bounds__(kThreads, 1)
             };
             if (first < last) load_s(ns);
             if (!ok) break;
-            // blocks from here on hold slots that some row of the warp does not see, or that are not
+            // blocks from here on hold slots that some row of the tile does not see, or that are not
             // cached (whose V rows the four warps zero together)
-            const int edge_from = __reduce_min_sync(0xffffffffu, live ? max(lim + 1, 0) : len) / kBlk;
+            const int seen_all = uniform(seen_by_all(p, g, t)), edge_from = seen_all / kBlk;
             const uint64_t scale2 = pack_f2(scale, scale);
             // One block; edge: with slots that are not seen.  Two copies, because a path beside the common
             // one costs that one a fifth of its time even where it is not taken.
             auto step = [&](auto edge, int b, int bits) {
                 const int j0 = b * kBlk, n = nblk + (b - first);
                 const uint32_t ts = s0 + 64 * (ns & 1);
+                uint32_t lo = 0, hi = 0;  // bit c of the pair: the row sees slot j0 + c
+                bool by_hand = false;
                 tmem_wait_ld();
                 if constexpr (decltype(edge)::value) {
-                    // bit c of the pair: the row sees slot j0 + c
                     const int seen = lim - j0 + 1;
-                    uint32_t lo = (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
-                    uint32_t hi = (bits & 4 ? 0xffffu : 0u) | (bits & 8 ? 0xffff0000u : 0u);
+                    lo = (bits & 1 ? 0xffffu : 0u) | (bits & 2 ? 0xffff0000u : 0u);
+                    hi = (bits & 4 ? 0xffffu : 0u) | (bits & 8 ? 0xffff0000u : 0u);
                     if (seen < 32) lo &= (1u << max(seen, 0)) - 1;
                     if (seen < 64) hi &= (1u << max(seen - 32, 0)) - 1;
 #pragma unroll
@@ -389,6 +442,16 @@ __global__ void __launch_bounds__(kThreads, 1)
                                 make_uint4(0, 0, 0, 0);
                         }
                         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    }
+                    // An infinite or NaN V at a slot that some row does not see would reach that row
+                    // too (0 x inf): such a block is summed by its rows themselves.
+                    // (This costs 1 us of 23 with 8 x 60 rows, 5 of 491 with 4096 rows.)
+                    if (b >= edge_from && j0 < len) {
+                        unsigned w = 0;
+                        for (int it = 0; ok && ((w = *(volatile unsigned*)&sm.last_bad[n & 15]) >> 8) != (n & 0xffffffu); it++)
+                            if (it > kWaitLimit || *failed) *failed = 1, ok = false;
+                        ok = __all_sync(0xffffffffu, ok);
+                        by_hand = ok && uniform((int)(w & 255)) > max(0, seen_all - j0);
                     }
                 }
                 float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
@@ -430,6 +493,49 @@ __global__ void __launch_bounds__(kThreads, 1)
                     pk[i] = pack_h2(x, y);
                 }
                 tmem_st32(ts, pk);
+                if constexpr (decltype(edge)::value) {
+                    if (B2_RARE(by_hand)) {
+                        tmem_wait_st();
+                        if (b > first) {
+                            ok = ok && warp_wait(&sm.o_done[t][(ns - 1) & 1], ((ns - 1) >> 1) & 1, failed);
+                            tc_fence_after();
+                        }
+                        const unsigned char* v = sm.ring[n % C::kStages][1];
+#pragma unroll 1
+                        for (int c = 0; c < HD && ok; c += 32) {
+                            uint32_t ov[32];
+#pragma unroll
+                            for (int i = 0; i < 32; i++) ov[i] = 0u;
+                            if (b > first) {
+                                tmem_ld32<0>(to + c, ov);
+                                tmem_wait_ld();
+                            }
+#pragma unroll 1
+                            for (int s = 0; s < kBlk; s++) {
+                                __syncwarp();
+                                const uint32_t w = tmem_ld1(ts + s / 2);
+                                tmem_wait_ld();
+                                const float ps = __half2float(__ushort_as_half((unsigned short)(s & 1 ? w >> 16 : w)));
+                                const bool see = (s < 32 ? lo : hi) >> (s & 31) & 1;
+#pragma unroll
+                                for (int i = 0; i < 4; i++) {
+                                    const uint4 u = *reinterpret_cast<const uint4*>(
+                                        v + (c >> 6) * C::kHalf + s * 128 + ((((c & 63) >> 3) + i) ^ (s & 7)) * 16);
+                                    const uint32_t h[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+                                    for (int e = 0; e < 8; e++) {
+                                        const float x = __half2float(
+                                            __ushort_as_half((unsigned short)(e & 1 ? h[e / 2] >> 16 : h[e / 2])));
+                                        if (see) ov[8 * i + e] = __float_as_uint(fmaf(ps, x, __uint_as_float(ov[8 * i + e])));
+                                    }
+                                }
+                            }
+                            __syncwarp();
+                            tmem_st32(to + c, ov);
+                        }
+                        if ((threadIdx.x & 127) == 0) sm.skip[t][ns & 1] = n;
+                    }
+                }
                 l2 = add_f2(l2, add_f2(add[0], add[1]));
                 if (b + 1 < last) load_s(ns + 1);
                 tmem_wait_st();

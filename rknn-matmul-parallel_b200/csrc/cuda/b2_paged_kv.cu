@@ -48,7 +48,8 @@ struct PageStrides {
 // squares across the warp.  Bound by HBM: 4 bytes read and 2 written per
 // element.  A warp takes `steps` times kHeads heads of one row, kHeads at a time
 // and the next ones on their way: with many rows a whole row, so that its place
-// and angles are looked up once, with few rows kHeads, so that there are warps.
+// and angles are looked up once, with few rows kHeads, so that there are warps.  7600 rows of 32
+// heads, hd 128: 41 us, 0.70 of the measured copy rate; 64 rows: 4.5.
 constexpr int kAppendThreads = 128;
 constexpr int kHeads = 4;
 
@@ -437,7 +438,9 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
 }
 
 // Moves the kept rows: 16 bytes per thread, K and V of a row by neighbouring
-// threads, four rows in flight per thread.  Bound by HBM.
+// threads, four rows in flight per thread.  Bound by HBM: 16 x 8 heads of 1024 rows
+// take about 20 us (134 MB moved: 1.0 of the measured copy rate), one context of 20
+// thousand rows 27 (164 MB, 0.92).
 constexpr int kMoveThreads = 256;
 constexpr int kMoveRows = 4;
 
@@ -487,7 +490,7 @@ extern "C" int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int
     if (rc) return rc;
     if (!q16 || !qkv || !cos_tab || !sin_tab || M < 0 || nq <= 0 || max_pos <= 0 || (rope_style != 0 && rope_style != 1))
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_qk_rope_kv_paged: bad arguments");
-    if (ldqkv < (nq + 2 * nkv) * hd || ldq < nq * hd || ldqkv % 4 || ldq % 4 ||
+    if (ldqkv < (nq + 2ll * nkv) * hd || ldq < (long long)nq * hd || ldqkv % 4 || ldq % 4 ||
         (reinterpret_cast<uintptr_t>(qkv) & 15) || (reinterpret_cast<uintptr_t>(q16) & 7))
         return b2_set_error(B2_ERR_INVALID_ARG,
                             "b2_qk_rope_kv_paged: rows must be aligned (qkv 16 bytes, ldqkv %% 4; q16 8 bytes, ldq %% 4) "

@@ -16,8 +16,7 @@ __device__ __forceinline__ void tmem_free512(uint32_t tmem) {
 }
 // The issuing warp runs converged and `lead` (one lane, always the same) issues:
 // with a divergent branch around them every operand would go through a vector
-// register first, which took longer than the product (a 128 x 128 x 128 product
-// was issued in 900 cycles that the tensor cores finish in 512).
+// register first (4096 new rows after 12288: 555 us with it, 534 without).
 __device__ __forceinline__ void umma_commit(uint64_t* bar, uint32_t lead) {
     asm volatile(
         "{\n .reg .pred q;\n setp.ne.b32 q, %1, 0;\n @q "
@@ -103,6 +102,40 @@ __device__ __forceinline__ uint64_t add_f2(uint64_t a, uint64_t b) {
     uint64_t d;
     asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
+}
+__device__ __forceinline__ uint64_t mul_f2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+// (2^x, 2^y) without the exponential unit: x = n + f with n whole and |f| <= 1/2
+// (adding 1.5 2^23 rounds to whole numbers), 2^f by the polynomial of degree 5 of
+// least relative error (7.5e-8 before rounding, 2.1e-7 with FP32 arithmetic; fitted
+// by the Remez exchange), and 2^n from its exponent field,
+// which is 0 from n = -127 down and infinity from 128 up.  NaN gives NaN.
+__device__ __forceinline__ uint64_t ex2_f2(float x, float y) {
+    asm("{max.NaN.f32 %0, %0, %2; max.NaN.f32 %1, %1, %2; min.NaN.f32 %0, %0, %3; min.NaN.f32 %1, %1, %3;}"
+        : "+f"(x), "+f"(y)
+        : "f"(-127.f), "f"(128.f));
+    const uint64_t v = pack_f2(x, y), magic = pack_f2(12582912.f, 12582912.f);
+    const uint64_t r = add_f2(v, magic), n = add_f2(r, pack_f2(-12582912.f, -12582912.f));
+    const uint64_t f = fma_f2(n, pack_f2(-1.f, -1.f), v);
+    auto both = [](float c) { return pack_f2(c, c); };
+    uint64_t p = fma_f2(both(0x1.5c08e6p-10f), f, both(0x1.3d0c52p-7f));
+    p = fma_f2(p, f, both(0x1.c6b6e4p-5f));
+    p = fma_f2(p, f, both(0x1.ebf918p-3f));
+    p = fma_f2(p, f, both(0x1.62e428p-1f));
+    p = fma_f2(p, f, both(0x1.000002p+0f));
+    float a, b;
+    unpack_f2(r, a, b);
+    return mul_f2(p, pack_f2(__uint_as_float((__float_as_uint(a) << 23) + 0x3f800000u),
+                             __uint_as_float((__float_as_uint(b) << 23) + 0x3f800000u)));
+}
+// One column of a warp's 32 lanes.
+__device__ __forceinline__ uint32_t tmem_ld1(uint32_t addr) {
+    uint32_t v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x1.b32 {%0}, [%1];" : "=r"(v) : "r"(addr) : "memory");
+    return v;
 }
 // max of three (a NaN loses).
 __device__ __forceinline__ float max3(float a, float b, float c) {

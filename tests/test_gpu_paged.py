@@ -646,3 +646,208 @@ def test_serving_loop():
                 assert bool(((K[:, h] - kept_rows[s][h]).abs() <= U * kept_rows[s][h].abs() + 2.0 ** -18).all())
             pos[s] += news[s]
     assert err.item() == 0
+
+
+# ── what one row may see and another may not, and sizes past the usual ──
+
+
+@pytest.mark.parametrize("nq,nkv,hd,page", [(4, 2, 128, 64), (2, 2, 64, 16), (16, 1, 128, 32), (3, 1, 64, 128)])
+@pytest.mark.parametrize("q", [2, 5, 16, 40, 140, 300])
+def test_attention_non_finite_values_of_later_rows(nq, nkv, hd, page, q):
+    """An infinite or NaN V (an overflow in the cache) reaches the rows that see it, in its column of its kv head,
+    and no row before it."""
+    G = nq // nkv
+    seqs = [(q, 200 + q, ()), (q, q, ()), (q, q + 31, (0,)), (1, 80, ())]
+    b = Paged(seqs, nq, nkv, hd, page, seed=q)
+    hit = torch.zeros(b.M, nq, hd, dtype=torch.bool, device=DEV)
+    clean, _ = b.attend()
+    kept = b.v.clone()
+    for s, row, d, bad in [(0, 1, 3, math.inf), (0, q - 1, 3, -math.inf), (0, q // 2, hd - 1, math.nan),
+                           (1, 0, 9, math.inf), (1, q - 1, 10, math.nan), (2, q // 3, 0, -math.inf), (3, 0, 1, math.nan)]:
+        j, h = seqs[s][1] - seqs[s][0] + row, (row + d) % nkv
+        if j // page in seqs[s][2]:
+            continue
+        b.v[b.table[s, j // page], h, j % page, d] = bad
+        a = int(b.starts[s])
+        hit[a + row:a + seqs[s][0], h * G:(h + 1) * G, d] = True
+    out, lse = b.attend()
+    b.v.copy_(kept)
+    hit = hit.view(b.M, -1)
+    assert not bool(out[hit].isfinite().any()) and bool(out[~hit].isfinite().all())
+    check_attention(b, torch.where(hit, clean, out), lse)
+
+
+@pytest.mark.parametrize("q", [1, 6, 40, 140, 300])
+def test_weights_non_finite_keys(q):
+    """K that is not finite at one slot gives that slot's weight, and no other's, whoever sees it."""
+    b = Paged([(q, 180 + q, ()), (q, q + 5, ())], 4, 2, 128, 64, seed=q)
+    _, lse = b.attend()
+    ldw = 200 + q
+    out = b.weigh(lse, None, torch.zeros(2, 2, ldw, device=DEV))
+    check_weights(b, lse, None, out, ldw, 0.0)
+    where = [(0, 0, 180 + q // 2), (1, 1, q + 4), (0, 1, 17)]
+    for s, h, j in where:
+        b.k[b.table[s, j // 64], h, j % 64, 5] = math.nan
+    got = b.weigh(lse, None, torch.zeros(2, 2, ldw, device=DEV))
+    for s, h, j in where:
+        assert math.isnan(got[s, h, j].item())
+        got[s, h, j] = out[s, h, j]
+    assert torch.equal(got, out)
+
+
+def test_weights_of_rows_without_weight():
+    """Rows whose lse is -infinity give exactly nothing, whatever their scores."""
+    b = Paged([(150, 400, ()), (3, 200, ())], 4, 2, 64, 32, seed=2)
+    none = torch.full((b.M, b.nq), -math.inf, device=DEV)
+    out = b.weigh(none, None, torch.full((2, 2, 400), 7.0, device=DEV))
+    assert not bool(out[0].any()) and not bool(out[1, :, :200].any())
+
+
+@pytest.mark.parametrize("G,seqs_n,q", [(16, 100, 400), (8, 900, 33), (1, 1, 2500)])
+def test_attention_many_chunks(G, seqs_n, q):
+    """More tiles than the chunk kernel keeps places for, many sequences of chunks, one head of its own."""
+    b = Paged([(q, q + (s * 7) % 50, ()) for s in range(seqs_n)], G, 1, 64, 64, seed=G)
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    prev = torch.rand(seqs_n, 1, q + 50, device=DEV)
+    w = b.weigh(lse, prev, prev.clone())
+    for s in range(0, seqs_n, 37):  # every row gives each of its heads one
+        n = b.seqs[s][1]
+        given = (w - prev)[s, 0, :n].to(F64).sum() / (q * G)
+        assert abs(float(given) - 1) < 2.0 ** -10
+
+
+@pytest.mark.parametrize("seqs_n,n", [(150, 60_000), (1, 400_000)])
+def test_evict_more_slots_than_fit(seqs_n, n):
+    """More slots than the CTAs of one kv head hold keys for."""
+    page, budget = 128, 5000
+    per = -(-budget // page)
+    b = Paged([(0, n, ())] + [(0, 40 + s, ()) for s in range(seqs_n - 1)], 1, 1, 64, page, seed=1,
+              extra_pages=per * seqs_n + 1)
+    dst = torch.tensor(b.spare[:per * seqs_n], dtype=torch.int32, device=DEV).view(seqs_n, per)
+    w = (torch.rand(seqs_n, 1, n, device=DEV) * 1000).floor()
+    kept, dw, got = evict(b, w, budget, 3, 500, dst)
+    for s, heads in enumerate(evict_reference(b, w, budget, 3, 500)):
+        assert kept[s, 0, :int(got[s])].tolist() == heads[0]
+        j = torch.tensor(heads[0], device=DEV)
+        to = torch.arange(len(j), device=DEV)
+        assert torch.equal(dw[s, 0, :len(j)], w[s, 0, j])
+        assert torch.equal(b.k[dst[s, to // page].long(), 0, to % page], b.k[b.table[s, j // page].long(), 0, j % page])
+
+
+@pytest.mark.parametrize("q", [1, 90])
+def test_pages_far_apart(q):
+    """Pages of one layer in a pool whose offsets pass 32 bits."""
+    b = Paged([(q, 300 + q, ()), (q, q + 20, ())], 4, 2, 128, 64, seed=q, extra_pages=20)
+    stride, n = 1 << 28, b.n_pages
+    big = torch.empty(n * stride, dtype=torch.float16, device=DEV)
+    k, v = (big.as_strided((n, 2, 64, 128), (stride, 64 * 128, 128, 1), at) for at in (0, stride // 2))
+    k.copy_(b.k)
+    v.copy_(b.v)
+    assert int(b.table.max()) * stride > 1 << 32  # elements
+    b.k, b.v = k, v
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    w = b.weigh(lse, None, torch.zeros(2, 2, 400, device=DEV))
+    check_weights(b, lse, None, w, 400, 0.0)
+    qkv = torch.randn(b.M, (4 + 2 * 2) * 128, device=DEV)
+    pos = torch.arange(b.M, dtype=torch.int32, device=DEV)
+    cos, sin = torch.ones(b.M, 64, device=DEV), torch.zeros(b.M, 64, device=DEV)
+    bd.check(bd.capi().b2_qk_rope_kv_paged(b.q16.data_ptr(), b.q16.stride(0), qkv.data_ptr(), qkv.stride(0), b.M, 4, 2,
+                                           128, None, None, 1e-6, cos.data_ptr(), sin.data_ptr(), b.M, 0, pos.data_ptr(),
+                                           ctypes.byref(b.kv()), stream()))
+    for s in range(2):
+        for i in (0, q - 1):
+            j, m = b.seqs[s][1] - q + i, int(b.starts[s]) + i
+            at = int(b.table[s, j // 64])
+            assert torch.equal(b.k[at, :, j % 64], qkv[m, 512:768].half().view(2, 128))
+            assert torch.equal(b.v[at, :, j % 64], qkv[m, 768:].half().view(2, 128))
+    dst = torch.tensor(b.spare[:8], dtype=torch.int32, device=DEV).view(2, 4)
+    kept, _, got = evict(b, w, 200, 4, 16, dst)
+    for s in range(2):
+        m = int(got[s])
+        assert m == min(200, b.seqs[s][1])
+        to = torch.arange(m, device=DEV)
+        for h in range(2):
+            j = kept[s, h, :m].long()
+            assert torch.equal(b.v[dst[s, to // 64].long(), h, to % 64], b.v[b.table[s, j // 64].long(), h, j % 64])
+
+
+def test_captured_step():
+    """Append, attention and weights captured as one step and replayed on other rows and lengths, and the eviction
+    after it: what the calls give one by one."""
+    nq, nkv, hd, page = 8, 2, 128, 32
+    b = Paged([(1, 100, ()), (70, 200, ()), (1, 333, ())], nq, nkv, hd, page, seed=3, extra_pages=16)
+    M = b.M
+    qkv = torch.randn(M, (nq + 2 * nkv) * hd, device=DEV)
+    pos = torch.arange(M, dtype=torch.int32, device=DEV)
+    angle = torch.rand(M, hd // 2, device=DEV) * 6
+    cos, sin = angle.cos(), angle.sin()
+    out = torch.zeros(M, nq * hd, dtype=torch.float16, device=DEV)
+    lse = torch.zeros(M, nq, device=DEV)
+    w = torch.zeros(3, nkv, 340, device=DEV)
+    dst = torch.tensor(b.spare[:12], dtype=torch.int32, device=DEV).view(3, 4)
+    kept, moved = torch.zeros(3, nkv, 120, dtype=torch.int32, device=DEV), torch.zeros(3, nkv, 120, device=DEV)
+    new = torch.zeros(3, dtype=torch.int32, device=DEV)
+    kv, L = b.kv(), bd.capi()
+
+    def step():
+        st = torch.cuda.current_stream().cuda_stream
+        bd.check(L.b2_qk_rope_kv_paged(b.q16.data_ptr(), b.q16.stride(0), qkv.data_ptr(), qkv.stride(0), M, nq, nkv, hd,
+                                       None, None, 1e-6, cos.data_ptr(), sin.data_ptr(), M, 1, pos.data_ptr(),
+                                       ctypes.byref(kv), st))
+        bd.check(L.b2_attention_paged(out.data_ptr(), lse.data_ptr(), b.q16.data_ptr(), b.q16.stride(0), M, M, nq, nkv,
+                                      hd, ctypes.byref(kv), b.work.data_ptr(), b.err.data_ptr(), st))
+        bd.check(L.b2_attention_paged_weights(w.data_ptr(), w.data_ptr(), 340, b.q16.data_ptr(), b.q16.stride(0),
+                                              lse.data_ptr(), M, M, nq, nkv, hd, ctypes.byref(kv), b.err.data_ptr(), st))
+        bd.check(L.b2_kv_evict_paged(ctypes.byref(kv), nkv, hd, w.data_ptr(), 340, 120, 4, 16, dst.data_ptr(), 4,
+                                     kept.data_ptr(), moved.data_ptr(), new.data_ptr(), st))
+
+    results = (out, lse, w, kept, moved, new, b.k, b.v)
+    start = [t.clone() for t in results]
+    step()
+    torch.cuda.synchronize()
+    assert b.err.item() == 0
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        step()
+    for news in ([1, 70, 1], [70, 1, 1], [0, 30, 42], [2, 2, 2]):
+        lens = [n + q for n, q in zip((60, 40, 200), news)]
+        b.kv_len.copy_(torch.tensor(lens, dtype=torch.int32))
+        b.q_start.copy_(torch.tensor([0, *np.cumsum(news)], dtype=torch.int32))
+        qkv.copy_(torch.randn(qkv.shape, device=DEV))
+        got = []
+        for run in (step, graph.replay):
+            for t, s in zip(results, start):
+                t.copy_(s)
+            run()
+            torch.cuda.synchronize()
+            got.append([t.clone() for t in results])
+        for a, c in zip(*got):
+            assert torch.equal(a.nan_to_num(9.0), c.nan_to_num(9.0))
+    assert b.err.item() == 0
+
+
+def test_calls_at_once():
+    """Calls with workspaces of their own on two streams, over the same pages."""
+    b = Paged([(1, 900, ()), (200, 700, ()), (1, 50, ()), (9, 300, ())], seed=6)
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    w = b.weigh(lse, None, torch.zeros(4, b.nkv, 900, device=DEV))
+    sides = [torch.cuda.Stream() for _ in range(2)]
+    works = [b.work, torch.zeros_like(b.work)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(4):
+        for st, work in zip(sides, works):
+            with torch.cuda.stream(st):
+                b.work = work
+                o, l = b.attend(st=st.cuda_stream)
+                x = torch.zeros_like(w)
+                bd.check(bd.capi().b2_attention_paged_weights(
+                    x.data_ptr(), None, 900, b.q16.data_ptr(), b.q16.stride(0), l.data_ptr(), b.M, b.max_q, b.nq, b.nkv,
+                    b.hd, ctypes.byref(b.kv()), b.err.data_ptr(), st.cuda_stream))
+                got.append((o, l, x))
+    torch.cuda.synchronize()
+    for o, l, x in got:
+        assert torch.equal(o, out) and torch.equal(l, lse) and torch.equal(x, w)
