@@ -299,7 +299,8 @@ int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq
  * with q16, ldq, max_q and lse as given to and by b2_attention_paged; a row
  * whose lse is -infinity gives nothing.  weights and prev: device FP32
  * [n_seqs][nkv][ldw]; prev may be NULL (zeros) or weights itself.  Slots from
- * kv_len[q] or ldw on are left as they are.  FP32 sums in a fixed order.  err as
+ * kv_len[q] or ldw on are left as they are.  FP32 sums in an order that the shapes of
+ * the call fix.  err as
  * in b2_attention_paged. */
 int b2_attention_paged_weights(float* weights, const float* prev, long long ldw, const uint16_t* q16, int ldq,
                                const float* lse, int M, int max_q, int nq, int nkv, int hd, const B2PagedKV* kv,

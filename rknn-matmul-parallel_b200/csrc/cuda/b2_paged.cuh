@@ -161,23 +161,30 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
 }
 
 // Work of each sequence -> exclusive prefix pre[0..n] (shared memory, n + 1
-// ints), by all threads of the CTA.
+// ints), by all threads of the CTA.  The sums stop at kMaxWork, which the host
+// checks for sequences that share no rows: with any q_start the prefix rises, and
+// a place below pre[n] lies in the work of the sequence that prefix_find gives.
+constexpr unsigned kMaxWork = (1u << 31) - 65536;
+__device__ __forceinline__ unsigned add_sat(unsigned a, unsigned b) {
+    return a + b < a ? ~0u : a + b;
+}
 template <typename F>
 __device__ __forceinline__ void prefix_work(int* pre, int n, F work) {
     for (int s = threadIdx.x; s < n; s += blockDim.x) pre[s + 1] = work(s);
     __syncthreads();
     if (threadIdx.x < 32) {
         const int lane = threadIdx.x;
-        int carry = 0;
+        unsigned carry = 0;
         for (int b = 0; b < n; b += 32) {
-            int v = b + lane < n ? pre[b + lane + 1] : 0;
+            unsigned v = b + lane < n ? (unsigned)pre[b + lane + 1] : 0u;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
-                const int t = __shfl_up_sync(0xffffffffu, v, o);
-                if (lane >= o) v += t;
+                const unsigned t = __shfl_up_sync(0xffffffffu, v, o);
+                if (lane >= o) v = add_sat(v, t);
             }
-            if (b + lane < n) pre[b + lane + 1] = carry + v;
-            carry += __shfl_sync(0xffffffffu, v, 31);
+            v = min(add_sat(carry, v), kMaxWork);
+            if (b + lane < n) pre[b + lane + 1] = (int)v;
+            carry = __shfl_sync(0xffffffffu, v, 31);
         }
         if (lane == 0) pre[0] = 0;
     }

@@ -4,6 +4,8 @@
 //   o_i = sum_j exp(s_ij - m_i) v_j / l_i,   lse_i = m_i + ln l_i,
 // with the running maximum m and sum l of one pass over the slots (the online
 // softmax): a new maximum rescales what was summed before it.
+#include <algorithm>
+
 #include "b2_paged.cuh"
 
 namespace {
@@ -734,7 +736,7 @@ int launch_short(const AttnParams& p, const B2PagedKV* kv, int dev, int sms, lon
     int rc = b2_paged_map(&tk, kv->k_pages, kv, p.nkv, HD, box, HD / 64);
     if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, p.nkv, HD, box, HD / 64);
     if (rc) return rc;
-    long long grid = short_grid<HD, NT>(dev, sms);
+    long long grid = std::min<long long>(short_grid<HD, NT>(dev, sms), kCounterBytes / sizeof(int) / 3);
     if (!p.long_ctas && grid > (blocks + kMinBlocks - 1) / kMinBlocks) grid = (blocks + kMinBlocks - 1) / kMinBlocks;
     e = b2::launch_pdl(attn_short_kernel<HD, NT>, dim3((unsigned)grid), dim3(kThreads), smem, s, tk, tv, p);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged: %s", cudaGetErrorString(e));

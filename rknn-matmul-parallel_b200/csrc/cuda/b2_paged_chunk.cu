@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // only now that they are done.
     b2::pdl_trigger();
     prefix_work(sm.pre_seq, bt.n_seqs, [&](int s) { return cdiv(pairs_of(p, bt.seq(s)), p.group); });
-    const int items = sm.pre_seq[bt.n_seqs];
+    const int items = min(sm.pre_seq[bt.n_seqs], kMaxItems);  // (more only when sequences share rows)
     prefix_work(sm.pre, items, [&](int e) {
         const int s = prefix_find(sm.pre_seq, bt.n_seqs, e);
         const Seq q = bt.seq(s);

@@ -412,11 +412,6 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 uint32_t va[32], vb[32];
                 // 32 columns from c0 on, the next ones on their way
                 auto add = [&](uint32_t (&v)[32], int col) {
-                    if constexpr (decltype(edge)::value) {
-#pragma unroll
-                        for (int c = 0; c < 32; c++)
-                            if (col + c < c0 || col + c >= c1) v[c] = 0xff800000u;  // -inf
-                    }
 #pragma unroll
                     for (int c = 0; c < 32; c += 4) {
                         const float4 n4 = nl[(col + c) / 4];
@@ -426,6 +421,11 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                             unpack_f2(fma_f2(pack_f2(__uint_as_float(v[c + 2 * e]), __uint_as_float(v[c + 2 * e + 1])), scale2,
                                              e ? pack_f2(n4.z, n4.w) : pack_f2(n4.x, n4.y)),
                                       x, y);
+                            if constexpr (decltype(edge)::value) {  // (here, where a row's NaN sum is in it too)
+                                const int r = col + c + 2 * e;
+                                if (r < c0 || r >= c1) x = -INFINITY;
+                                if (r + 1 < c0 || r + 1 >= c1) y = -INFINITY;
+                            }
                             const bool poly = (c / 2 + e) % kPoly == kPoly - 1;
                             acc[e] = add_f2(acc[e], poly ? ex2_f2(x, y) : pack_f2(ex2(x), ex2(y)));
                         }

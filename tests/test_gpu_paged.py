@@ -851,3 +851,42 @@ def test_calls_at_once():
     torch.cuda.synchronize()
     for o, l, x in got:
         assert torch.equal(o, out) and torch.equal(l, lse) and torch.equal(x, w)
+
+
+@pytest.mark.parametrize("q", [2, 6, 40, 140, 300])
+def test_weights_of_a_row_that_is_not_a_number(q):
+    """A row whose sum is NaN or infinite reaches the slots that it sees and no others."""
+    b = Paged([(q, 180 + q, ()), (q, q + 5, ())], 4, 2, 64, 64, seed=q)
+    _, lse = b.attend()
+    ldw = 200 + q
+    out = b.weigh(lse, None, torch.zeros(2, 2, ldw, device=DEV))
+    row = q // 2
+    lse[row, 0] = math.nan                 # sequence 0, kv head 0: slots 0 .. 180 + row
+    lse[int(b.starts[1]) + row, 3] = math.nan  # sequence 1, kv head 1: slots 0 .. 5 + row
+    got = b.weigh(lse, None, torch.zeros(2, 2, ldw, device=DEV))
+    assert bool(got[0, 0, :181 + row].isnan().all()) and bool(got[1, 1, :6 + row].isnan().all())
+    got[0, 0, :181 + row], got[1, 1, :6 + row] = out[0, 0, :181 + row], out[1, 1, :6 + row]
+    assert torch.equal(got, out)
+
+
+@pytest.mark.parametrize("G,q,seqs_n", [(16, 200, 1024), (2, 4, 1024), (2, 9, 64)])
+def test_sequences_that_share_rows(G, q, seqs_n):
+    """Row ranges that are no partition: the first sequence's rows and the caller's memory stay right, and the
+    workspace serves the next call."""
+    one = Paged([(q, 300 + q, ())], G, 1, 64, 64, seed=5)
+    b = Paged([(0, 300 + q, ())] * seqs_n, G, 1, 64, 64, seed=6)
+    b.M, b.rows, b.max_q, b.q16 = one.M, one.rows, q, one.q16
+    b.k, b.v, b.n_pages = one.k, one.v, one.n_pages
+    b.table = one.table.repeat(seqs_n, 1)
+    b.work = torch.zeros_like(b.work)
+    b.q_start = torch.tensor([0, q] * (seqs_n // 2) + [0], dtype=torch.int32, device=DEV)
+    out, lse = b.attend()
+    assert b.err.item() == 0 and not bool(b.work[:4096].any())
+    check_attention(one, out, lse)
+    w = torch.full((seqs_n, 1, 300 + q), 7.0, device=DEV)
+    b.weigh(lse, None, w)
+    # (not bit by bit: how many CTAs share a slot's rows, and so the order of its sum, depends on the batch)
+    check_weights(one, lse, None, w[:1], 300 + q, 7.0)
+    assert not bool(w[1].any())
+    one.work = b.work
+    check_attention(one, *one.attend())
