@@ -278,6 +278,7 @@ int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int
  * -infinity.  max_q: no sequence brings more rows than this (M is always
  * right; a decode step passes 1); a sequence's rows past the first max_q are
  * left as they are.
+ * out16 and lse must not overlap what is read.
  * Sums and the softmax are FP32; the softmax weights are rounded to FP16 for
  * the product with V.  Whatever K and V hold at slots that a row does not see
  * (infinities and NaN too) has no part in the row.
@@ -299,9 +300,8 @@ int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq
  * with q16, ldq, max_q and lse as given to and by b2_attention_paged; a row
  * whose lse is -infinity gives nothing.  weights and prev: device FP32
  * [n_seqs][nkv][ldw]; prev may be NULL (zeros) or weights itself.  Slots from
- * kv_len[q] or ldw on are left as they are.  FP32 sums in an order that the shapes of
- * the call fix.  err as
- * in b2_attention_paged. */
+ * kv_len[q] or ldw on are left as they are.  FP32 sums in an order that the
+ * call's shapes and lengths fix.  err as in b2_attention_paged. */
 int b2_attention_paged_weights(float* weights, const float* prev, long long ldw, const uint16_t* q16, int ldq,
                                const float* lse, int M, int max_q, int nq, int nkv, int hd, const B2PagedKV* kv,
                                int* err, b2_stream_t s);

@@ -192,8 +192,9 @@ __global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(
 // lowest first.  A warp owns a contiguous run of its CTA's slots, 32 at a time, so
 // ballots give the places in slot order and one scan over the warps joins them.
 // The search ends early once all slots that share the digits so far are kept.
-// Bound by latency: 2 to 4 digits of a few microseconds each; 100 thousand slots of
-// 8 heads take 33 us, 4096 slots of 128 (sequence, head) pairs 18 us.
+// Bound by latency: 100 thousand slots of 8 heads take 24 us (the keys and the first
+// digit 8, each other digit 3, the places 7), 4096 slots of 128 (sequence, head)
+// pairs 11.
 constexpr int kBatch = 8;  // groups of 32 slots whose loads a warp has in flight
 constexpr int kMaxKeys = 48 * 1024;  // keys a CTA holds; more are formed again for every digit
 constexpr int kMaxSplit = 8;
@@ -273,14 +274,6 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
         }
     };
     for (int i = tid; i < 2 * 257; i += kSelThreads) (&hist[0][0])[i] = 0;
-    if (cached)
-        for (int q = w0; q < w1; q += kBatch) {
-            uint32_t key[kBatch];
-            make_keys(q, key);
-#pragma unroll
-            for (int e = 0; e < kBatch; e++)
-                if (q + e < w1) keys[(q + e - g0) * 32 + lane] = key[e];
-        }
     __syncthreads();
     uint32_t prefix = 0;  // the digits found so far of the k-th largest key
     int need = 0, k = 0;  // slots still to take among those that share them; slots kept
@@ -291,15 +284,34 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
         int none = 0;
         for (int q = w0; q < w1; q += kBatch) {
             uint32_t keyv[kBatch];
-            get_keys(q, keyv);
+            if (d == 0) {
+                make_keys(q, keyv);
 #pragma unroll
-            for (int e = 0; e < kBatch; e++) {
-                const uint32_t key = keyv[e];
-                const bool in = key != 0 && (d == 0 || (key >> (shift + 8)) == (prefix >> (shift + 8)));
-                if (d == 0) none += q + e < w1 && (q + e) * 32 + lane < len && key == 0;
-                // one addition per distinct digit of the warp: weights share exponents
-                const unsigned same = __match_any_sync(0xffffffffu, in ? (key >> shift) & 255 : 256u);
-                if (in && lane == __ffs(same) - 1) atomicAdd(&h[(key >> shift) & 255], __popc(same));
+                for (int e = 0; e < kBatch; e++) {
+                    const uint32_t key = keyv[e];
+                    if (cached && q + e < w1) keys[(q + e - g0) * 32 + lane] = key;
+                    none += q + e < w1 && (q + e) * 32 + lane < len && key == 0;
+                    // one addition per distinct digit of the warp: weights share exponents
+                    const unsigned same = __match_any_sync(0xffffffffu, key ? key >> 24 : 256u);
+                    if (key && lane == __ffs(same) - 1) atomicAdd(&h[key >> 24], __popc(same));
+                }
+            } else {
+                get_keys(q, keyv);
+#pragma unroll
+                for (int e = 0; e < kBatch; e++) {
+                    const uint32_t key = keyv[e];
+                    const bool in = (key >> (shift + 8)) == (prefix >> (shift + 8)) && key != 0;
+                    const unsigned who = __ballot_sync(0xffffffffu, in);
+                    if (who == 0) continue;
+                    // few slots share a prefix, and their digits differ, unless their weights are equal:
+                    // one addition for the first one's digit, others by themselves
+                    const unsigned dig = (key >> shift) & 255;
+                    const int first = __ffs(who) - 1;
+                    const unsigned lead = __shfl_sync(0xffffffffu, dig, first);
+                    const unsigned same = __ballot_sync(0xffffffffu, in && dig == lead);
+                    if (lane == first) atomicAdd(&h[dig], __popc(same));
+                    else if (in && !(same >> lane & 1)) atomicAdd(&h[dig], 1);
+                }
             }
         }
         if (d == 0) {
@@ -307,15 +319,14 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
             if (lane == 0 && none) atomicAdd(&h[256], none);
         }
         sync_cluster(S);
-        if (tid < 256) {
-            int v = 0;
-            for (int r = 0; r < S; r++) v += S > 1 ? ld_rank(&h[tid], r) : h[tid];
-            sum[tid] = v;
-        }
-        if (d == 0 && tid == 256) {
-            int v = 0;
-            for (int r = 0; r < S; r++) v += S > 1 ? ld_rank(&h[256], r) : h[256];
-            unmapped = v;
+        if (tid < 256 || (d == 0 && tid == 256)) {
+            int v[kMaxSplit];  // every CTA's asked for before any is used
+#pragma unroll
+            for (int r = 0; r < kMaxSplit; r++) v[r] = S == 1 ? (r == 0 ? h[tid] : 0) : r < S ? ld_rank(&h[tid], r) : 0;
+            int all = 0;
+#pragma unroll
+            for (int r = 0; r < kMaxSplit; r++) all += v[r];
+            (tid < 256 ? sum[tid] : unmapped) = all;
         }
         __syncthreads();
         if (d == 0) {
@@ -395,14 +406,10 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
             if (lane == 31) counts[0] = a, counts[1] = b;
         }
         sync_cluster(S);
-        if (tid == 0) {
-            int a = 0, b = 0;
-            for (int r = 0; r < rank; r++) {
-                a += ld_rank(&counts[0], r);
-                b += ld_rank(&counts[1], r);
-            }
-            before[0] = a;
-            before[1] = b;
+        if (warp == 0) {
+            const int a = __reduce_add_sync(0xffffffffu, lane < rank ? ld_rank(&counts[0], lane) : 0);
+            const int b = __reduce_add_sync(0xffffffffu, lane < rank ? ld_rank(&counts[1], lane) : 0);
+            if (lane == 0) before[0] = a, before[1] = b;
         }
         __syncthreads();
         int above = before[0] + warp_gt[warp], equal = before[1] + warp_eq[warp];  // in slots before this group
@@ -439,9 +446,9 @@ __global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_
 
 // Moves the kept rows: 16 bytes per thread, K and V of a row by neighbouring
 // threads, four rows in flight per thread.  Bound by HBM: 16 x 8 heads of 1024 rows
-// take about 20 us (134 MB moved: 1.0 of the measured copy rate), one context of 20
-// thousand rows 27 (164 MB, 0.92).
-constexpr int kMoveThreads = 256;
+// take 24 us (134 MB moved: 0.85 of the measured copy rate), one context of 20
+// thousand rows 30 (164 MB, 0.84).  Two or eight rows per thread: 1 us more.
+constexpr int kMoveThreads = 128;
 constexpr int kMoveRows = 4;
 
 template <int HD>
@@ -473,10 +480,10 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(b2p::Batch bt,
 #pragma unroll
         for (int i = 0; i < kMoveRows; i++)
             if (page[i] >= 0)
-                v[i] = b2::ld_stream16(pool + page[i] * pg.page + (from[i] & mask) * pg.row);
+                v[i] = *reinterpret_cast<const uint4*>(pool + page[i] * pg.page + (from[i] & mask) * pg.row);
 #pragma unroll
         for (int i = 0; i < kMoveRows; i++)
-            if (page[i] >= 0) *reinterpret_cast<uint4*>(pool + to[i] * pg.page + ((j0 + i * kRows) & mask) * pg.row) = v[i];
+            if (page[i] >= 0) __stcs(reinterpret_cast<uint4*>(pool + to[i] * pg.page + ((j0 + i * kRows) & mask) * pg.row), v[i]);
     }
 }
 

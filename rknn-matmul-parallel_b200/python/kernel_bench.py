@@ -7,13 +7,16 @@ workloads (Qwen3-0.6B: hidden 1024, 16 q / 8 kv heads of 128, ffn 3072).
     (gemm-qkv, gemm-o, gemm-down likewise)
     python rknn-matmul-parallel_b200/python/kernel_bench.py log-mel     [--seconds 30]
     python rknn-matmul-parallel_b200/python/kernel_bench.py sample      [--top-k 50] [--top-p 0.9]
+    python rknn-matmul-parallel_b200/python/kernel_bench.py paged-attn  [--rows 64] [--chunk 1] [--page 64]
+    (paged-append, paged-weights likewise; paged-evict [--budget 1024])
 
 Attention rows are independent sequences whose cache lengths are drawn
-uniformly from [128, 4096) (the batched-decode workload, seeded); GEMM
+uniformly from [128, 4096) (the batched-decode workload, seeded), and for the
+paged kernels each sequence brings --chunk new rows behind them; GEMM
 weights are random bytes of the given type.  Each timed iteration follows
 a 256 MB write that flushes L2; the line printed per case gives the median
 and minimum device time (CUDA events around the C-ABI call) and the
-algorithmic bytes (weights, or the K and V rows attended) per microsecond;
+algorithmic bytes (weights, or the K and V rows attended, moved or written) per microsecond;
 for log-mel (the ASR front end) the FLOPs of the direct 400-point DFT and
 the mel product per second; for sample (on-device sampling over the 151936
 logits of one token) the logit bytes read per second.
@@ -38,12 +41,13 @@ GEMMS = {  # name: (epilogue, K, N)
     "gemm-gu": (bd.EPI_SILU_PAIR, H, FFN),
     "gemm-down": (bd.EPI_ADD, FFN, H),
 }
+PAGED = ["paged-append", "paged-attn", "paged-weights", "paged-evict"]
 WTYPES = {"f16": (bd.W_F16, 2.0), "i8": (bd.W_I8, 1.0), "i4": (bd.W_I4, 0.5)}
 
 
 def main() -> int:
     ap = argparse.ArgumentParser(description=__doc__, formatter_class=argparse.RawDescriptionHelpFormatter)
-    ap.add_argument("kernel", choices=["attn-blocks", "attn-split", "log-mel", "sample"] + sorted(GEMMS))
+    ap.add_argument("kernel", choices=["attn-blocks", "attn-split", "log-mel", "sample"] + PAGED + sorted(GEMMS))
     ap.add_argument("--top-k", type=int, default=50, help="sample: top_k (0: all)")
     ap.add_argument("--top-p", type=float, default=0.9, help="sample: top_p")
     ap.add_argument("--seconds", type=float, default=30.0, help="log-mel: audio length at 16 kHz")
@@ -51,6 +55,9 @@ def main() -> int:
     ap.add_argument("--wtype", choices=sorted(WTYPES), default="i4")
     ap.add_argument("--split", type=int, default=0, help="GEMM split-K cluster size (0: automatic)")
     ap.add_argument("--block", type=int, default=512, help="attention positions per work unit")
+    ap.add_argument("--chunk", type=int, default=1, help="paged-*: new rows of each sequence")
+    ap.add_argument("--page", type=int, default=64, help="paged-*: positions of a page")
+    ap.add_argument("--budget", type=int, default=1024, help="paged-evict: slots kept of each kv head")
     ap.add_argument("--max-seq", type=int, default=4108)
     ap.add_argument("--iters", type=int, default=10)
     ap.add_argument("--seed", type=int, default=5)
@@ -113,6 +120,58 @@ def main() -> int:
 
         def run():
             bd.check(lib.b2_gemm(ctypes.byref(args), stream), a.kernel)
+    elif a.kernel in PAGED:
+        Q, rows, page = a.chunk, M * a.chunk, a.page
+        ctx = rng.integers(128, 4096, M)
+        pages = -(-(ctx + Q) // page)
+        per = -(-a.budget // page)  # pages that an eviction fills
+        order = rng.permutation(int(pages.sum()) + M * per).astype(np.int32)
+        table = np.full((M, int(pages.max())), -1, np.int32)
+        table[np.arange(table.shape[1])[None] < pages[:, None]] = order[:pages.sum()]
+        k, v = ((torch.randn((len(order), NKV, page, HD), device=dev) * 0.1).half() for _ in range(2))
+        table_d = torch.from_numpy(table).to(dev)
+        fresh = torch.from_numpy(order[pages.sum():]).to(dev)
+        kv_len = torch.from_numpy((ctx + Q).astype(np.int32)).to(dev)
+        q_start = torch.arange(0, rows + 1, Q, dtype=torch.int32, device=dev)
+        kv = bd.B2PagedKV(k.data_ptr(), v.data_ptr(), k.stride(0), k.stride(1), k.stride(2), len(order), page, M,
+                          table.shape[1], table_d.data_ptr(), kv_len.data_ptr(), q_start.data_ptr())
+        qkv = torch.randn((rows, (NQ + 2 * NKV) * HD), device=dev)
+        norm = torch.ones(HD, device=dev)
+        cos, sin = torch.ones((4096 + Q, HD // 2), device=dev), torch.zeros((4096 + Q, HD // 2), device=dev)
+        q16 = torch.randn((rows, NQ * HD), device=dev).half()
+        out16, lse = torch.empty_like(q16), torch.empty((rows, NQ), device=dev)
+        work = torch.zeros(lib.b2_attention_paged_workspace(M, Q, NQ, NKV, HD), dtype=torch.uint8, device=dev)
+        err = torch.zeros(1, dtype=torch.int32, device=dev)
+        weights = torch.rand((M, NKV, table.shape[1] * page), device=dev)
+        kept = torch.empty((M, NKV, a.budget), dtype=torch.int32, device=dev)
+        moved, new_len = torch.empty((M, NKV, a.budget), device=dev), torch.empty(M, dtype=torch.int32, device=dev)
+        cached = float((ctx + Q).sum()) * NKV * HD * 2  # of K, or of V
+        nbytes = {"paged-append": rows * (NQ + 2 * NKV) * HD * 6.0, "paged-attn": 2 * cached,
+                  "paged-weights": cached + 2.0 * float((ctx + Q).sum()) * NKV * 4,
+                  "paged-evict": 4.0 * float(np.minimum(ctx + Q, a.budget).sum()) * NKV * HD * 2}[a.kernel]
+        label = f"{a.kernel} sequences={M} ctx=U[128,4096) chunk={Q} page={page}"
+
+        def attend():
+            bd.check(lib.b2_attention_paged(out16.data_ptr(), lse.data_ptr(), q16.data_ptr(), NQ * HD, rows, Q, NQ, NKV,
+                                            HD, ctypes.byref(kv), work.data_ptr(), err.data_ptr(), stream), a.kernel)
+
+        def run():
+            if a.kernel == "paged-append":
+                bd.check(lib.b2_qk_rope_kv_paged(q16.data_ptr(), NQ * HD, qkv.data_ptr(), qkv.shape[1], rows, NQ, NKV, HD,
+                                                 norm.data_ptr(), norm.data_ptr(), 1e-6, cos.data_ptr(), sin.data_ptr(),
+                                                 4096 + Q, 0, None, ctypes.byref(kv), stream), a.kernel)
+            elif a.kernel == "paged-attn":
+                attend()
+            elif a.kernel == "paged-weights":
+                bd.check(lib.b2_attention_paged_weights(weights.data_ptr(), weights.data_ptr(), weights.shape[2],
+                                                        q16.data_ptr(), NQ * HD, lse.data_ptr(), rows, Q, NQ, NKV, HD,
+                                                        ctypes.byref(kv), err.data_ptr(), stream), a.kernel)
+            else:
+                bd.check(lib.b2_kv_evict_paged(ctypes.byref(kv), NKV, HD, weights.data_ptr(), weights.shape[2], a.budget,
+                                               4, a.budget // 4, fresh.data_ptr(), per, kept.data_ptr(),
+                                               moved.data_ptr(), new_len.data_ptr(), stream), a.kernel)
+
+        attend()
     else:
         max_seq = a.max_seq
         pos = rng.integers(128, min(4096, max_seq), M).astype(np.int32)
