@@ -532,8 +532,8 @@ extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const flo
     const PageStrides pg{kv->k_pages, kv->v_pages, kv->page_stride, kv->head_stride, kv->row_stride};
     cudaStream_t st = (cudaStream_t)s;
     // CTAs per (sequence, kv head): as many as have 4096 slots each when the table is
-    // full, and as two per SM have room for.  (4096 slots: 39 us with one, 40 with
-    // two; 100 thousand slots of 8 heads: 264 us with one, 61 with eight.)
+    // full, and as two per SM have room for.  (4096 slots of 128 pairs: 35 us with
+    // one, 37 with two; 100 thousand slots of 8 heads: 233 us with one, 54 with eight.)
     const long long cap = (long long)kv->max_pages * kv->page_size, heads = (long long)kv->n_seqs * nkv;
     int dev = 0, sms = 148, S = 1;
     cudaGetDevice(&dev);
