@@ -153,6 +153,7 @@ constexpr int kUnit = 256;
 constexpr int kLongThreads = 320;
 constexpr int kRowsT = 128;  // rows of a Q tile
 constexpr int kMaxCluster = 4;
+constexpr int kMaxRounds = 16;  // units per CTA up to which several CTAs may share one
 // One pair of exponentials in kPoly takes a polynomial instead of the exponential
 // unit: 2048 rows after 6144, 16 q heads, take 101 us with 3, 104 with 4, 108 without.
 constexpr int kPoly = 3;
@@ -185,9 +186,11 @@ __device__ __forceinline__ Unit find_unit(const WeightParams& p, const int* pre,
     Unit u;
     u.s = prefix_find(pre, p.bt.n_seqs, x);
     u.sq = p.bt.seq(u.s);
-    const int nb = cdiv(u.sq.len, kUnit), off = x - pre[u.s];
-    u.g = off / nb;
-    u.j0 = off % nb * kUnit;
+    // heads of the same slots side by side: a sequence's last units, which its early rows do
+    // not see, come last
+    const int off = x - pre[u.s];
+    u.g = off % p.nkv;
+    u.j0 = off / p.nkv * kUnit;
     const int toks = min(u.sq.Q, p.max_q);
     u.rows = toks * p.G;
     u.tiles = cdiv(toks, T);
@@ -263,15 +266,33 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         const Seq q = p.bt.seq(s);
         return min(q.Q, p.max_q) * p.G > p.short_rows ? cdiv(q.len, kUnit) * p.nkv : 0;
     });
-    // CTAs per unit: the fewest that give the shortest schedule, a unit costing its Q
-    // tiles and about one more for its K tiles.
-    const int W = sm.pre[p.bt.n_seqs], all_tiles = cdiv(p.max_q, T);
+    // Units go round the groups of S CTAs and back, as later ones of a sequence cost
+    // less.  S: the fewest that give the shortest schedule, a unit costing its Q tiles
+    // and about one more for its K tiles, judged by the first group and the last.  Many
+    // rounds are even enough.  (2048 rows after 6144, 8 kv heads: 90 us with two CTAs, 96 with
+    // one, 98 with one and the groups always in the same order.)
+    const int W = sm.pre[p.bt.n_seqs];
+    auto place = [](int round, int c, int n) { return round * n + (round & 1 ? n - 1 - c : c); };
     int S = 1;
-    for (int c = 2; c <= cluster; c *= 2) {
-        auto cost = [&](int n) { return (long long)cdiv(W, gridDim.x / n) * (cdiv(all_tiles, n) + 1); };
-        if (cost(c) < cost(S)) S = c;
+    if (cdiv(W, gridDim.x) <= kMaxRounds) {
+        int best = 0;
+        for (int c = 1; c <= cluster; c *= 2) {
+            const int n = gridDim.x / c;
+            int sum[2] = {0, 0};
+            for (int r = lane; r * n < W; r += 32) {
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int x = place(r, e ? n - 1 : 0, n);
+                    if (x >= W) continue;
+                    const Unit u = find_unit(p, sm.pre, T, x);
+                    sum[e] += cdiv(max(0, u.tiles - u.first), c) + 1;
+                }
+            }
+            const int cost = max(__reduce_add_sync(0xffffffffu, sum[0]), __reduce_add_sync(0xffffffffu, sum[1]));
+            if (c == 1 || cost < best) best = cost, S = c;
+        }
     }
-    const int step = gridDim.x / S, rank = (int)blockIdx.x % S;
+    const int step = gridDim.x / S, group = (int)blockIdx.x / S, rank = (int)blockIdx.x % S;
     const uint32_t lead_cta = cluster > 1 ? cluster_rank() - rank : 0;  // this unit's first CTA, in the cluster
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) mbar_init(&sm.sum_full[i], S > 1 ? 256 * (S - 1) : 1);
@@ -296,7 +317,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             tok[e] = (32 * e + lane) / p.G;
             head[e] = (32 * e + lane) % p.G;
         }
-        for (int x = blockIdx.x / S; x < W && ok; x += step) {
+        for (int r = 0, x; ok && (x = place(r, group, step)) < W; r++) {
             const Unit u = find_unit(p, sm.pre, T, x);
             const int first = uniform(u.first) + rank, tiles = uniform(u.tiles), toks = u.rows / p.G;
             if (first >= tiles) continue;
@@ -360,7 +381,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         // descriptors of the first element; later ones add to the 14-bit address field
         const uint64_t dk = sw128_desc(smem_u32(sm.k[0]), 16), dq = sw128_desc(smem_u32(sm.q[0]), 16);
         int nu = 0, nq = 0;
-        for (int x = blockIdx.x / S; x < W && ok; x += step) {
+        for (int r = 0, x; ok && (x = place(r, group, step)) < W; r++) {
             const Unit u = find_unit(p, sm.pre, T, x);
             const int first = uniform(u.first) + rank, tiles = uniform(u.tiles);
             if (first >= tiles) continue;
@@ -396,7 +417,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         const float scale = kLog2e / sqrtf((float)HD);
         const uint64_t scale2 = pack_f2(scale, scale);
         int nq = 0, done = 0;  // Q tiles; units (all of them, with work here or not)
-        for (int x = blockIdx.x / S; x < W && ok; x += step, done++) {
+        for (int x; ok && (x = place(done, group, step)) < W; done++) {
             const Unit u = find_unit(p, sm.pre, T, x);
             const int j = u.j0 + slot;
             uint64_t acc[2] = {pack_f2(0.f, 0.f), pack_f2(0.f, 0.f)};
@@ -529,9 +550,12 @@ int launch_long(const WeightParams& p, const B2PagedKV* kv, int dev, int sms, cu
     int rc = b2_paged_map(&tk, kv->k_pages, kv, p.nkv, HD, box, 1);
     if (!rc) rc = q_map(&tq, p.q16, p.ldq, p.bt.M, p.nkv, p.G, HD, T);
     if (rc) return rc;
-    // clusters of as many CTAs as the Q tiles of a unit can keep busy
+    // Clusters of as many CTAs as the Q tiles of a unit can keep busy, and of four only where
+    // the units could not fill the SMs: they leave some SMs without work (98 us instead of 90,
+    // for the call above).
     const int tiles = cdiv(p.max_q, T);
-    int S = tiles >= 4 ? 4 : tiles >= 2 ? 2 : 1, clusters = max_clusters<HD>(S, dev, sms, smem);
+    const long long units = ((long long)kv->max_pages * kv->page_size + kUnit - 1) / kUnit * p.nkv * kv->n_seqs;
+    int S = tiles >= 4 && units <= sms ? 4 : tiles >= 2 ? 2 : 1, clusters = max_clusters<HD>(S, dev, sms, smem);
     if (clusters == 0) clusters = sms, S = 1;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(clusters * S);
