@@ -144,8 +144,9 @@ __global__ void __launch_bounds__(kThreads, 4) weights_short_kernel(const Weight
 // Q tile brought in once serves both K tiles.  Where there are too few units to
 // go round, S CTAs of a cluster take every S-th Q tile of one; their sums meet in
 // the first one's shared memory and are added in rank order.
-// 2048 rows after 6144, 16 q heads, hd 128: 101 us, where the exponentials alone
-// would fill the unit for 52 and the product takes 37.
+// 2048 rows after 6144, 16 q heads, hd 128: 91 us, where the exponentials alone
+// would fill the unit for 52 and the product takes 37.  (16 warps of half the columns
+// each in place of 8: the same, and 3 to 19 % slower with chunks of 60 to 1000 rows.)
 //   warp 8      producer: the unit's K tiles, Q tiles and their rows' -lse;
 //   warp 9      tensor cores;
 //   warps 0-3, 4-7   the exponentials of K tile 0 and 1, one slot per thread.
@@ -155,7 +156,8 @@ constexpr int kRowsT = 128;  // rows of a Q tile
 constexpr int kMaxCluster = 4;
 constexpr int kMaxRounds = 16;  // units per CTA up to which several CTAs may share one
 // One pair of exponentials in kPoly takes a polynomial instead of the exponential
-// unit: 2048 rows after 6144, 16 q heads, take 101 us with 3, 104 with 4, 108 without.
+// unit: 2048 rows after 6144, 16 q heads, took 101 us with 3, 104 with 4, 108 without
+// (before units were dealt out as below).
 constexpr int kPoly = 3;
 
 template <int HD>
