@@ -43,9 +43,11 @@ struct Batch {
     const int* q_start;
     int n_seqs, max_pages, n_pages, page_shift, M;
 
-    __device__ __forceinline__ Seq seq(int s) const {
+    __device__ __forceinline__ Seq seq(int s) const { return seq_of(q_start[s], q_start[s + 1], kv_len[s]); }
+    // From the sequence's entries.
+    __device__ __forceinline__ Seq seq_of(int start, int end, int cached) const {
         Seq x;
-        const int a = min(max(q_start[s], 0), M), b = min(max(q_start[s + 1], a), M), n = max(kv_len[s], 0);
+        const int a = min(max(start, 0), M), b = min(max(end, a), M), n = max(cached, 0);
         x.row0 = a;
         x.Q = b - a;
         x.base = n - x.Q;

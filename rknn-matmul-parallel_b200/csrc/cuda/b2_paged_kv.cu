@@ -89,17 +89,25 @@ __global__ void __launch_bounds__(kAppendThreads, 8) append_kernel(
     const float* src = qkv + (size_t)m * ldqkv + lane * E;
 #pragma unroll
     for (int i = 0; i < kHeads; i++) load_vec(x[i], src + (size_t)min(h0 + i, heads - 1) * HD, true);
-    // largest s with q_start[s] <= m: every lane tests one splitter per round
+    int pos = pos_of ? pos_of[m] : 0;
+    // largest s with q_start[s] <= m: every lane tests one splitter per round, and in the
+    // last one has the sequence's entries at hand (what a row waits for is this chain of loads)
     int lo = 0, hi = bt.n_seqs;
-    while (hi - lo > 1) {
+    b2p::Seq sq;
+    for (bool found = false; !found;) {
         const int step = (hi - lo + 31) / 32, at = lo + lane * step;
-        const unsigned le = __ballot_sync(0xffffffffu, at < hi && bt.q_start[at] <= m);
-        lo += (31 - __clz(le)) * step;
+        const bool in = at < hi;
+        found = step == 1;
+        const int start = in ? bt.q_start[at] : 0;
+        const int end = in && found ? bt.q_start[at + 1] : 0, cached = in && found ? bt.kv_len[at] : 0;
+        const int f = 31 - __clz(__ballot_sync(0xffffffffu, in && start <= m));
+        lo += f * step;
         hi = min(hi, lo + step);
+        sq = bt.seq_of(__shfl_sync(0xffffffffu, start, f), __shfl_sync(0xffffffffu, end, f),
+                       __shfl_sync(0xffffffffu, cached, f));
     }
-    const b2p::Seq sq = bt.seq(lo);
     const int slot = sq.base + (m - sq.row0);
-    const int pos = pos_of ? pos_of[m] : slot;
+    if (!pos_of) pos = slot;
     if (pos < 0 || pos >= max_pos || m - sq.row0 >= sq.Q) return;
     const int page = slot >= 0 && slot < sq.len ? bt.page(lo, slot) : -1;
     const long long at = page >= 0 ? page * pg.page + (slot & ((1 << bt.page_shift) - 1)) * pg.row : 0;
