@@ -235,7 +235,8 @@ int b2_attention_blocks(float* out, uint16_t* out16, const float* q, int ldq, in
  * i of them has slot kv_len[q] - Q + i with Q = q_start[q+1] - q_start[q].  Q may
  * be 0 (an idle sequence), 1 (a decode step) or a whole prompt.  Rows from
  * q_start[n_seqs] on belong to nobody and are left as they are.  kv_len counts
- * the new rows.  q_start must not decrease.
+ * the new rows.  q_start must not decrease.  M may be 0 (every sequence idle); the
+ * row arrays may then be NULL.
  *
  * k_pages and v_pages 16-byte aligned, strides multiples of 8 elements, the
  * strides below 2^39 elements; page_size 16, 32, 64 or 128; n_seqs <=

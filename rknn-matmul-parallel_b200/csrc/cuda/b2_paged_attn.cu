@@ -772,7 +772,7 @@ extern "C" int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q
                                   int nkv, int hd, const B2PagedKV* kv, void* work, int* err, b2_stream_t s) {
     int rc = b2_paged_check("b2_attention_paged", kv, nkv, hd, true);
     if (rc) return rc;
-    if (!out16 || !q16 || !work || !err || M < 0 || max_q < 0 || nq <= 0 || nq % nkv || nq / nkv > kMaxGroup)
+    if ((M > 0 && (!out16 || !q16)) || !work || !err || M < 0 || max_q < 0 || nq <= 0 || nq % nkv || nq / nkv > kMaxGroup)
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_attention_paged: bad arguments (nq a multiple of nkv, at most %d)",
                             kMaxGroup);
     if (ldq < (long long)nq * hd || ldq % 8 || (reinterpret_cast<uintptr_t>(q16) & 15) || (reinterpret_cast<uintptr_t>(out16) & 15) ||

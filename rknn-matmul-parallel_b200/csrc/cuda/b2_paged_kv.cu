@@ -541,7 +541,7 @@ extern "C" int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int
                                    const B2PagedKV* kv, b2_stream_t s) {
     int rc = b2_paged_check("b2_qk_rope_kv_paged", kv, nkv, hd, true);
     if (rc) return rc;
-    if (!q16 || !qkv || !cos_tab || !sin_tab || M < 0 || nq <= 0 || max_pos <= 0 || (rope_style != 0 && rope_style != 1))
+    if ((M > 0 && (!q16 || !qkv)) || !cos_tab || !sin_tab || M < 0 || nq <= 0 || max_pos <= 0 || (rope_style != 0 && rope_style != 1))
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_qk_rope_kv_paged: bad arguments");
     if (ldqkv < (nq + 2ll * nkv) * hd || ldq < (long long)nq * hd || ldqkv % 4 || ldq % 4 ||
         (reinterpret_cast<uintptr_t>(qkv) & 15) || (reinterpret_cast<uintptr_t>(q16) & 7))

@@ -890,3 +890,25 @@ def test_sequences_that_share_rows(G, q, seqs_n):
     assert not bool(w[1].any())
     one.work = b.work
     check_attention(one, *one.attend())
+
+
+def test_no_rows():
+    """A batch whose sequences are all idle: nothing to append or attend, the weights are what they were."""
+    b = Paged([(0, 100, ()), (0, 7, ())], 4, 2, 64, 16)
+    L, kv = bd.capi(), b.kv()
+    before = [t.clone() for t in (b.k, b.v)]
+    cos = torch.ones(128, 32, device=DEV)
+    bd.check(L.b2_qk_rope_kv_paged(None, 256, None, 512, 0, 4, 2, 64, None, None, 1e-6, cos.data_ptr(), cos.data_ptr(), 128,
+                                   0, None, ctypes.byref(kv), stream()))
+    bd.check(L.b2_attention_paged(None, None, None, 256, 0, 0, 4, 2, 64, ctypes.byref(kv), b.work.data_ptr(),
+                                  b.err.data_ptr(), stream()))
+    prev = torch.rand(2, 2, 100, device=DEV)
+    for p, max_q in ((prev, 0), (None, 0), (prev, 64)):
+        out = torch.full((2, 2, 100), 7.0, device=DEV)
+        bd.check(L.b2_attention_paged_weights(out.data_ptr(), None if p is None else p.data_ptr(), 100, None, 256, None, 0,
+                                              max_q, 4, 2, 64, ctypes.byref(kv), b.err.data_ptr(), stream()))
+        exp = torch.zeros_like(out) if p is None else p.clone()
+        exp[1, :, 7:] = 7.0
+        assert torch.equal(out, exp)
+    for t, e in zip((b.k, b.v), before):
+        assert torch.equal(t.nan_to_num(9.0), e.nan_to_num(9.0))
