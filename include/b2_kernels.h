@@ -235,8 +235,8 @@ int b2_attention_blocks(float* out, uint16_t* out16, const float* q, int ldq, in
  * i of them has slot kv_len[q] - Q + i with Q = q_start[q+1] - q_start[q].  Q may
  * be 0 (an idle sequence), 1 (a decode step) or a whole prompt.  Rows from
  * q_start[n_seqs] on belong to nobody and are left as they are.  kv_len counts
- * the new rows.  q_start must not decrease.  M may be 0 (every sequence idle); the
- * row arrays may then be NULL.
+ * the new rows.  q_start must not decrease.  M may be 0 (every sequence idle) and
+ * n_seqs may be 0; arrays without entries may then be NULL.
  *
  * k_pages and v_pages 16-byte aligned, strides multiples of 8 elements, the
  * strides below 2^39 elements; page_size 16, 32, 64 or 128; n_seqs <=
@@ -321,7 +321,7 @@ int b2_attention_paged_weights(float* weights, const float* prev, long long ldw,
  *   dst_weights  device FP32  [n_seqs][nkv][budget]  their weights (may be NULL)
  *   new_len      device int   [n_seqs]               slots kept per kv head
  * Entries from new_len[q] on are left as they are.  kv->q_start is not read.
- * sink + recent <= budget. */
+ * sink + recent <= budget; with a budget of 0 dst_table and kept may be NULL. */
 int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const float* weights, long long ldw, int budget, int sink,
                       int recent, const int* dst_table, int dst_max_pages, int* kept, float* dst_weights, int* new_len,
                       b2_stream_t s);

@@ -3,7 +3,8 @@
 #include "b2_paged.cuh"
 
 int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool rows) {
-    if (!kv || !kv->k_pages || !kv->v_pages || !kv->page_table || !kv->kv_len || (rows && !kv->q_start))
+    if (!kv || !kv->k_pages || !kv->v_pages ||
+        (kv->n_seqs > 0 && (!kv->page_table || !kv->kv_len || (rows && !kv->q_start))))
         return b2_set_error(B2_ERR_INVALID_ARG, "%s: null pointer in the cache description", who);
     if (hd != 64 && hd != 128) return b2_set_error(B2_ERR_INVALID_ARG, "%s: head_dim %d not in {64, 128}", who, hd);
     if (kv->page_size != 16 && kv->page_size != 32 && kv->page_size != 64 && kv->page_size != 128)
@@ -569,8 +570,8 @@ extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const flo
                                  float* dst_weights, int* new_len, b2_stream_t s) {
     int rc = b2_paged_check("b2_kv_evict_paged", kv, nkv, hd, false);
     if (rc) return rc;
-    if (!weights || !dst_table || !kept || !new_len || ldw < 0 || budget < 0 || sink < 0 || recent < 0 ||
-        dst_max_pages <= 0 || (long long)sink + recent > budget || nkv > 65535)
+    if ((kv->n_seqs > 0 && (!weights || !new_len)) || ldw < 0 || budget < 0 || sink < 0 || recent < 0 ||
+        (budget > 0 && (!dst_table || !kept || dst_max_pages <= 0)) || (long long)sink + recent > budget || nkv > 65535)
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_kv_evict_paged: bad arguments (sink + recent <= budget)");
     if (kv->n_seqs == 0) return 0;
     const b2p::Batch bt = b2p::make_batch(kv, 0);

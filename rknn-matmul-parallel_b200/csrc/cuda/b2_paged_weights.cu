@@ -586,7 +586,7 @@ extern "C" int b2_attention_paged_weights(float* weights, const float* prev, lon
                                           const B2PagedKV* kv, int* err, b2_stream_t s) {
     int rc = b2_paged_check("b2_attention_paged_weights", kv, nkv, hd, true);
     if (rc) return rc;
-    if (!weights || (M > 0 && (!q16 || !lse)) || !err || ldw < 0 || M < 0 || max_q < 0 || nq <= 0 || nq % nkv || nq / nkv > 16)
+    if ((kv->n_seqs > 0 && !weights) || (M > 0 && (!q16 || !lse)) || !err || ldw < 0 || M < 0 || max_q < 0 || nq <= 0 || nq % nkv || nq / nkv > 16)
         return b2_set_error(B2_ERR_INVALID_ARG,
                             "b2_attention_paged_weights: bad arguments (nq a multiple of nkv, at most 16)");
     if (ldq < (long long)nq * hd || ldq % 8 || (reinterpret_cast<uintptr_t>(q16) & 15))

@@ -912,3 +912,13 @@ def test_no_rows():
         assert torch.equal(out, exp)
     for t, e in zip((b.k, b.v), before):
         assert torch.equal(t.nan_to_num(9.0), e.nan_to_num(9.0))
+
+
+def test_evict_to_nothing():
+    """A budget of 0 keeps nothing and needs no place for it."""
+    b = Paged([(0, 100, ()), (0, 0, ())], 4, 2, 64, 16)
+    before = b.k.clone()
+    w, n = torch.rand(2, 2, 100, device=DEV), torch.full((2,), 7, dtype=torch.int32, device=DEV)
+    bd.check(bd.capi().b2_kv_evict_paged(ctypes.byref(b.kv()), 2, 64, w.data_ptr(), 100, 0, 0, 0, None, 0, None, None,
+                                         n.data_ptr(), stream()))
+    assert n.tolist() == [0, 0] and torch.equal(b.k.nan_to_num(9.0), before.nan_to_num(9.0))

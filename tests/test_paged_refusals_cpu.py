@@ -114,3 +114,14 @@ def test_nothing_to_do():
 def test_workspace_size():
     size = bd.capi().b2_attention_paged_workspace
     assert 0 < size(1, 1, 16, 8, 64) < size(64, 4096, 16, 8, 128) < 256 << 20
+
+
+def test_arrays_without_entries():
+    """No sequences, no rows or no budget: the arrays that would be empty may be NULL."""
+    none = cache(n_seqs=0, page_table=None, kv_len=None, q_start=None)
+    assert append(kv=none, M=0, q16=None, qkv=None) == 0
+    assert attend(kv=none, M=0, q16=None, out=None) == 0
+    assert weigh(kv=none, M=0, q16=None, lse=None, w=None) == 0
+    assert evict(kv=none, w=None, new_len=None) == 0
+    assert append(M=0, q16=None, qkv=None) == 0 and attend(M=0, q16=None, out=None) == 0
+    assert append(M=1, q16=None) == -1 and attend(M=1, out=None) == -1 and weigh(M=1, lse=None) == -1
