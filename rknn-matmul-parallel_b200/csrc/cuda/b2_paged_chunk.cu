@@ -496,6 +496,8 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if constexpr (decltype(edge)::value) {
                     if (B2_RARE(by_hand)) {
                         tmem_wait_st();
+                        // (V is there: the warp that looked has seen it; this wait makes it visible here)
+                        ok = ok && warp_wait(&sm.full[n % C::kStages], (n / C::kStages) & 1, failed);
                         if (b > first) {
                             ok = ok && warp_wait(&sm.o_done[t][(ns - 1) & 1], ((ns - 1) >> 1) & 1, failed);
                             tc_fence_after();
