@@ -255,11 +255,12 @@ __device__ __forceinline__ void merge_task(const AttnParams& p, int owner, const
     if (c0 == 0 && p.lse) p.lse[row * p.nq + h] = l == 0.f ? -INFINITY : M * kLn2 + logf(l);
 }
 
+// scratch: kMergeInts ints that only the four computing warps touch.
+constexpr int kMergeInts = kMaxLongCtas + 1 + 4;
 template <int HD>
 __device__ __forceinline__ void merge_long(const AttnParams& p, int* scratch) {
     constexpr int kMaxCuts = kMaxLongCtas;
     static_assert(kMaxCuts == 2 * 128, "two cuts per thread");
-    static_assert(kMaxCuts + 1 + 4 <= B2_PAGED_MAX_SEQS, "scratch");
     constexpr int kFew = 16;  // pieces up to which a task takes four chunks; more pieces, more tasks
     int* before = scratch;    // tasks of the cuts before each
     int* sums = scratch + kMaxCuts + 1;
@@ -703,7 +704,9 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
     if (!ok && lane == 0) atomicExch(p.err, 1);
     if (p.long_ctas) {
         b2::pdl_wait();
-        merge_long<HD>(p, sm.pre);
+        // (not over sm.pre: nothing orders a CTA without a tile behind its producer's reads of that)
+        static_assert(sizeof(sm.o) >= kMergeInts * sizeof(int), "scratch of the merge");
+        merge_long<HD>(p, reinterpret_cast<int*>(sm.o));
     }
 }
 

@@ -922,3 +922,27 @@ def test_evict_to_nothing():
     bd.check(bd.capi().b2_kv_evict_paged(ctypes.byref(b.kv()), 2, 64, w.data_ptr(), 100, 0, 0, 0, None, 0, None, None,
                                          n.data_ptr(), stream()))
     assert n.tolist() == [0, 0] and torch.equal(b.k.nan_to_num(9.0), before.nan_to_num(9.0))
+
+
+@pytest.mark.parametrize("seqs", [[(90, 90, ())], [(60, 700, ())] * 3, [(300, 4000, ()), (200, 9000, ())],
+                                  [(40, 2500, ()), (1, 30, ())]])
+def test_attention_chunks_alone_repeat(seqs):
+    """Chunks only, or next to one token: most CTAs of the kernel behind the chunks have no tile of their own and go
+    straight to the merge of the chunks' pieces.  Calls one right behind the other give the same bits."""
+    b = Paged(seqs, seed=len(seqs))
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    o2, l2 = torch.empty_like(out), torch.empty_like(lse)
+    kv, L = b.kv(), bd.capi()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        for _ in range(50):
+            bd.check(L.b2_attention_paged(o2.data_ptr(), l2.data_ptr(), b.q16.data_ptr(), b.q16.stride(0), b.M, b.max_q, b.nq,
+                                          b.nkv, b.hd, ctypes.byref(kv), b.work.data_ptr(), b.err.data_ptr(),
+                                          torch.cuda.current_stream().cuda_stream))
+    for _ in range(4):
+        o2.fill_(7.0), l2.fill_(7.0)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(o2, out) and torch.equal(l2, lse)
+    assert b.err.item() == 0 and not b.work[:4096].any()
