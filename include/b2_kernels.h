@@ -288,8 +288,8 @@ int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int
  * its counters zero, and one buffer of the largest size serves calls of any
  * shape one after the other, but not calls that may overlap.  A copy that does
  * not arrive within the wait limit sets *err (device int) to 1 and leaves rows
- * unfinished; zero work again after that.  q16 16-byte aligned, ldq a multiple
- * of 8. */
+ * unfinished; zero work again after that, and after a call that returned
+ * B2_ERR_CUDA.  q16 16-byte aligned, ldq a multiple of 8. */
 size_t b2_attention_paged_workspace(int n_seqs, int max_q, int nq, int nkv, int hd);
 int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq, int M, int max_q, int nq, int nkv,
                        int hd, const B2PagedKV* kv, void* work, int* err, b2_stream_t s);

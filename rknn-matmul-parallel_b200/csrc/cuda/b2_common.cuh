@@ -34,7 +34,9 @@ namespace b2 {
 // kernel launched this way calls pdl_wait() before it reads anything an
 // earlier kernel of the same step writes, and before its first global store;
 // only reads of data written by earlier steps (weights, older KV positions)
-// and L2 prefetches may come before it.
+// and L2 prefetches may come before it.  (One kernel begins beside the one before
+// it, without a wait: attn_short_kernel acquires what a CTA of that one released
+// behind its own pdl_wait(); launch_dependents alone orders no memory.)
 template <typename... KArgs, typename... Args>
 inline cudaError_t launch_pdl(void (*kern)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t s,
                               Args&&... args) {

@@ -212,13 +212,33 @@ struct AttnParams {
     float* lse;
     int max_q, nq, nkv, G;
     int short_rows;  // sequences with at most this many (token, head) rows per kv head are the short kernel's
-    int* counters;   // zero between calls
+    int* counters;   // kCounters of them, zero between calls
     float* part;     // the short kernel's partial tiles
     struct Cut* cuts;       // [long CTAs] tiles that the long kernel left in pieces
     float* long_part;       // their pieces
     int long_ctas;          // CTAs of the long kernel (0: none launched)
     int* err;
 };
+
+// The short kernel's CTAs begin beside the long kernel, which their own wait would
+// have to see complete.  What the kernels before the two wrote they see through the
+// last counter: a CTA of the long kernel adds kWaited there (release) behind its own
+// wait, before it lets the short kernel start, and the short kernel's CTAs acquire
+// that.  Each then adds one, and the last of them makes the counter zero again.
+constexpr int kCounters = 1024;
+constexpr int kWaited = 1 << 16;
+__device__ __forceinline__ int* waited_word(const AttnParams& p) { return p.counters + kCounters - 1; }
+__device__ __forceinline__ void tell_waited(const AttnParams& p) {
+    asm volatile("red.release.gpu.global.add.s32 [%0], %1;" ::"l"(waited_word(p)), "r"(kWaited) : "memory");
+}
+// True with what the telling CTA saw visible.  The word is there before the short kernel
+// starts; should it not be seen at once, the caller waits for the long kernel instead.
+__device__ __forceinline__ bool was_told(const AttnParams& p) {
+    int v = 0;
+    for (int it = 0; it < 64 && v < kWaited; it++)
+        asm volatile("ld.acquire.gpu.global.s32 %0, [%1];" : "=r"(v) : "l"(waited_word(p)) : "memory");
+    return v >= kWaited;
+}
 
 // A tile pair that the long kernel's CTA c (its owner) began and later CTAs
 // finished: pieces c, c + 1, ... wait for the merge.

@@ -324,15 +324,26 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
     }
     b2::pdl_trigger();
-    // Behind the long kernel this grid starts once that one's CTAs have seen the
-    // kernels before them complete; it works beside them and waits for them below.
-    if (!p.long_ctas) b2::pdl_wait();
+    // Behind the long kernel this grid begins on the SMs whose long CTA is done (no SM has
+    // shared memory for both) and waits for the others only before it merges.
+    int before = 0;
+    if (!p.long_ctas) {
+        b2::pdl_wait();
+    } else {
+        if (threadIdx.x == 0) sm.last = was_told(p);
+        __syncthreads();
+        if (!sm.last) b2::pdl_wait();
+        if (threadIdx.x == 0) before = atomicAdd(waited_word(p), 1);
+        // what the kernels before wrote, for the copies too
+        asm volatile("fence.proxy.async.global;" ::: "memory");
+    }
     const int T = R / p.G;
     prefix_work(sm.pre, p.bt.n_seqs, [&](int s) {
         const Seq q = p.bt.seq(s);
         const int n = min(q.Q, p.max_q);
         return n * p.G > p.short_rows ? 0 : cdiv(n, T) * p.nkv * max(1, cdiv(q.len, kBlk));
     });
+    if (before == kWaited + (int)gridDim.x - 1) *waited_word(p) = 0;  // (only where a long kernel ran)
     const int W = sm.pre[p.bt.n_seqs];
     const int per = max(kMinBlocks, cdiv(W, gridDim.x));
     const int x0 = stretch_start(p, sm.pre, W, per, blockIdx.x), x1 = stretch_start(p, sm.pre, W, per, blockIdx.x + 1);
@@ -712,7 +723,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
 
 constexpr int kMaxGroup = 16;
 constexpr int kShortRows = 16;  // (token, head) rows of a kv head that the short kernel takes, at most
-constexpr size_t kCounterBytes = 4096, kCutBytes = kMaxLongCtas * sizeof(Cut);
+constexpr size_t kCounterBytes = kCounters * sizeof(int), kCutBytes = kMaxLongCtas * sizeof(Cut);
 
 // CTAs of a launch: one or two per SM.
 template <int HD, int NT>
@@ -742,7 +753,7 @@ int launch_short(const AttnParams& p, const B2PagedKV* kv, int dev, int sms, lon
     int rc = b2_paged_map(&tk, kv->k_pages, kv, p.nkv, HD, box, HD / 64);
     if (!rc) rc = b2_paged_map(&tv, kv->v_pages, kv, p.nkv, HD, box, HD / 64);
     if (rc) return rc;
-    long long grid = std::min<long long>(short_grid<HD, NT>(dev, sms), kCounterBytes / sizeof(int) / 3);
+    long long grid = std::min<long long>(short_grid<HD, NT>(dev, sms), (kCounters - 1) / 3);
     if (!p.long_ctas && grid > (blocks + kMinBlocks - 1) / kMinBlocks) grid = (blocks + kMinBlocks - 1) / kMinBlocks;
     e = b2::launch_pdl(attn_short_kernel<HD, NT>, dim3((unsigned)grid), dim3(kThreads), smem, s, tk, tv, p);
     if (e != cudaSuccess) return b2_set_error(B2_ERR_CUDA, "b2_attention_paged: %s", cudaGetErrorString(e));

@@ -189,9 +189,9 @@ __global__ void __launch_bounds__(kThreads, 1)
     }
     if (warp == 9) tmem_alloc512(&sm.tmem);
     b2::pdl_wait();
-    // The kernel behind this one works on other rows and waits for this grid before
-    // it merges, but it does not wait for the kernels before this one: let it start
-    // only now that they are done.
+    // The kernel behind this one works on other rows and waits for this grid only before
+    // it merges: it may start now that the kernels before this one are done, and is told so.
+    if (blockIdx.x == 0 && threadIdx.x == 0) tell_waited(p.a);
     b2::pdl_trigger();
     prefix_work(sm.pre_seq, bt.n_seqs, [&](int s) { return cdiv(pairs_of(p, bt.seq(s)), p.group); });
     const int items = min(sm.pre_seq[bt.n_seqs], kMaxItems);  // (more only when sequences share rows)

@@ -946,3 +946,42 @@ def test_attention_chunks_alone_repeat(seqs):
         torch.cuda.synchronize()
         assert torch.equal(o2, out) and torch.equal(l2, lse)
     assert b.err.item() == 0 and not b.work[:4096].any()
+
+
+def test_mixed_steps_back_to_back():
+    """Append and attention of chunks next to single tokens, 24 steps without a host in between: the kernel of the
+    single tokens, which begins beside that of the chunks, finds what the append just wrote.  Same bits as the same
+    steps with the GPU idle between any two calls."""
+    nq, nkv, hd = 8, 4, 128
+    b = Paged([(50, 130, ()), (1, 700, ()), (1, 64, ()), (3, 900, ()), (120, 1000, ())], nq, nkv, hd, 32, seed=8)
+    M, L, kv = b.M, bd.capi(), b.kv()
+    angle = torch.rand(M, hd // 2, device=DEV) * 6
+    cos, sin = angle.cos(), angle.sin()
+    pos = torch.arange(M, dtype=torch.int32, device=DEV)
+    qkv = torch.randn(24, M, (nq + 2 * nkv) * hd, device=DEV)
+    b.q16 = torch.zeros(M, nq * hd, dtype=torch.float16, device=DEV)
+    start = [t.clone() for t in (b.k, b.v)]
+
+    def steps(idle):
+        b.k.copy_(start[0]), b.v.copy_(start[1])
+        out, lse = torch.zeros(24, M, nq * hd, dtype=torch.float16, device=DEV), torch.zeros(24, M, nq, device=DEV)
+        torch.cuda.synchronize()
+        for i in range(24):
+            bd.check(L.b2_qk_rope_kv_paged(b.q16.data_ptr(), nq * hd, qkv[i].data_ptr(), qkv.stride(1), M, nq, nkv, hd, None,
+                                           None, 1e-6, cos.data_ptr(), sin.data_ptr(), M, 1, pos.data_ptr(),
+                                           ctypes.byref(kv), stream()))
+            if idle:
+                torch.cuda.synchronize()
+            bd.check(L.b2_attention_paged(out[i].data_ptr(), lse[i].data_ptr(), b.q16.data_ptr(), nq * hd, M, b.max_q, nq, nkv,
+                                          hd, ctypes.byref(kv), b.work.data_ptr(), b.err.data_ptr(), stream()))
+            if idle:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        assert b.err.item() == 0 and not b.work[:4096].any()
+        return out, lse
+
+    out, lse = steps(True)
+    check_attention(b, out[-1], lse[-1])
+    for _ in range(3):
+        o2, l2 = steps(False)
+        assert torch.equal(o2, out) and torch.equal(l2, lse)
