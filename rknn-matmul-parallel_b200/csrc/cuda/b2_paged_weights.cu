@@ -25,7 +25,6 @@ struct WeightParams {
     const float* prev;
     long long ldw;
     int short_rows;  // sequences with at most this many (token, head) rows per kv head are the short kernel's
-    int after_long;  // the long kernel was launched before the short one
     int* err;
 };
 
@@ -41,13 +40,21 @@ struct WeightParams {
 constexpr int kThreads = 128;
 constexpr int kBlk = 128;
 
+// (not the read-only path: the kernel may have started while K was being appended)
+__device__ __forceinline__ uint4 ld_k16(const void* p) {
+    uint4 r;
+    asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w)
+                 : "l"(p)
+                 : "memory");
+    return r;
+}
+
 template <int HD>
 __global__ void __launch_bounds__(kThreads, 4) weights_short_kernel(const WeightParams p) {
     __shared__ int pre[B2_PAGED_MAX_SEQS + 1];
     b2::pdl_trigger();
-    // Behind the long kernel this grid starts once that one's CTAs have seen the
-    // kernels before them complete, works beside them and waits for them at the end.
-    if (!p.after_long) b2::pdl_wait();
+    b2::pdl_wait();  // (behind the long kernel too: there is no workspace to hand over what that one waited for)
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, n = lane >> 2, c4 = lane & 3;
     prefix_work(pre, p.bt.n_seqs, [&](int s) {
         const Seq q = p.bt.seq(s);
@@ -79,8 +86,8 @@ __global__ void __launch_bounds__(kThreads, 4) weights_short_kernel(const Weight
                                      (long long)(((j0 + 16 * t) & slot_mask) + n) * p.row_stride + 8 * c4;
 #pragma unroll
                 for (int u = 0; u < HD / 32; u++) {
-                    a[t][0][u] = page[t] >= 0 ? b2::ld_stream16(kp + 32 * u) : make_uint4(0, 0, 0, 0);
-                    a[t][1][u] = page[t] >= 0 ? b2::ld_stream16(kp + 8 * p.row_stride + 32 * u) : make_uint4(0, 0, 0, 0);
+                    a[t][0][u] = page[t] >= 0 ? ld_k16(kp + 32 * u) : make_uint4(0, 0, 0, 0);
+                    a[t][1][u] = page[t] >= 0 ? ld_k16(kp + 8 * p.row_stride + 32 * u) : make_uint4(0, 0, 0, 0);
                 }
             }
             for (int r0 = r_first; r0 < rows; r0 += 8) {
@@ -132,7 +139,6 @@ __global__ void __launch_bounds__(kThreads, 4) weights_short_kernel(const Weight
         const float v = lane < 16 ? (lane < 8 ? v00 : v01) : (lane < 24 ? v10 : v11);
         if (out) p.weights[o] = was + v;
     }
-    if (p.after_long) b2::pdl_wait();
 }
 
 // ─── many rows per sequence: chunks ───
@@ -262,7 +268,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
     }
     if (warp == 9) tmem_alloc512(&sm.tmem);
     b2::pdl_wait();
-    b2::pdl_trigger();  // only now: the kernel behind this one does not wait for those before it
+    b2::pdl_trigger();
     const int T = kRowsT / p.G;
     prefix_work(sm.pre, p.bt.n_seqs, [&](int s) {
         const Seq q = p.bt.seq(s);
@@ -602,13 +608,12 @@ extern "C" int b2_attention_paged_weights(float* weights, const float* prev, lon
     cudaGetDevice(&dev);
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     if (max_q > M) max_q = M;
-    WeightParams p{make_batch(kv, M), kv->k_pages, kv->page_stride, kv->head_stride, kv->row_stride,
+    const WeightParams p{make_batch(kv, M), kv->k_pages, kv->page_stride, kv->head_stride, kv->row_stride,
                          reinterpret_cast<const __half*>(q16), ldq, lse, max_q, nq, nkv, nq / nkv, weights, prev, ldw,
-                   kShortRows, 0, err};
+                         kShortRows, err};
     if ((long long)max_q * p.G > kShortRows) {
         rc = hd == 128 ? launch_long<128>(p, kv, dev, sms, (cudaStream_t)s) : launch_long<64>(p, kv, dev, sms, (cudaStream_t)s);
         if (rc) return rc;
-        p.after_long = 1;
     }
     const long long grid = blocks < sms * 4 ? blocks : sms * 4;  // what is resident
     const cudaError_t e = b2::launch_pdl(hd == 128 ? weights_short_kernel<128> : weights_short_kernel<64>,

@@ -985,3 +985,39 @@ def test_mixed_steps_back_to_back():
     for _ in range(3):
         o2, l2 = steps(False)
         assert torch.equal(o2, out) and torch.equal(l2, lse)
+
+
+def test_weights_back_to_back():
+    """Append and weights of chunks next to single tokens, 24 steps without a host in between: the same bits as with
+    the GPU idle between any two calls."""
+    nq, nkv, hd = 8, 4, 128
+    b = Paged([(50, 130, ()), (1, 700, ()), (1, 64, ()), (3, 900, ()), (120, 1000, ())], nq, nkv, hd, 32, seed=9)
+    M, L, kv = b.M, bd.capi(), b.kv()
+    angle = torch.rand(M, hd // 2, device=DEV) * 6
+    cos, sin = angle.cos(), angle.sin()
+    pos = torch.arange(M, dtype=torch.int32, device=DEV)
+    qkv = torch.randn(24, M, (nq + 2 * nkv) * hd, device=DEV)
+    b.q16 = torch.zeros(M, nq * hd, dtype=torch.float16, device=DEV)
+    lse = torch.rand(M, nq, device=DEV) + 8
+    start = [t.clone() for t in (b.k, b.v)]
+
+    def steps(idle):
+        b.k.copy_(start[0]), b.v.copy_(start[1])
+        out = torch.zeros(24, 5, nkv, 1000, device=DEV)
+        torch.cuda.synchronize()
+        for i in range(24):
+            bd.check(L.b2_qk_rope_kv_paged(b.q16.data_ptr(), nq * hd, qkv[i].data_ptr(), qkv.stride(1), M, nq, nkv, hd, None,
+                                           None, 1e-6, cos.data_ptr(), sin.data_ptr(), M, 1, pos.data_ptr(),
+                                           ctypes.byref(kv), stream()))
+            if idle:
+                torch.cuda.synchronize()
+            b.weigh(lse, out[i - 1] if i else None, out[i])
+            if idle:
+                torch.cuda.synchronize()
+        torch.cuda.synchronize()
+        return out
+
+    out = steps(True)
+    check_weights(b, lse, out[-2], out[-1], 1000, 0.0)
+    for _ in range(3):
+        assert torch.equal(steps(False), out)
