@@ -2,6 +2,10 @@
 // accumulated attention weight (b2_kv_evict_paged).
 #include "b2_paged.cuh"
 
+// (No pointer of these kernels is __restrict__: they may start while the kernel before
+// them still writes what they read behind their wait, and the compiler would take the
+// read-only path, which no wait orders.)
+
 int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool rows) {
     if (!kv || !kv->k_pages || !kv->v_pages ||
         (kv->n_seqs > 0 && (!kv->page_table || !kv->kv_len || (rows && !kv->q_start))))
@@ -105,9 +109,9 @@ __device__ __forceinline__ void four_norms(const float (&x)[kHeads][HD / 32], fl
 // with eight, 39.9 with nine, whose registers hold fewer loads ahead.
 template <int HD>
 __global__ void __launch_bounds__(kAppendThreads, 7) append_kernel(
-    __half* __restrict__ q16, int ldq, const float* __restrict__ qkv, int ldqkv, int nq, int nkv,
-    const float* __restrict__ q_norm_w, const float* __restrict__ k_norm_w, float eps, const float* __restrict__ cos_tab,
-    const float* __restrict__ sin_tab, int max_pos, int rope_style, const int* __restrict__ pos_of, b2p::Batch bt,
+    __half* q16, int ldq, const float* qkv, int ldqkv, int nq, int nkv,
+    const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_tab,
+    const float* sin_tab, int max_pos, int rope_style, const int* pos_of, b2p::Batch bt,
     PageStrides pg, bool aligned, int steps) {
     constexpr int E = HD / 32;  // elements per lane
     b2::pdl_trigger();
@@ -268,11 +272,11 @@ __device__ __forceinline__ void sync_cluster(int S) {
 
 // S = gridDim.x.
 template <int kSelThreads>
-__global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_kernel(b2p::Batch bt, const float* __restrict__ weights,
+__global__ void __launch_bounds__(kSelThreads, 1024 / kSelThreads) evict_select_kernel(b2p::Batch bt, const float* weights,
                                                                    long long ldw, int nkv, int budget, int sink,
-                                                                   int recent, int held, int* __restrict__ kept,
-                                                                   float* __restrict__ dst_weights,
-                                                                   int* __restrict__ new_len) {
+                                                                   int recent, int held, int* kept,
+                                                                   float* dst_weights,
+                                                                   int* new_len) {
     constexpr int kSelWarps = kSelThreads / 32;
     extern __shared__ uint32_t keys[];
     __shared__ int hist[2][257];  // [digit parity]; [256]: unmapped slots
@@ -500,9 +504,9 @@ constexpr int kMoveRows = 4;
 
 template <int HD>
 __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(b2p::Batch bt, PageStrides pg, int budget,
-                                                                  const int* __restrict__ dst_table, int dst_max_pages,
-                                                                  const int* __restrict__ kept,
-                                                                  const int* __restrict__ new_len) {
+                                                                  const int* dst_table, int dst_max_pages,
+                                                                  const int* kept,
+                                                                  const int* new_len) {
     constexpr int C = HD / 8;  // 16-byte chunks of a row
     constexpr int kRows = kMoveThreads / (2 * C);
     b2::pdl_trigger();
