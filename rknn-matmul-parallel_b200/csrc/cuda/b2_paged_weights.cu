@@ -477,8 +477,9 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 add(vb, 96);
             };
             for (int i = first; i < tiles; i += S, nq++) {
-                // columns of tokens from the slot's own on, and rows that exist
-                const int c0 = min(j - u.sq.base - i * T, kRowsT) * p.G, c1 = min(T * p.G, u.rows - i * T * p.G);
+                // columns of tokens from the slot's own on, and rows that exist (bounded before the product:
+                // a slot may lie 2^31 before the new rows)
+                const int c0 = max(0, min(j - u.sq.base - i * T, kRowsT)) * p.G, c1 = min(T * p.G, u.rows - i * T * p.G);
                 if (B2_RARE(__any_sync(0xffffffffu, c0 > 0 || c1 < kRowsT))) step(std::true_type{}, c0, c1);
                 else step(std::false_type{}, c0, c1);
                 if (B2_RARE(!ok)) break;

@@ -1021,3 +1021,58 @@ def test_weights_back_to_back():
     check_weights(b, lse, out[-2], out[-1], 1000, 0.0)
     for _ in range(3):
         assert torch.equal(steps(False), out)
+
+
+@pytest.mark.parametrize("q", [3, 20, 60])
+@pytest.mark.parametrize("G,n", [(16, (1 << 27) + 700), (16, (1 << 28) + 80), (16, 2**31 - 1), (8, (1 << 28) + 700),
+                                 (2, (1 << 30) + 900), (16, (1 << 27) - 50)])
+def test_weights_far_below_the_new_rows(G, n, q):
+    """Slots so far before the new rows that the distance times the group passes 32 bits: every row sees them."""
+    b = Paged([(q, 128 + q, ()), (1, 40, ())], G, 1, 64, 64, seed=G + q)
+    b.seqs[0] = (q, n, ())  # a table of 128 slots and a bit, all of them before the first new row
+    b.kv_len[0] = n
+    b.table = b.table[:, :2].contiguous()
+    r = slice(0, q)
+    K = b.slots(0)[1][:, 0]
+    x = torch.einsum("rgd,jd->rgj", b.q16[r, :G * 64].to(F64).view(q, G, 64), K) / 8
+    lse = torch.full((b.M, G), 3.0, device=DEV)
+    lse[:q] = x.logsumexp(-1).float()
+    out = b.weigh(lse, None, torch.full((2, 1, 200), 7.0, device=DEV))
+    exp = (x - lse[:q].to(F64)[..., None]).exp().sum((0, 1))
+    # scores are off by (hd + 2) 2^-23 sum|q k| / 8 at most, here below 2^-13; the other roundings below 2^-15
+    assert bool(((out[0, 0, :128].to(F64) - exp).abs() <= 2.0 ** -12 * exp).all())
+    assert bool((out[0, 0, 128:] == 7).all()) and b.err.item() == 0
+
+
+@pytest.mark.parametrize("q", [2, 20])
+def test_first_page_and_a_window_far_behind(q):
+    """One context of 150 million slots of which the first page and the newest are mapped: attention and weights."""
+    nq, hd, page = 16, 64, 128
+    n, pages = 150_000_000, -(-150_000_000 // 128)
+    b = Paged([(q, 2 * page + q, ())], nq, 1, hd, page, seed=q)
+    first, late = int(b.table[0, 0]), [int(x) for x in b.table[0, 1:]]
+    window = (n - q) // page  # the page of the first new row
+    b.k[late[0]], b.v[late[0]] = (torch.randn(1, page, hd, device=DEV).half() for _ in range(2))
+    b.table = torch.full((1, pages), -1, dtype=torch.int32, device=DEV)
+    b.table[0, 0], b.table[0, window - 1] = first, late[0]
+    for p in range(window, pages):
+        b.table[0, p] = late[1] if p == window else b.spare[p - window - 1]
+    m = n - window * page  # slots cached on the pages from `window` on
+    for i in range(0, m, page):
+        at = int(b.table[0, window + i // page])
+        for t in (b.k, b.v):
+            t[at, :, :min(page, m - i)] = torch.randn(1, min(page, m - i), hd, device=DEV).half()
+    b.seqs, b.kv_len[0] = [(q, n, ())], n
+    near = torch.arange((window - 1) * page, n, device=DEV)
+    j = torch.cat([torch.arange(page, device=DEV), near])
+    at, off = b.table[0, j // page].long(), j % page
+    b.slots = lambda s: (j, b.k[at, :, off].to(F64), b.v[at, :, off].to(F64))
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    K, Q = b.slots(0)[1][:, 0], b.q16[:q, :nq * hd].to(F64).view(q, nq, hd)
+    x = torch.einsum("rgd,jd->rgj", Q, K) / 8
+    x = x.masked_fill((j[None] > n - q + torch.arange(q, device=DEV)[:, None])[:, None], -math.inf)
+    exp = (x - lse[:q].to(F64)[..., None]).exp().sum((0, 1))
+    got = b.weigh(lse, None, torch.full((1, 1, n), 7.0, device=DEV))[0, 0]
+    assert bool(((got[j].to(F64) - exp).abs() <= 2.0 ** -12 * exp).all())
+    assert not bool(got[page:(window - 1) * page].any()) and b.err.item() == 0
