@@ -173,6 +173,7 @@ struct LongSmem {
     alignas(1024) unsigned char k[2][kTile];  // [tile]
     alignas(1024) unsigned char q[kQStages][kTile];
     alignas(16) float nl[16][kRowsT];            // -lse log2(e) of the rows of Q tile (count % 16)
+    int none[16];                                // some of them are -infinity: rows without weight
     float part[2][kMaxCluster - 1][kUnit];       // first CTA: the others' sums, by unit parity
     uint64_t k_full, k_empty, q_full[kQStages], q_empty[kQStages];
     uint64_t s_full[2][2], s_free[2][2];         // [K tile][buffer]
@@ -359,9 +360,14 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 const int qb = nq % Sm::kQStages;
                 if (nq >= Sm::kQStages) ok = warp_wait(&sm.q_empty[qb], (nq / Sm::kQStages - 1) & 1, failed);
                 if (!ok) break;
+                bool none = false;
 #pragma unroll
-                for (int e = 0; e < 4; e++)
+                for (int e = 0; e < 4; e++) {
+                    none |= next[e] == -INFINITY;
                     sm.nl[nq & 15][32 * e + lane] = next[e] == -INFINITY ? -INFINITY : -next[e] * kLog2e;
+                }
+                none = __any_sync(0xffffffffu, none);
+                if (lane == 0) sm.none[nq & 15] = none;
                 __syncwarp();
                 if (lane == 0) mbar_expect_tx(&sm.q_full[qb], T * p.G * HD * 2);
                 __syncwarp();
@@ -430,15 +436,14 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             const int j = u.j0 + slot;
             uint64_t acc[2] = {pack_f2(0.f, 0.f), pack_f2(0.f, 0.f)};
             const int first = uniform(u.first) + rank, tiles = uniform(u.tiles);
-            // One Q tile; edge: with columns that the slot is not seen by.  Two copies, because a path beside
-            // the common one costs that one time even where it is not taken.
-            auto step = [&](auto edge, int c0, int c1) {
+            // One Q tile; edge: with columns that the slot is not seen by, or of rows without weight, whose
+            // product with K may be anything.  Two copies, because a path beside the common one costs that one
+            // time even where it is not taken.
+            // (its first 32 columns are on their way)
+            auto step = [&](auto edge, uint32_t ts, uint32_t (&va)[32], int c0, int c1) {
                 const int b = nq & 1;
-                ok = warp_wait(&sm.s_full[t][b], (nq / 2) & 1, failed);
-                tc_fence_after();
-                const uint32_t ts = tmem + lanes + (2 * t + b) * 128;
                 const float4* nl = reinterpret_cast<const float4*>(sm.nl[nq & 15]);
-                uint32_t va[32], vb[32];
+                uint32_t vb[32];
                 // 32 columns from c0 on, the next ones on their way
                 auto add = [&](uint32_t (&v)[32], int col) {
 #pragma unroll
@@ -452,15 +457,14 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                                       x, y);
                             if constexpr (decltype(edge)::value) {  // (here, where a row's NaN sum is in it too)
                                 const int r = col + c + 2 * e;
-                                if (r < c0 || r >= c1) x = -INFINITY;
-                                if (r + 1 < c0 || r + 1 >= c1) y = -INFINITY;
+                                if (r < c0 || r >= c1 || (e ? n4.z : n4.x) == -INFINITY) x = -INFINITY;
+                                if (r + 1 < c0 || r + 1 >= c1 || (e ? n4.w : n4.y) == -INFINITY) y = -INFINITY;
                             }
                             const bool poly = (c / 2 + e) % kPoly == kPoly - 1;
                             acc[e] = add_f2(acc[e], poly ? ex2_f2(x, y) : pack_f2(ex2(x), ex2(y)));
                         }
                     }
                 };
-                tmem_ld32<0>(ts, va);
                 tmem_wait_ld();
                 tmem_ld32<0>(ts + 32, vb);
                 add(va, 0);
@@ -480,8 +484,14 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 // columns of tokens from the slot's own on, and rows that exist (bounded before the product:
                 // a slot may lie 2^31 before the new rows)
                 const int c0 = max(0, min(j - u.sq.base - i * T, kRowsT)) * p.G, c1 = min(T * p.G, u.rows - i * T * p.G);
-                if (B2_RARE(__any_sync(0xffffffffu, c0 > 0 || c1 < kRowsT))) step(std::true_type{}, c0, c1);
-                else step(std::false_type{}, c0, c1);
+                const uint32_t ts = tmem + lanes + (2 * t + (nq & 1)) * 128;
+                uint32_t va[32];
+                ok = warp_wait(&sm.s_full[t][nq & 1], (nq / 2) & 1, failed);
+                tc_fence_after();
+                tmem_ld32<0>(ts, va);
+                const int none = *(volatile int*)&sm.none[nq & 15];
+                if (B2_RARE(__any_sync(0xffffffffu, c0 > 0 || c1 < kRowsT || none))) step(std::true_type{}, ts, va, c0, c1);
+                else step(std::false_type{}, ts, va, c0, c1);
                 if (B2_RARE(!ok)) break;
             }
             if (!ok) break;

@@ -1076,3 +1076,25 @@ def test_first_page_and_a_window_far_behind(q):
     got = b.weigh(lse, None, torch.full((1, 1, n), 7.0, device=DEV))[0, 0]
     assert bool(((got[j].to(F64) - exp).abs() <= 2.0 ** -12 * exp).all())
     assert not bool(got[page:(window - 1) * page].any()) and b.err.item() == 0
+
+
+@pytest.mark.parametrize("q", [6, 60, 150, 300])
+def test_weights_without_excluded_rows(q):
+    """Rows that the caller excludes (lse -infinity) give nothing whatever q holds there, and slots whose K is not
+    finite get nothing from them; the other rows' weights stay what they were."""
+    b = Paged([(q, 180 + q, ()), (q, q + 5, ())], 4, 2, 64, 64, seed=q)
+    _, lse = b.attend()
+    out = torch.arange(b.M, device=DEV) % 3 == 1  # excluded rows
+    out[:min(q, 140)] |= q >= 150                 # a whole tile of them
+    lse[out] = -math.inf
+    ldw = 200 + q
+    exp = b.weigh(lse, None, torch.zeros(2, 2, ldw, device=DEV))
+    check_weights(b, lse, None, exp, ldw, 0.0)
+    b.q16[out, :256] = math.nan
+    assert torch.equal(b.weigh(lse, None, torch.zeros(2, 2, ldw, device=DEV)), exp)
+    b.q16[out, :256] = math.inf
+    assert torch.equal(b.weigh(lse, None, torch.zeros(2, 2, ldw, device=DEV)), exp)
+    b.q16[out, :256] = 1.0
+    lse[:q] = -math.inf  # all of sequence 0
+    b.k[b.table[0, 1], :, 3], b.k[b.table[0, 0], 1, 7, 5] = math.inf, math.nan
+    assert not bool(b.weigh(lse, None, torch.full((2, 2, ldw), 7.0, device=DEV))[0, :, :180 + q].any())
