@@ -321,6 +321,8 @@ int b2_attention_paged_weights(float* weights, const float* prev, long long ldw,
  *   dst_weights  device FP32  [n_seqs][nkv][budget]  their weights (may be NULL)
  *   new_len      device int   [n_seqs]               slots kept per kv head
  * Entries from new_len[q] on are left as they are.  kv->q_start is not read.
+ * None of the three may overlap another, weights, kv_len, page_table or dst_table
+ * (refused).
  * sink + recent <= budget; with a budget of 0 dst_table and kept may be NULL. */
 int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const float* weights, long long ldw, int budget, int sink,
                       int recent, const int* dst_table, int dst_max_pages, int* kept, float* dst_weights, int* new_len,

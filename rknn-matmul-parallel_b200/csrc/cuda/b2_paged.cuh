@@ -16,6 +16,11 @@ int b2_tensor_map_f16_5d(void* map, const void* base, const uint64_t (&dims)[5],
 
 // Host checks shared by the entry points; 0 or an error code with its message.
 int b2_paged_check(const char* who, const B2PagedKV* kv, int nkv, int hd, bool rows);
+// Whether two arrays of so many 4-byte entries share any.
+inline bool b2_paged_overlap(const void* a, long long na, const void* b, long long nb) {
+    const uintptr_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    return a && b && na > 0 && nb > 0 && (x < y ? y - x < 4ull * na : x - y < 4ull * nb);
+}
 // Tensor map of K or V pages: dimensions (64 dims, rows of a page, head_dim / 64,
 // kv heads, pages), boxes of box_rows rows and box_halves times 64 dims: a box
 // lands as [box_halves][box_rows][128 bytes], each 128-byte row swizzled.

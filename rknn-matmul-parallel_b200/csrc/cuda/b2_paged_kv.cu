@@ -578,6 +578,21 @@ extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const flo
         (budget > 0 && (!dst_table || !kept || dst_max_pages <= 0)) || (long long)sink + recent > budget || nkv > 65535)
         return b2_set_error(B2_ERR_INVALID_ARG, "b2_kv_evict_paged: bad arguments (sink + recent <= budget)");
     if (kv->n_seqs == 0) return 0;
+    // One head's CTAs store while others still read: nothing that is written may be among what is read.
+    const long long n = kv->n_seqs, rows = n * nkv, row = ldw < (1ll << 34) ? ldw : 1ll << 34;
+    const struct {
+        const void* p;
+        long long count;
+    } out[3] = {{kept, rows * budget}, {dst_weights, rows * budget}, {new_len, n}},
+      in[4] = {{weights, rows * row}, {kv->page_table, n * kv->max_pages}, {kv->kv_len, n}, {dst_table, n * dst_max_pages}};
+    for (int i = 0; i < 3; i++) {
+        bool bad = false;
+        for (int j = 0; j < 4; j++) bad |= b2_paged_overlap(out[i].p, out[i].count, in[j].p, in[j].count);
+        for (int j = 0; j < i; j++) bad |= b2_paged_overlap(out[i].p, out[i].count, out[j].p, out[j].count);
+        if (bad)
+            return b2_set_error(B2_ERR_INVALID_ARG, "b2_kv_evict_paged: %s overlaps another array of the call",
+                                i == 0 ? "kept" : i == 1 ? "dst_weights" : "new_len");
+    }
     const b2p::Batch bt = b2p::make_batch(kv, 0);
     const PageStrides pg{kv->k_pages, kv->v_pages, kv->page_stride, kv->head_stride, kv->row_stride};
     cudaStream_t st = (cudaStream_t)s;

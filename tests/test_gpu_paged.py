@@ -1098,3 +1098,22 @@ def test_weights_without_excluded_rows(q):
     lse[:q] = -math.inf  # all of sequence 0
     b.k[b.table[0, 1], :, 3], b.k[b.table[0, 0], 1, 7, 5] = math.inf, math.nan
     assert not bool(b.weigh(lse, None, torch.full((2, 2, ldw), 7.0, device=DEV))[0, :, :180 + q].any())
+
+
+def test_evict_arrays_side_by_side():
+    """The arrays that an eviction reads and writes one right behind the other: no overlap, no refusal."""
+    b = Paged([(0, 100, ()), (0, 60, ())], 2, 1, 64, 16, extra_pages=8)
+    sizes = [2 * 100, 2 * 32, 2 * 32, 2, 2 * 7, 2, 2 * 2]  # weights, kept, moved weights, new_len, table, kv_len, dst
+    at = [sum(sizes[:i]) for i in range(len(sizes))]
+    pool = torch.zeros(sum(sizes), dtype=torch.int32, device=DEV)
+    w, kept, dw, new, table, kl, dst = (pool[a:a + n] for a, n in zip(at, sizes))
+    w.view(torch.float32).copy_(torch.rand(200, device=DEV))
+    table.copy_(b.table.flatten()), kl.copy_(b.kv_len), dst.copy_(torch.tensor(b.spare[:4]))
+    ref = evict_reference(b, w.view(torch.float32).view(2, 1, 100), 32, 2, 5)
+    kv = b.kv()
+    kv.page_table, kv.kv_len = table.data_ptr(), kl.data_ptr()
+    bd.check(bd.capi().b2_kv_evict_paged(ctypes.byref(kv), 1, 64, w.data_ptr(), 100, 32, 2, 5, dst.data_ptr(), 2,
+                                         kept.data_ptr(), dw.data_ptr(), new.data_ptr(), stream()))
+    assert new.tolist() == [32, 32] and kept.view(2, 32).tolist() == [ref[0][0], ref[1][0]]
+    assert torch.equal(dw.view(torch.float32).view(2, 32),
+                       torch.stack([w.view(torch.float32)[s * 100:][kept.view(2, 32)[s].long()] for s in range(2)]))

@@ -125,3 +125,31 @@ def test_arrays_without_entries():
     assert evict(kv=none, w=None, new_len=None) == 0
     assert append(M=0, q16=None, qkv=None) == 0 and attend(M=0, q16=None, out=None) == 0
     assert append(M=1, q16=None) == -1 and attend(M=1, out=None) == -1 and weigh(M=1, lse=None) == -1
+
+
+def arrays_of_an_eviction(**at):
+    """Two sequences, 8 kv heads, rows of 256 weights, 64 slots kept; `at` moves arrays."""
+    a = dict(w=1 << 20, kept=2 << 20, dw=3 << 20, new_len=4 << 20, table=5 << 20, kv_len=6 << 20, dst=7 << 20)
+    a.update(at)
+    return a
+
+
+def evict_at(**at):
+    a = arrays_of_an_eviction(**at)
+    kv = cache(page_table=a["table"], kv_len=a["kv_len"])
+    return bd.capi().b2_kv_evict_paged(ctypes.byref(kv), 8, 128, a["w"], 256, 64, 4, 8, a["dst"], 1, a["kept"], a["dw"],
+                                       a["new_len"], None)
+
+
+W, K = 2 * 8 * 256 * 4, 2 * 8 * 64 * 4  # bytes of weights; of kept and of dst_weights
+
+
+@pytest.mark.parametrize("bad", [
+    dict(dw=1 << 20), dict(dw=(1 << 20) + W - 4), dict(dw=(1 << 20) - K + 4),           # weights moved in place
+    dict(kept=1 << 20), dict(kept=(1 << 20) + W - 4), dict(kept=3 << 20), dict(kept=(3 << 20) - K + 4),
+    dict(kept=(5 << 20) + 28), dict(kept=7 << 20), dict(kept=(7 << 20) + 4), dict(kept=6 << 20),
+    dict(new_len=6 << 20), dict(new_len=(6 << 20) + 4), dict(new_len=(6 << 20) - 4),     # lengths updated in place
+    dict(new_len=1 << 20), dict(new_len=2 << 20), dict(new_len=(3 << 20) + K - 4), dict(new_len=5 << 20), dict(new_len=7 << 20)])
+def test_evict_refuses_overlap(bad):
+    assert evict_at(**bad) == -1
+    assert b"overlaps" in bd.capi().b2_last_error()
