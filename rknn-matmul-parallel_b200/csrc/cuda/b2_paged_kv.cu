@@ -511,19 +511,20 @@ __global__ void __launch_bounds__(kMoveThreads) evict_move_kernel(b2p::Batch bt,
     constexpr int kRows = kMoveThreads / (2 * C);
     b2::pdl_trigger();
     b2::pdl_wait();
-    const int s = blockIdx.z, g = blockIdx.y, nkv = gridDim.y, n = new_len[s];
+    const int s = blockIdx.z, g = blockIdx.y, nkv = gridDim.y;
+    const unsigned n = new_len[s];  // (unsigned: a place past it, by up to a stride of the grid, may pass 2^31)
     const int c = threadIdx.x % C, which = threadIdx.x / C % 2;
     uint16_t* pool = (which ? pg.v : pg.k) + g * pg.head + c * 8;
     const int mask = (1 << bt.page_shift) - 1;
     const int* from_of = kept + ((size_t)s * nkv + g) * budget;
-    for (int j0 = blockIdx.x * kRows * kMoveRows + threadIdx.x / (2 * C); j0 < n; j0 += gridDim.x * kRows * kMoveRows) {
+    for (unsigned j0 = blockIdx.x * kRows * kMoveRows + threadIdx.x / (2 * C); j0 < n; j0 += gridDim.x * kRows * kMoveRows) {
         int from[kMoveRows], to[kMoveRows], page[kMoveRows];
         uint4 v[kMoveRows];
 #pragma unroll
         for (int i = 0; i < kMoveRows; i++) {
-            const int j = j0 + i * kRows, dp = j >> bt.page_shift;
+            const unsigned j = j0 + i * kRows, dp = j >> bt.page_shift;
             from[i] = j < n ? from_of[j] : -1;
-            to[i] = j < n && dp < dst_max_pages ? dst_table[(size_t)s * dst_max_pages + dp] : -1;
+            to[i] = j < n && dp < (unsigned)dst_max_pages ? dst_table[(size_t)s * dst_max_pages + dp] : -1;
         }
 #pragma unroll
         for (int i = 0; i < kMoveRows; i++)
@@ -629,8 +630,8 @@ extern "C" int b2_kv_evict_paged(const B2PagedKV* kv, int nkv, int hd, const flo
                            dst_weights, new_len);
     if (e == cudaSuccess && budget > 0) {
         const int rows = kMoveThreads / (2 * (hd / 8)) * kMoveRows;
-        const int want = (budget + rows - 1) / rows;
-        const dim3 grid(want < 4096 ? want : 4096, nkv, kv->n_seqs);
+        const long long want = ((long long)budget + rows - 1) / rows;
+        const dim3 grid((unsigned)(want < 4096 ? want : 4096), nkv, kv->n_seqs);
         e = b2::launch_pdl(hd == 128 ? evict_move_kernel<128> : evict_move_kernel<64>, grid, dim3(kMoveThreads), 0, st, bt,
                            pg, budget, dst_table, dst_max_pages, (const int*)kept, (const int*)new_len);
     }

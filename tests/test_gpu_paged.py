@@ -1117,3 +1117,20 @@ def test_evict_arrays_side_by_side():
     assert new.tolist() == [32, 32] and kept.view(2, 32).tolist() == [ref[0][0], ref[1][0]]
     assert torch.equal(dw.view(torch.float32).view(2, 32),
                        torch.stack([w.view(torch.float32)[s * 100:][kept.view(2, 32)[s].long()] for s in range(2)]))
+
+
+def test_evict_budget_of_any_size():
+    """A budget far beyond the slots there are (rows of kept as long as an int counts) keeps them all."""
+    budget = 2**31 - 1
+    b = Paged([(0, 500, (1,))], 2, 1, 64, 16, extra_pages=40)
+    kept = torch.empty(budget, dtype=torch.int32, device=DEV)
+    kept[:600] = -7
+    dst = torch.tensor([b.spare[:32]], dtype=torch.int32, device=DEV)
+    w, n = torch.rand(1, 1, 500, device=DEV), torch.zeros(1, dtype=torch.int32, device=DEV)
+    bd.check(bd.capi().b2_kv_evict_paged(ctypes.byref(b.kv()), 1, 64, w.data_ptr(), 500, budget, 4, 2**31 - 100, dst.data_ptr(),
+                                         32, kept.data_ptr(), None, n.data_ptr(), stream()), "b2_kv_evict_paged")
+    j = b.slots(0)[0]
+    assert int(n) == 484 and torch.equal(kept[:484], j.int()) and bool((kept[484:600] == -7).all())
+    to = torch.arange(484, device=DEV)
+    for t in (b.k, b.v):
+        assert torch.equal(t[dst[0, to // 16].long(), 0, to % 16], t[b.table[0, j // 16].long(), 0, j % 16])
