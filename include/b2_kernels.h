@@ -308,15 +308,17 @@ int b2_attention_paged_weights(float* weights, const float* prev, long long ldw,
                                int* err, b2_stream_t s);
 
 /* Eviction by accumulated attention weight: of each sequence's mapped slots
- * below kv_len, each kv head keeps the first `sink` slots and the last `recent`
- * slots, and of the rest those of the largest weight (device FP32
- * [n_seqs][nkv][ldw], as b2_attention_paged_weights leaves them; the lowest
- * slots among equal ones, NaN last), `budget` in all or every mapped slot when
- * there are fewer.  Slots from ldw on weigh nothing.  What is kept moves, in slot
+ * below n = kv_len (at most what its table row holds), each kv head keeps those
+ * below `sink` and those from n - recent on, and of the rest those of the largest
+ * weight (device FP32 [n_seqs][nkv][ldw], as b2_attention_paged_weights leaves
+ * them; the lowest slots among equal ones, NaN last), `budget` in all or every
+ * mapped slot when there are fewer.  `sink` and `recent` count slots, mapped or not:
+ * with the first page unmapped, a sink within it keeps nothing.  Slots from ldw on
+ * weigh nothing.  What is kept moves, in slot
  * order, to slots 0, 1, ... of the pages dst_table [n_seqs][dst_max_pages] of the
  * same pool (unmapped entries are left out).  No page of dst_table may be among
  * the sequences' own pages, which stay as they are: they may belong to other
- * sequences too.
+ * sequences too.  Nor may dst_table hold a page twice.
  *   kept         device int   [n_seqs][nkv][budget]  slots kept
  *   dst_weights  device FP32  [n_seqs][nkv][budget]  their weights (may be NULL)
  *   new_len      device int   [n_seqs]               slots kept per kv head

@@ -1134,3 +1134,15 @@ def test_evict_budget_of_any_size():
     to = torch.arange(484, device=DEV)
     for t in (b.k, b.v):
         assert torch.equal(t[dst[0, to // 16].long(), 0, to % 16], t[b.table[0, j // 16].long(), 0, j % 16])
+
+
+def test_evict_sink_and_recent_count_unmapped_slots():
+    """The first and last slots are kept by their place, not as the first and last that are mapped."""
+    b = Paged([(0, 320, (0, 4))], 2, 1, 64, 64, extra_pages=4)  # slots 64 .. 255 are mapped
+    w = torch.arange(320, 0, -1, device=DEV, dtype=torch.float32).view(1, 1, 320)
+    w[0, 0, 64:70], w[0, 0, 250:256] = -1.0, -2.0
+    dst = torch.tensor([b.spare[:3]], dtype=torch.int32, device=DEV)
+    for sink, recent, first, last in ((4, 64, (), ()), (66, 64, (64, 65), ()), (4, 66, (), (254, 255)), (67, 67, (64, 65, 66), (253, 254, 255))):
+        kept, _, n = evict(b, w, 150, sink, recent, dst)
+        rest = [j for j in range(70, 250)][:150 - len(first) - len(last)]
+        assert int(n) == 150 and kept[0, 0].tolist() == [*first, *rest, *last]
