@@ -594,7 +594,12 @@ int launch_long(const WeightParams& p, const B2PagedKV* kv, int dev, int sms, cu
     return 0;
 }
 
-constexpr int kShortRows = 64;
+// (token, head) rows of a kv head up to which the kernel of few rows takes a sequence:
+// it costs a product with every eight rows, the other one a tile of 128 at least.
+// 64 sequences (8 sequences) of 128 to 4096 slots, 8 kv heads, hd 128, two q heads each:
+// 16 tokens, 32 rows, take 121 us (27) here and 140 (32) there; 20 tokens 141 (29) and
+// 142 (32); 32 tokens, 64 rows, 203 (37) and 142 (34).
+constexpr int kShortRows = 32;
 
 }  // namespace
 

@@ -1146,3 +1146,17 @@ def test_evict_sink_and_recent_count_unmapped_slots():
         kept, _, n = evict(b, w, 150, sink, recent, dst)
         rest = [j for j in range(70, 250)][:150 - len(first) - len(last)]
         assert int(n) == 150 and kept[0, 0].tolist() == [*first, *rest, *last]
+
+
+@pytest.mark.parametrize("nq,nkv,qs", [(4, 2, (15, 16, 17, 31, 32, 33)), (16, 1, (1, 2, 3, 4, 5)), (5, 1, (6, 7, 12, 13))])
+def test_weights_around_the_kernels_border(nq, nkv, qs):
+    """Sequences on both sides of where the two kernels divide them, in one call and one by one."""
+    seqs = [(q, 200 + 7 * q, (1,)) for q in qs]
+    b = Paged(seqs, nq, nkv, 128, 32, seed=nq)
+    _, lse = b.attend()
+    ldw = 450
+    check_weights(b, lse, None, b.weigh(lse, None, torch.full((len(seqs), nkv, ldw), 0.0, device=DEV)), ldw, 0.0)
+    for q in qs:
+        one = Paged([(q, 200 + 7 * q, ())], nq, nkv, 128, 32, seed=q)
+        _, lse = one.attend()
+        check_weights(one, lse, None, one.weigh(lse, None, torch.full((1, nkv, ldw), 0.0, device=DEV)), ldw, 0.0)
