@@ -555,8 +555,14 @@ extern "C" int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int
                             "b2_qk_rope_kv_paged: rows must be aligned (qkv 16 bytes, ldqkv %% 4; q16 8 bytes, ldq %% 4) "
                             "and hold every head");
     if (M == 0 || kv->n_seqs == 0) return 0;
+    int dev = 0, sms = 148;
+    cudaGetDevice(&dev);
+    cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
+    // Whole rows once there are more jobs of four heads than warps that the SMs can hold.  32 heads of
+    // 128: 600 rows take 13.3 us as jobs of four heads and 16.4 as rows, 900 15.2 and 16.4, 1200 18.3
+    // and 16.4, 2000 23.2 and 18.4, 7500 58.3 and 41.0 (inputs not in L2).
     const int all = (nq + 2 * nkv + kHeads - 1) / kHeads;
-    const int steps = (long long)M * all > 148 * 64 ? all : 1;  // more than fits the SMs at once
+    const int steps = (long long)M * all > 64ll * sms ? all : 1;
     const long long jobs = (long long)M * ((all + steps - 1) / steps);
     const long long grid = (jobs + kAppendThreads / 32 - 1) / (kAppendThreads / 32);
     if (grid > 0x7fffffffll) return b2_set_error(B2_ERR_INVALID_ARG, "b2_qk_rope_kv_paged: too many rows");
