@@ -4,6 +4,7 @@
 #pragma once
 #include <cuda.h>  // CUtensorMap
 #include <math.h>
+#include <stdlib.h>
 
 #include <atomic>
 
@@ -98,18 +99,29 @@ __device__ __forceinline__ bool mbar_try_wait(uint64_t* bar, uint32_t parity) {
         : "memory");
     return ok != 0;
 }
+// Polls after which a wait gives up (a poll takes 1.5 us: six seconds).  The variable is for tests.
 constexpr int kWaitLimit = 1 << 22;
-// Bounded wait of a whole warp: false, with the CTA's failure flag set, after
-// kWaitLimit polls or once another warp has given up.  The warp polls as one: behind
+inline int wait_limit() {
+    const char* e = getenv("B2_PAGED_POLL_LIMIT");
+    return e ? atoi(e) : kWaitLimit;
+}
+// Bounded wait of a whole warp: false, with the CTA's failure flag failed[0] set, after
+// failed[1] polls or once another warp has given up.  The warp polls as one: behind
 // a loop that its lanes might leave one by one it would have to gather them again.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* failed) {
     for (int it = 0; B2_RARE(!__all_sync(0xffffffffu, mbar_try_wait(bar, parity))); it++) {
-        if (B2_RARE(__any_sync(0xffffffffu, it > kWaitLimit || *failed))) {
-            *failed = 1;
+        if (B2_RARE(__any_sync(0xffffffffu, it > failed[1] || failed[0]))) {
+            failed[0] = 1;
             return false;
         }
     }
     return true;
+}
+// For one thread of a CTA that gave up: the last `depth` of `count` copies (or of groups of
+// them) into a ring of so many barriers have landed.  Bounded again, by the usual limit.
+__device__ __forceinline__ void copies_land(uint64_t* bars, int depth, int count) {
+    for (int i = max(0, count - depth); i < count; i++)
+        for (int it = 0; it <= kWaitLimit && !mbar_try_wait(&bars[i % depth], (i / depth) & 1); it++) {}
 }
 __device__ __forceinline__ void tma_load_5d(void* dst, const CUtensorMap* map, int x, int row, int half, int head,
                                             int page, uint64_t* bar) {
@@ -223,6 +235,7 @@ struct AttnParams {
     float* long_part;       // their pieces
     int long_ctas;          // CTAs of the long kernel (0: none launched)
     int* err;
+    int limit;              // polls of a wait
 };
 
 // The short kernel's CTAs begin beside the long kernel, which their own wait would

@@ -96,7 +96,9 @@ struct ShortSmem {
     uint64_t q_full[Short<HD, NT>::kQ], q_empty[Short<HD, NT>::kQ];
     Seg seg[Short<HD, NT>::kQ];
     int mapped[Short<HD, NT>::kStages];  // bit w: the 16 slots of warp w are mapped
-    int failed, last;
+    volatile int failed[2];  // some warp's wait ran out; polls after which one does
+    volatile int copied, q_copied;  // blocks and Q tiles that the producer has asked for
+    int last;
     int pre[B2_PAGED_MAX_SEQS + 1];
 };
 
@@ -318,7 +320,9 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
             mbar_init(&sm.q_full[i], 1);
             mbar_init(&sm.q_empty[i], 4);
         }
-        sm.failed = 0;
+        sm.failed[0] = 0;
+        sm.failed[1] = p.limit;
+        sm.copied = sm.q_copied = 0;
         mbar_init_fence();
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tv) : "memory");
@@ -348,7 +352,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
     const int per = max(kMinBlocks, cdiv(W, gridDim.x));
     const int x0 = stretch_start(p, sm.pre, W, per, blockIdx.x), x1 = stretch_start(p, sm.pre, W, per, blockIdx.x + 1);
     const int page_rows = 1 << p.bt.page_shift, box_rows = min(page_rows, kBlk);
-    volatile int* failed = &sm.failed;
+    volatile int* failed = sm.failed;
 
     if (warp == 4) {  // producer: lane i copies the i-th box of a stage and the i-th row of a Q tile
         const int boxes = kBlk / box_rows, box_bytes = box_rows * HD * 2;
@@ -369,6 +373,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
             if (!ok) break;
             if (lane == 0) {
                 sm.seg[qb] = g;
+                sm.q_copied = n + 1;
                 mbar_expect_tx(&sm.q_full[qb], rows * HD * 2);
             }
             __syncwarp();
@@ -391,6 +396,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
                     int bits = 0;
                     for (int w = 0; w < 4; w++) bits |= (have >> (w * 16 / box_rows) & 1) << w;
                     sm.mapped[st] = bits;
+                    sm.copied = k + 1;
                     mbar_expect_tx(&sm.full[st], __popc(have) * 2 * box_bytes);
                 }
                 __syncwarp();
@@ -402,15 +408,12 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
                 }
             }
         }
-        if (!ok && lane == 0) {
+        __syncthreads();  // no warp waits for copies any more
+        if (*failed && lane == 0) {
+            // some warp may have given up with copies in flight, which the CTA must not end before
             atomicExch(p.err, 1);
-            // let the copies in flight land (again bounded) before the CTA ends
-            for (int i = max(0, k - C::kStages); i < k; i++)
-                for (int it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
-            for (int i = max(0, n + 1 - C::kQ); i <= n; i++)
-                for (int it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.q_full[i % C::kQ], (i / C::kQ) & 1)) break;
+            copies_land(sm.full, C::kStages, sm.copied);
+            copies_land(sm.q_full, C::kQ, sm.q_copied);
         }
         return;
     }
@@ -712,7 +715,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
         }
         sync4();  // the merge area is free for the next tile
     }
-    if (!ok && lane == 0) atomicExch(p.err, 1);
+    __syncthreads();
     if (p.long_ctas) {
         b2::pdl_wait();
         // (not over sm.pre: nothing orders a CTA without a tile behind its producer's reads of that)
@@ -809,7 +812,7 @@ extern "C" int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q
     AttnParams p{make_batch(kv, M), reinterpret_cast<const __half*>(q16), ldq, reinterpret_cast<__half*>(out16), lse, max_q,
                  nq, nkv, G, kShortRows, reinterpret_cast<int*>(w),
                  reinterpret_cast<float*>(w + kCounterBytes + kCutBytes), reinterpret_cast<Cut*>(w + kCounterBytes),
-                 reinterpret_cast<float*>(w + kCounterBytes + kCutBytes + short_part_bytes(sms, hd)), 0, err};
+                 reinterpret_cast<float*>(w + kCounterBytes + kCutBytes + short_part_bytes(sms, hd)), 0, err, wait_limit()};
     // the line's length when every sequence fills its table: what the kernel's 32-bit places must hold
     const long long cap = ((long long)kv->max_pages * kv->page_size + kBlk - 1) / kBlk;
     const long long tiles = (long long)kv->n_seqs * kShortRows;

@@ -75,8 +75,9 @@ struct Smem {
     uint64_t s_full[2][2], p_ready[2][2], o_done[2][2];
     uint64_t o_free[2], drain[2];
     uint32_t tmem;
-    int failed;
-    int issued;      // blocks that the producer has asked for
+    volatile int failed[2];  // some warp's wait ran out; polls after which one does
+    volatile int issued;     // blocks that the producer has asked for
+    volatile int q_issued;   // segments whose Q it has asked for
     int skip[2][2];  // [tile][buffer]: block count of a block whose product with V the softmax did itself
     unsigned last_bad[16];  // entry (block count % 16): the count, and 1 + the last slot whose V is not finite
     int mapped[16];  // bit w of entry (block count % 16): slots 16 w .. 16 w + 15 are mapped
@@ -161,7 +162,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     Smem<HD>& sm = *reinterpret_cast<Smem<HD>*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const Batch& bt = p.a.bt;
-    volatile int* failed = &sm.failed;
+    volatile int* failed = sm.failed;
     if (threadIdx.x == 0) {
         for (int i = 0; i < C::kStages; i++) {
             mbar_init(&sm.full[i], 1);
@@ -178,8 +179,9 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
             mbar_init(&sm.o_free[t], 4);
         }
-        sm.failed = 0;
-        sm.issued = 0;
+        sm.failed[0] = 0;
+        sm.failed[1] = p.a.limit;
+        sm.issued = sm.q_issued = 0;
         for (int i = 0; i < 4; i++) sm.skip[i >> 1][i & 1] = -1;
         for (int i = 0; i < 16; i++) sm.last_bad[i] = ~0u;
         mbar_init_fence();
@@ -239,7 +241,10 @@ __global__ void __launch_bounds__(kThreads, 1)
                 if (seg) ok = warp_wait(&sm.q_empty, (seg - 1) & 1, failed);
                 if (!ok) break;
                 const int tiles = g.tok1 ? 2 : 1, rows = p.T * p.a.G;
-                if (lane == 0) mbar_expect_tx(&sm.q_full, tiles * rows * HD * 2);
+                if (lane == 0) {
+                    mbar_expect_tx(&sm.q_full, tiles * rows * HD * 2);
+                    sm.q_issued = seg + 1;
+                }
                 __syncwarp();
                 if (lane < tiles * C::kHalves) {
                     const int t = lane / C::kHalves, h = lane % C::kHalves;
@@ -263,7 +268,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                         for (int w = 0; w < kBlk / 16; w++) bits |= (have >> (w * 16 / box_rows) & 1) << w;
                         sm.mapped[n & 15] = bits;
                         mbar_expect_tx(&sm.full[st], 2 * C::kTile);
-                        *(volatile int*)&sm.issued = n + 1;
+                        sm.issued = n + 1;
                     }
                     __syncwarp();
                     if (lane < 2 * per_kv)
@@ -271,13 +276,6 @@ __global__ void __launch_bounds__(kThreads, 1)
                                     page >= 0 ? page : bt.n_pages, &sm.full[st]);
                 }
             }
-            if (!ok && lane == 0)  // let the copies in flight land (bounded) before the CTA ends
-                for (int i = max(0, n - C::kStages); i < n; i++)
-                    for (int it = 0; it <= kWaitLimit; it++)
-                        if (mbar_try_wait(&sm.full[i % C::kStages], (i / C::kStages) & 1)) break;
-            if (!ok && lane == 0 && seg)
-                for (int it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.q_full, (seg - 1) & 1)) break;
         } else if (warp < 11) {
             // ── tensor cores, for tile t ──
             constexpr uint32_t id_s = idesc_f16(128, kBlk, false), id_o = idesc_f16(128, HD, true);
@@ -344,11 +342,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     umma_commit(&sm.empty[st], lead);
                 }
             }
-            if (!ok) {  // nothing of the tensor cores may be left running
-                umma_commit(&sm.drain[t], lead);
-                for (int it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.drain[t], 0)) break;
-            }
+            umma_commit(&sm.drain[t], lead);  // the CTA ends behind its products and their arrivals
+            __syncwarp();
+            copies_land(&sm.drain[t], 1, 1);
         } else {
             // ── the last slot of each block that some rows may not see whose V is not finite ──
             // (a stage of such a block is not given back before the softmax has this)
@@ -362,9 +358,9 @@ __global__ void __launch_bounds__(kThreads, 1)
                     const int k = n + b - b0, from = max(0, seen_all - b * kBlk), to = min(kBlk, len - b * kBlk);
                     // This warp waits for few of a stage's phases, so it first has to know that the one it
                     // means has begun.  (The limit starts again with every block: it may be far away.)
-                    for (int it = 0, was = 0, now; (now = *(volatile int*)&sm.issued) <= k && ok; it++) {
+                    for (int it = 0, was = 0, now; (now = sm.issued) <= k && ok; it++) {
                         if (now != was) was = now, it = 0;
-                        if (it > kWaitLimit || *failed) *failed = 1, ok = false;
+                        if (it > failed[1] || failed[0]) failed[0] = 1, ok = false;
                         __nanosleep(32);
                     }
                     ok = __all_sync(0xffffffffu, ok) && warp_wait(&sm.full[k % C::kStages], (k / C::kStages) & 1, failed);
@@ -449,7 +445,7 @@ __global__ void __launch_bounds__(kThreads, 1)
                     if (b >= edge_from && j0 < len) {
                         unsigned w = 0;
                         for (int it = 0; ok && ((w = *(volatile unsigned*)&sm.last_bad[n & 15]) >> 8) != (n & 0xffffffu); it++)
-                            if (it > kWaitLimit || *failed) *failed = 1, ok = false;
+                            if (it > failed[1] || failed[0]) failed[0] = 1, ok = false;
                         ok = __all_sync(0xffffffffu, ok);
                         by_hand = ok && uniform((int)(w & 255)) > max(0, seen_all - j0);
                     }
@@ -615,10 +611,20 @@ __global__ void __launch_bounds__(kThreads, 1)
             }
         }
         if (threadIdx.x == 0 && !owns) p.a.cuts[blockIdx.x] = Cut{0, 0, 0, 0};
+        tmem_wait_ld();  // (a wait that ran out may have left a load on its way)
+        tmem_wait_st();
     }
-    if (!ok && lane == 0) atomicExch(p.a.err, 1);
     tc_fence_before();
     __syncthreads();
+    if (B2_RARE(*failed)) {
+        // Some warp gave up: the CTA must not end before the copies that it has asked for have landed.
+        if (threadIdx.x == 0) atomicExch(p.a.err, 1);
+        if (warp == 8 && lane == 0) {
+            copies_land(sm.full, C::kStages, sm.issued);
+            copies_land(&sm.q_full, 1, sm.q_issued);
+        }
+        __syncthreads();
+    }
     if (warp == 9) {
         tc_fence_after();
         tmem_free512(tmem);

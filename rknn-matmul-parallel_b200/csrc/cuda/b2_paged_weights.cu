@@ -26,6 +26,7 @@ struct WeightParams {
     long long ldw;
     int short_rows;  // sequences with at most this many (token, head) rows per kv head are the short kernel's
     int* err;
+    int limit;       // polls of a wait
 };
 
 // ─── few rows per sequence ───
@@ -180,7 +181,8 @@ struct LongSmem {
     uint64_t sum_full[2], sum_free[2];
     uint64_t drain;
     uint32_t tmem;
-    int failed;
+    volatile int failed[2];          // some warp's wait ran out; polls after which one does
+    volatile int k_issued, q_issued; // units whose K, and Q tiles, that the producer has asked for
     int pre[B2_PAGED_MAX_SEQS + 1];
 };
 
@@ -231,8 +233,8 @@ __device__ __forceinline__ bool cluster_wait(uint64_t* bar, uint32_t parity, vol
             : "r"(smem_u32(bar)), "r"(parity)
             : "memory");
         if (__all_sync(0xffffffffu, ok)) return true;
-        if (__any_sync(0xffffffffu, it > kWaitLimit || *failed)) {
-            *failed = 1;
+        if (__any_sync(0xffffffffu, it > failed[1] || failed[0])) {
+            failed[0] = 1;
             return false;
         }
     }
@@ -247,7 +249,7 @@ __global__ void __launch_bounds__(kLongThreads, 1)
     extern __shared__ unsigned char smem_raw[];
     Sm& sm = *reinterpret_cast<Sm*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~(uintptr_t)1023);
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    volatile int* failed = &sm.failed;
+    volatile int* failed = sm.failed;
     if (threadIdx.x == 0) {
         for (int i = 0; i < 2; i++) {
             for (int t = 0; t < 2; t++) {
@@ -263,7 +265,9 @@ __global__ void __launch_bounds__(kLongThreads, 1)
         mbar_init(&sm.k_full, 1);
         mbar_init(&sm.k_empty, 1);
         mbar_init(&sm.drain, 1);
-        sm.failed = 0;
+        sm.failed[0] = 0;
+        sm.failed[1] = p.limit;
+        sm.k_issued = sm.q_issued = 0;
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tq) : "memory");
         asm volatile("prefetch.tensormap [%0];" ::"l"(&tk) : "memory");
     }
@@ -349,7 +353,10 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             if (nu) ok = warp_wait(&sm.k_empty, (nu - 1) & 1, failed);
             if (!ok) break;
             nu++;
-            if (lane == 0) mbar_expect_tx(&sm.k_full, 2 * Sm::kTile);
+            if (lane == 0) {
+                mbar_expect_tx(&sm.k_full, 2 * Sm::kTile);
+                sm.k_issued = nu;
+            }
             __syncwarp();
             if (box < boxes)
 #pragma unroll
@@ -369,19 +376,15 @@ __global__ void __launch_bounds__(kLongThreads, 1)
                 none = __any_sync(0xffffffffu, none);
                 if (lane == 0) sm.none[nq & 15] = none;
                 __syncwarp();
-                if (lane == 0) mbar_expect_tx(&sm.q_full[qb], T * p.G * HD * 2);
+                if (lane == 0) {
+                    mbar_expect_tx(&sm.q_full[qb], T * p.G * HD * 2);
+                    sm.q_issued = nq + 1;
+                }
                 __syncwarp();
                 if (lane < kHalves)
                     tma_load_5d(sm.q[qb] + lane * 16384, &tq, 0, 0, u.sq.row0 + i * T, lane, u.g, &sm.q_full[qb]);
                 if (i + S < tiles) load_lse(i + S);
             }
-        }
-        if (!ok && lane == 0) {  // let the copies in flight land (bounded) before the CTA ends
-            for (int it = 0; nu && it <= kWaitLimit; it++)
-                if (mbar_try_wait(&sm.k_full, (nu - 1) & 1)) break;
-            for (int i = max(0, nq - Sm::kQStages); i < nq; i++)
-                for (int it = 0; it <= kWaitLimit; it++)
-                    if (mbar_try_wait(&sm.q_full[i % Sm::kQStages], (i / Sm::kQStages) & 1)) break;
         }
     } else if (warp == 9) {
         // ── tensor cores ──
@@ -419,11 +422,9 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             }
             umma_commit(&sm.k_empty, lead);
         }
-        if (!ok) {  // nothing of the tensor cores may be left running
-            umma_commit(&sm.drain, lead);
-            for (int it = 0; it <= kWaitLimit; it++)
-                if (mbar_try_wait(&sm.drain, 0)) break;
-        }
+        umma_commit(&sm.drain, lead);  // the CTA ends behind its products and their arrivals
+        __syncwarp();
+        copies_land(&sm.drain, 1, 1);
     } else {
         // ── exponentials of K tile t: thread = slot ──
         const int t = warp >> 2, slot = threadIdx.x;
@@ -520,9 +521,17 @@ __global__ void __launch_bounds__(kLongThreads, 1)
             }
         }
     }
-    if (!ok && lane == 0) atomicExch(p.err, 1);
     tc_fence_before();
     __syncthreads();
+    if (B2_RARE(*failed)) {
+        // Some warp gave up: the CTA must not end before the copies that it has asked for have landed.
+        if (threadIdx.x == 0) atomicExch(p.err, 1);
+        if (warp == 8 && lane == 0) {
+            copies_land(&sm.k_full, 1, sm.k_issued);
+            copies_land(sm.q_full, Sm::kQStages, sm.q_issued);
+        }
+        __syncthreads();
+    }
     // the others may still write to or arrive at this CTA's shared memory
     if (cluster > 1) asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
     if (warp == 9) {
@@ -626,7 +635,7 @@ extern "C" int b2_attention_paged_weights(float* weights, const float* prev, lon
     if (max_q > M) max_q = M;
     const WeightParams p{make_batch(kv, M), kv->k_pages, kv->page_stride, kv->head_stride, kv->row_stride,
                          reinterpret_cast<const __half*>(q16), ldq, lse, max_q, nq, nkv, nq / nkv, weights, prev, ldw,
-                         kShortRows, err};
+                         kShortRows, err, wait_limit()};
     if ((long long)max_q * p.G > kShortRows) {
         rc = hd == 128 ? launch_long<128>(p, kv, dev, sms, (cudaStream_t)s) : launch_long<64>(p, kv, dev, sms, (cudaStream_t)s);
         if (rc) return rc;

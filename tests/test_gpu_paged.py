@@ -1160,3 +1160,53 @@ def test_weights_around_the_kernels_border(nq, nkv, qs):
         one = Paged([(q, 200 + 7 * q, ())], nq, nkv, 128, 32, seed=q)
         _, lse = one.attend()
         check_weights(one, lse, None, one.weigh(lse, None, torch.full((1, nkv, ldw), 0.0, device=DEV)), ldw, 0.0)
+
+
+# ── waits that run out ──
+
+
+@pytest.mark.parametrize("limit", [-1, 0, 2, 8])
+@pytest.mark.parametrize("hd,seqs", [(128, [(1, 3000, ())] * 40), (64, [(2, 900 + 50 * i, (1,)) for i in range(30)]),
+                                     (128, [(300, 2300, ()), (70, 900, ()), (300, 300, ())]),
+                                     (64, [(500, 1500, ()), (1, 2000, ()), (90, 90, ()), (3, 700, ())])])
+def test_waits_that_run_out(hd, seqs, limit, monkeypatch):
+    """With a limit of a few polls ordinary waits run out: the kernels return by themselves, err tells it, what is not
+    theirs stays, and with work and err zeroed the next call is right.  A call whose waits were all short enough is
+    right too."""
+    b = Paged(seqs, 8, 4, hd, 32, seed=hd, tail=2)
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    ldw = max(n for _, n, _ in seqs)
+    w = b.weigh(lse, None, torch.full((len(seqs), 4, ldw), 7.0, device=DEV))
+    pools = [t.clone() for t in (b.k, b.v)]
+    gave_up = [0, 0]
+    for _ in range(3):
+        torch.full((256 << 20,), 1, dtype=torch.uint8, device=DEV)  # K and V out of L2
+        monkeypatch.setenv("B2_PAGED_POLL_LIMIT", str(limit))
+        o2, l2 = b.attend()
+        torch.cuda.synchronize()
+        if b.err.item():
+            gave_up[0] += 1
+            assert bool((o2[b.rows:] == 7).all()) and bool((l2[b.rows:] == 7).all())
+        else:
+            assert torch.equal(o2, out) and torch.equal(l2, lse)
+        b.work.zero_(), b.err.zero_()
+        torch.full((256 << 20,), 1, dtype=torch.uint8, device=DEV)
+        w2 = b.weigh(lse, None, torch.full_like(w, 7.0))
+        torch.cuda.synchronize()
+        if b.err.item():
+            gave_up[1] += 1
+            for s, (_, n, _) in enumerate(seqs):
+                assert bool((w2[s, :, n:] == 7).all())
+        else:
+            assert torch.equal(w2, w)
+        b.err.zero_()
+        monkeypatch.delenv("B2_PAGED_POLL_LIMIT")
+        o2, l2 = b.attend()
+        assert torch.equal(o2, out) and torch.equal(l2, lse)
+        assert torch.equal(b.weigh(lse, None, torch.full_like(w, 7.0)), w)
+        assert b.err.item() == 0 and not b.work[:4096].any()
+    for t, e in zip((b.k, b.v), pools):
+        assert torch.equal(t.nan_to_num(9.0), e.nan_to_num(9.0))
+    if limit < 0:  # a poll takes 1.5 us, and the attention's first copies from HBM take longer
+        assert gave_up[0]
