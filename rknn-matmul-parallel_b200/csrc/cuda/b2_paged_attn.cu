@@ -727,9 +727,9 @@ __global__ void __launch_bounds__(kThreads, 2) attn_short_kernel(const __grid_co
 constexpr int kMaxGroup = 16;
 // (token, head) rows of a kv head up to which this file's kernel takes a sequence: one
 // tile, so that K and V are read once.  Two q heads each, 8 kv heads, hd 128, 128 to
-// 4096 slots: 8 tokens, 16 rows, take 136 us for 64 sequences (40 for 8, 350 for 200)
-// here and 198 (54, 507) in the chunk kernel; 9 tokens, 18 rows, as two tiles 215 (45,
-// 615) here and 202 (54, 513) there, 16 tokens 225 (47, 643) and 204 (56, 519).
+// 4096 slots: 8 tokens, 16 rows, take 83 us for 64 sequences (30 for 8, 205 for 200)
+// here and 137 (39, 370) in the chunk kernel; 9 tokens, as two tiles, 138 (32, 382) here
+// and 138 (38, 371) there, 16 tokens 144 (32, 393) and 142 (38, 372).
 constexpr int kShortRows = 16;
 constexpr size_t kCounterBytes = kCounters * sizeof(int), kCutBytes = kMaxLongCtas * sizeof(Cut);
 

@@ -560,7 +560,7 @@ extern "C" int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int
     cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev);
     // Whole rows once there are more jobs of four heads than warps that the SMs can hold.  32 heads of
     // 128: 600 rows take 13.3 us as jobs of four heads and 16.4 as rows, 900 15.2 and 16.4, 1200 18.3
-    // and 16.4, 2000 23.2 and 18.4, 7500 58.3 and 41.0 (inputs not in L2).
+    // and 16.4, 2000 23.2 and 18.4, 7500 58.3 and 41.0 (launch by launch, inputs not in L2).
     const int all = (nq + 2 * nkv + kHeads - 1) / kHeads;
     const int steps = (long long)M * all > 64ll * sms ? all : 1;
     const long long jobs = (long long)M * ((all + steps - 1) / steps);

@@ -604,11 +604,11 @@ int launch_long(const WeightParams& p, const B2PagedKV* kv, int dev, int sms, cu
 }
 
 // (token, head) rows of a kv head up to which the kernel of few rows takes a sequence:
-// it costs a product with every eight rows, the other one a tile of 128 at least.
-// 64 sequences (8 sequences) of 128 to 4096 slots, 8 kv heads, hd 128, two q heads each:
-// 16 tokens, 32 rows, take 121 us (27) here and 140 (32) there; 20 tokens 141 (29) and
-// 142 (32); 32 tokens, 64 rows, 203 (37) and 142 (34).
-constexpr int kShortRows = 32;
+// it costs a product with every eight rows, the other one a tile of 128 at least.  Two q
+// heads each, 8 kv heads, hd 128, 128 to 4096 slots: 16 tokens, 32 rows, take 71 us for
+// 64 sequences (11 for 8, 186 for 200) here and 83 (17, 214) there; 20 tokens 84 (13, 221)
+// and 83 (17, 215); 24 tokens 97 (14, 256) and 83 (17, 216).
+constexpr int kShortRows = 40;
 
 }  // namespace
 

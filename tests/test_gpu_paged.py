@@ -1148,7 +1148,7 @@ def test_evict_sink_and_recent_count_unmapped_slots():
         assert int(n) == 150 and kept[0, 0].tolist() == [*first, *rest, *last]
 
 
-@pytest.mark.parametrize("nq,nkv,qs", [(4, 2, (15, 16, 17, 31, 32, 33)), (16, 1, (1, 2, 3, 4, 5)), (5, 1, (6, 7, 12, 13))])
+@pytest.mark.parametrize("nq,nkv,qs", [(4, 2, (15, 16, 17, 20, 21, 31, 32, 33)), (16, 1, (1, 2, 3, 4, 5)), (5, 1, (6, 7, 8, 9, 13))])
 def test_weights_around_the_kernels_border(nq, nkv, qs):
     """Sequences on both sides of where the two kernels divide them, in one call and one by one."""
     seqs = [(q, 200 + 7 * q, (1,)) for q in qs]
