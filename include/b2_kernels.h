@@ -265,7 +265,8 @@ typedef struct {
  * evicted.  A row whose position is outside [0, max_pos) is left out entirely;
  * one whose slot is not mapped only writes q16.  qkv: device FP32 [M][ldqkv] =
  * [q (nq*hd) | k (nkv*hd) | v (nkv*hd)], read only; 16-byte aligned, ldqkv a
- * multiple of 4, ldq of 4. */
+ * multiple of 4, ldq of 4.  q16 must not overlap what is read, and a page that
+ * new rows go to belongs to one sequence (pages of earlier slots may be shared). */
 int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int M, int nq, int nkv, int hd,
                         const float* q_norm_w, const float* k_norm_w, float eps, const float* cos_tab,
                         const float* sin_tab, int max_pos, int rope_style, const int* pos, const B2PagedKV* kv,
@@ -276,9 +277,11 @@ int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int
  * 1 / sqrtf(hd).  q16: device FP16 [M][ldq] (first nq*hd), out16: device FP16
  * [M][nq*hd], lse (may be NULL): device FP32 [M][nq], the natural logarithm of
  * the row's sum of exponentials.  A row that sees no slot gives zeros and
- * -infinity.  max_q: no sequence brings more rows than this (M is always
- * right; a decode step passes 1); a sequence's rows past the first max_q are
- * left as they are.
+ * -infinity.  max_q: no sequence brings more rows than this; a sequence's rows past
+ * the first max_q are left as they are.  M is always right, but a call whose max_q
+ * times nq / nkv passes 16 launches the kernel for chunks as well, whether a
+ * sequence needs it or not: 76 us instead of 55 for a decode step of 64 sequences,
+ * so a decode step passes 1.
  * out16 and lse must not overlap what is read.
  * Sums and the softmax are FP32; the softmax weights are rounded to FP16 for
  * the product with V.  Whatever K and V hold at slots that a row does not see
@@ -289,7 +292,11 @@ int b2_qk_rope_kv_paged(uint16_t* q16, int ldq, const float* qkv, int ldqkv, int
  * shape one after the other, but not calls that may overlap.  A copy that does
  * not arrive within the wait limit sets *err (device int) to 1 and leaves rows
  * unfinished; zero work again after that, and after a call that returned
- * B2_ERR_CUDA.  q16 16-byte aligned, ldq a multiple of 8. */
+ * B2_ERR_CUDA.  q16 16-byte aligned, ldq a multiple of 8.
+ * Refused, as if every sequence filled its row of the table: with B = max_pages *
+ * page_size / 64, G = nq / nkv and T = 128 / G (rounded down), calls of 2^31 - 65536
+ * blocks or more by min(M, 16 n_seqs) nkv B, or where max_q G > 16 by
+ * (M / 2T + n_seqs) nkv B. */
 size_t b2_attention_paged_workspace(int n_seqs, int max_q, int nq, int nkv, int hd);
 int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq, int M, int max_q, int nq, int nkv,
                        int hd, const B2PagedKV* kv, void* work, int* err, b2_stream_t s);
@@ -299,10 +306,14 @@ int b2_attention_paged(uint16_t* out16, float* lse, const uint16_t* q16, int ldq
  *     weights[q][g][j] = prev[q][g][j] + sum over the rows i that see j and the
  *                        q heads h of g of exp(score(i, h, j) - lse[i][h])
  * with q16, ldq, max_q and lse as given to and by b2_attention_paged; a row
- * whose lse is -infinity gives nothing.  weights and prev: device FP32
- * [n_seqs][nkv][ldw]; prev may be NULL (zeros) or weights itself.  Slots from
+ * whose lse is -infinity gives nothing, whatever its q holds.  weights and prev:
+ * device FP32 [n_seqs][nkv][ldw]; prev may be NULL (zeros) or weights itself, and
+ * otherwise shares no entry with it.  Slots from
  * kv_len[q] or ldw on are left as they are.  FP32 sums in an order that the
- * call's shapes and lengths fix.  err as in b2_attention_paged. */
+ * call's shapes and lengths fix.  err as in b2_attention_paged; the kernel for
+ * chunks is launched where max_q nq / nkv passes 40 (a decode step of 64 sequences
+ * takes 54 us instead of 33 with it).  Refused: n_seqs nkv max_pages page_size / 128
+ * of 2^31 - 65536 or more. */
 int b2_attention_paged_weights(float* weights, const float* prev, long long ldw, const uint16_t* q16, int ldq,
                                const float* lse, int M, int max_q, int nq, int nkv, int hd, const B2PagedKV* kv,
                                int* err, b2_stream_t s);

@@ -1210,3 +1210,24 @@ def test_waits_that_run_out(hd, seqs, limit, monkeypatch):
         assert torch.equal(t.nan_to_num(9.0), e.nan_to_num(9.0))
     if limit < 0:  # a poll takes 1.5 us, and the attention's first copies from HBM take longer
         assert gave_up[0]
+
+
+@pytest.mark.parametrize("q", [1, 5, 80])
+def test_pages_that_sequences_share(q):
+    """A common prefix: four sequences whose tables begin with the same pages, each with rows of its own behind."""
+    b = Paged([(q, 160 + q + 9 * i, ()) for i in range(4)], 4, 2, 64, 32, seed=q, extra_pages=20)
+    b.table[1:, :5] = b.table[0, :5]
+    out, lse = b.attend()
+    check_attention(b, out, lse)
+    ldw = 200 + q
+    w = b.weigh(lse, None, torch.zeros(4, 2, ldw, device=DEV))
+    check_weights(b, lse, None, w, ldw, 0.0)
+    dst = torch.tensor(b.spare[:16], dtype=torch.int32, device=DEV).view(4, 4)
+    before = [t.clone() for t in (b.k, b.v)]
+    kept, _, n = evict(b, w, 100, 4, 20, dst)
+    for s, heads in enumerate(evict_reference(b, w, 100, 4, 20)):
+        for h, js in enumerate(heads):
+            assert int(n[s]) == 100 and kept[s, h].tolist() == js
+            j, to = torch.tensor(js, device=DEV), torch.arange(100, device=DEV)
+            for t, e in zip((b.k, b.v), before):
+                assert torch.equal(t[dst[s, to // 32].long(), h, to % 32], e[b.table[s, j // 32].long(), h, j % 32])

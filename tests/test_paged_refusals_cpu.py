@@ -153,3 +153,13 @@ W, K = 2 * 8 * 256 * 4, 2 * 8 * 64 * 4  # bytes of weights; of kept and of dst_w
 def test_evict_refuses_overlap(bad):
     assert evict_at(**bad) == -1
     assert b"overlaps" in bd.capi().b2_last_error()
+
+
+def test_blocks_of_work_in_one_call():
+    """Products of rows, heads and table width that the kernels' 32-bit places could not hold."""
+    wide = cache(n_seqs=1024, max_pages=16384)  # tables of a million slots: 2^14 blocks of 64
+    assert attend(kv=wide, M=16384, max_q=1) == -1 and b"blocks of work" in bd.capi().b2_last_error()
+    assert attend(kv=cache(n_seqs=1, max_pages=1 << 24), M=1 << 20, max_q=1 << 20) == -1
+    assert b"blocks of work" in bd.capi().b2_last_error()
+    assert weigh(kv=cache(n_seqs=1024, max_pages=1 << 19)) == -1
+    assert b"blocks of work" in bd.capi().b2_last_error()
