@@ -44,9 +44,9 @@ __device__ __forceinline__ uint32_t movm_t(uint32_t x) {
 // summed in pieces, which the last CTA to arrive merges in the line's order.
 // A boundary near a tile's end moves there.
 //
-// One step of 64 sequences of up to 4096 slots, 8 kv heads, hd 128: 54 us, 0.81
+// One step of 64 sequences of up to 4096 slots, 8 kv heads, hd 128: 55 us, 0.80
 // of the measured copy rate (50 without computing and merging); one step of a
-// context of 200 thousand slots, 2 kv heads: 44 us, 0.71, of which two levels of
+// context of 200 thousand slots, 2 kv heads: 45 us, 0.70, of which two levels of
 // merging 148 pieces of a head take 9.
 //
 // A producer warp walks the stretch: for each tile it copies the Q rows, then

@@ -25,11 +25,12 @@
 // changes no result (the sum carries the same factor).
 //
 // Bound by the two products (4 hd FLOP per row and slot) and, at hd 128 just as
-// much, by the exponentials: 16 per clock and SM.  Those 4096 rows take 491 us,
-// 980 TFLOP/s, 0.59 of a library product's rate; the products and their barriers alone take 468,
-// the softmax without the products 460.  Every fourth exponential by a polynomial
-// instead made it 501: the softmax waits for the order of its steps, not for the
-// exponential unit.
+// much, by the exponentials: 16 per clock and SM.  Those 4096 rows take 566 us (502 at
+// best) called again and again, 850 TFLOP/s, 0.51 of a library product's rate, the SM clock
+// at 1.72 GHz under the power cap; in shorter runs, at a higher clock, 491.  In those the
+// products and their barriers alone took 468, the softmax without the products 460, and
+// every fourth exponential by a polynomial instead 501: the softmax waits for the order of
+// its steps, not for the exponential unit.
 //
 // The work of the call is one line of blocks, cut into equal stretches for the
 // CTAs; pairs that a cut divides leave pieces (maximum, sum, unnormalised O) in

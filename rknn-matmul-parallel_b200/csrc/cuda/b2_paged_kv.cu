@@ -53,8 +53,8 @@ struct PageStrides {
 // squares across the warp.  Bound by HBM: 4 bytes read and 2 written per
 // element.  A warp takes `steps` times kHeads heads of one row, kHeads at a time
 // and the next ones on their way: with many rows a whole row, so that its place
-// and angles are looked up once, with few rows kHeads, so that there are warps.  7600 rows of 32
-// heads, hd 128: 34.7 us, 0.83 of the measured copy rate; 64 rows: 4.0.
+// and angles are looked up once, with few rows kHeads, so that there are warps.  7467 rows of 32
+// heads, hd 128: 35.7 us at 1.78 GHz (33.7 at best), 0.80 of the measured copy rate; 64 rows: 3.9.
 constexpr int kAppendThreads = 128;
 constexpr int kHeads = 4;
 
@@ -83,7 +83,7 @@ __device__ __forceinline__ void load_shared(float (&v)[E], const float* p) {
 
 // The four heads' sums together: two exchanges halve what a lane adds for, so that
 // eight lanes each end with one head, and take its root once.  (One by one: 0.3 us more
-// of 4.3 with 64 rows, 0.5 of 40 with 7600.)
+// of 4.3 with 64 rows, 0.5 of 40 with 7467.)
 template <int HD>
 __device__ __forceinline__ void four_norms(const float (&x)[kHeads][HD / 32], float eps, int lane, float (&norm)[kHeads]) {
     static_assert(kHeads == 4, "two exchanges");
@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kAppendThreads, 7) append_kernel(
     int h0 = (int)(job % per_row) * kHeads * steps;
     const int h_end = min(heads, h0 + kHeads * steps);
     // The norm weights wait in shared memory: in eight registers of every thread they
-    // cost the loads ahead their room (7600 rows: 39.5 us so, 35.8 here).
+    // cost the loads ahead their room (7467 rows: 39.5 us so, 35.8 here).
     __shared__ alignas(16) float nw[2][HD];
     static_assert(kAppendThreads >= HD, "one element per thread");
     if (threadIdx.x < HD) {

@@ -36,8 +36,9 @@ struct WeightParams {
 // The dims of the sum may go in any order as long as K and Q agree, so a lane takes
 // 16 consecutive bytes of its row for two k steps and the fragments come straight
 // from global memory, a row's four lanes reading 64 consecutive bytes.  Everything
-// a block needs is asked for before any of it is used.  64 sequences of 2048 to 4096
-// slots with 8 kv heads, hd 128, take 32.3 us: 0.70 of the measured copy rate.
+// a block needs is asked for before any of it is used.  64 sequences of 128 to 4096
+// slots (70 thousand in all) with 8 kv heads, hd 128, take 32.7 us: 0.69 of the measured
+// copy rate.
 constexpr int kThreads = 128;
 constexpr int kBlk = 128;
 
@@ -151,9 +152,10 @@ __global__ void __launch_bounds__(kThreads, 4) weights_short_kernel(const Weight
 // Q tile brought in once serves both K tiles.  Where there are too few units to
 // go round, S CTAs of a cluster take every S-th Q tile of one; their sums meet in
 // the first one's shared memory and are added in rank order.
-// 2048 rows after 6144, 16 q heads, hd 128: 91 us, where the exponentials alone
-// would fill the unit for 52 and the product takes 37.  (16 warps of half the columns
-// each in place of 8: the same, and 3 to 19 % slower with chunks of 60 to 1000 rows.)
+// 2048 rows after 6144, 16 q heads, hd 128: 97 us at 1.93 GHz, where the exponentials
+// alone would fill the unit for 52 and the product takes 37.  (16 warps of half the columns
+// each in place of 8: the same, and 3 to 19 % slower with chunks of 60 to 1000 rows.
+// Telling tiles with excluded rows apart costs 2 of the 97.)
 //   warp 8      producer: the unit's K tiles, Q tiles and their rows' -lse;
 //   warp 9      tensor cores;
 //   warps 0-3, 4-7   the exponentials of K tile 0 and 1, one slot per thread.
@@ -282,8 +284,8 @@ __global__ void __launch_bounds__(kLongThreads, 1)
     // Units go round the groups of S CTAs and back, as later ones of a sequence cost
     // less.  S: the fewest that give the shortest schedule, a unit costing its Q tiles
     // and about one more for its K tiles, judged by the first group and the last.  Many
-    // rounds are even enough.  (2048 rows after 6144, 8 kv heads: 90 us with two CTAs, 96 with
-    // one, 98 with one and the groups always in the same order.)
+    // rounds are even enough.  (2048 rows after 6144, 8 kv heads, before excluded rows were told
+    // apart: 90 us with two CTAs, 96 with one, 98 with one and the groups always in the same order.)
     const int W = sm.pre[p.bt.n_seqs];
     auto place = [](int round, int c, int n) { return round * n + (round & 1 ? n - 1 - c : c); };
     int S = 1;
