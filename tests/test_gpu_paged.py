@@ -1231,3 +1231,35 @@ def test_pages_that_sequences_share(q):
             j, to = torch.tensor(js, device=DEV), torch.arange(100, device=DEV)
             for t, e in zip((b.k, b.v), before):
                 assert torch.equal(t[dst[s, to // 32].long(), h, to % 32], e[b.table[s, j // 32].long(), h, j % 32])
+
+
+@pytest.mark.parametrize("norms", ["q", "k", "both"])
+@pytest.mark.parametrize("style", [0, 1])
+@pytest.mark.parametrize("nq,nkv,hd,rows", [(16, 8, 128, 1300), (5, 5, 64, 2700), (3, 1, 128, 5000), (7, 1, 64, 30)])
+def test_append_many_rows(nq, nkv, hd, rows, style, norms):
+    """More rows than warps (each takes a whole row then), norm weights of q or of k alone, angle tables at an odd
+    address; K, V and q of every row against the 64-bit form."""
+    b = Paged([(rows // 2, rows // 2 + 40, ()), (1, 900, ()), (rows - rows // 2 - 1, rows + 3, ())], nq, nkv, hd, 32, seed=rows)
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    qkv = torch.randn(b.M, (nq + 2 * nkv) * hd, generator=g, device=DEV) * 2
+    qn, kn = (1 + 0.2 * torch.randn(hd, generator=g, device=DEV) if norms in (n, "both") else None for n in "qk")
+    angle = torch.rand(700, hd // 2, generator=g, device=DEV, dtype=F64) * 6.3
+    tables = []
+    for t in (angle.cos(), angle.sin()):
+        pool = torch.zeros(t.numel() + 1, device=DEV)
+        tables.append(pool[1:].view(700, hd // 2).copy_(t))
+    pos = torch.randint(0, 700, (b.M,), generator=g, device=DEV, dtype=torch.int32)
+    q16 = torch.full((b.M, nq * hd), 7.0, dtype=torch.float16, device=DEV)
+    bd.check(bd.capi().b2_qk_rope_kv_paged(
+        q16.data_ptr(), nq * hd, qkv.data_ptr(), qkv.stride(0), b.M, nq, nkv, hd, None if qn is None else qn.data_ptr(),
+        None if kn is None else kn.data_ptr(), 1e-6, tables[0].data_ptr(), tables[1].data_ptr(), 700, style, pos.data_ptr(),
+        ctypes.byref(b.kv()), stream()), "b2_qk_rope_kv_paged")
+    z, v, mag = rope_reference(b, qkv, qn, kn, *tables, pos, style)
+    tol = U * z.abs() + 16 * 2.0 ** -24 * mag + 2.0 ** -25  # as in test_append
+    assert bool(((q16.to(F64).view(b.M, nq, hd) - z[:, :nq]).abs() <= tol[:, :nq]).all())
+    for s, (q, n, _) in enumerate(b.seqs):
+        j = torch.arange(n - q, n, device=DEV)
+        r = slice(int(b.starts[s]), int(b.starts[s]) + q)
+        at = b.table[s, j // 32].long()
+        assert bool(((b.k[at, :, j % 32].to(F64) - z[r, nq:]).abs() <= tol[r, nq:]).all())
+        assert torch.equal(b.v[at, :, j % 32], v[r].half())
